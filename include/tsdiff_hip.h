@@ -34,7 +34,8 @@
  *     (the forward, sampling-loop, geometry / topology and training entry points run inside "tsd:<name>"
  *     ranges that `rocprofv3 --marker-trace` records; absent a profiler the ranges are no-ops); a process may drive several devices (the device current
  *     at the call is used), one stream per call;
- *   - every tensor at this boundary is fp32; the GEMMs run on the fp32-input MFMA (exact-f32 FMA chains) or, in the
+ *   - every tensor at this boundary is fp32 (the attention-block entry points, tsd_layer_norm_*, tsd_gated_linear_* and
+ *     tsd_graph_attention_*, also take bf16 and f16); the GEMMs run on the fp32-input MFMA (exact-f32 FMA chains) or, in the
  *     inference forward when the batch carries `weights16`, on the f16 MFMA with split operands and fp32 accumulation
  *     (22-bit operands: the fp32 error class, see tsd_pack_weights16); indices at this
  *     boundary are int32 except where the reference surface hands over int64 tensors
@@ -59,6 +60,11 @@ extern "C" {
 #define TSD_ERR_RANGE (-5)       /* tsd_train_backward2 of a split-f16 step (tsd_batch.reserved bit 5) whose forward raised
                                     TSD_STATUS_RANGE: nothing was launched; run tsd_train_forward again without the bit
                                     (same workspace, same loss buffer), then the backward */
+
+/* element types of the attention-block entry points (every other entry point is fp32) */
+#define TSD_F32 0
+#define TSD_BF16 1
+#define TSD_F16 2
 
 #define TSD_EDGE_TILE 32         /* edges per workgroup tile of every per-edge kernel */
 #define TSD_NODE_TILE 16         /* nodes per workgroup tile of the per-node kernels */
@@ -602,6 +608,56 @@ int tsd_dual_score(int32_t num_nodes, const float* eq_local, const float* eq_glo
  *   out[e] = [exp(coeff (d_e - offset_k)^2) for k < K, bond_emb[type_e]]   -> [E, 2K] */
 int tsd_gaussian_edge_encode(int64_t num_edges, int32_t K, float coeff, const float* d, const float* offset,
                              const int64_t* type, const float* bond_emb, float* out, void* stream);
+
+/* ---- an attention block over ragged graphs ---------------------------------------------------------------
+ * Three operators by which the nodes of a graph see each other beside message passing, forward and backward
+ * (tsdiff_amd/block_ops.py: the same as autograd functions; tsdiff_amd/encoder/transformer.py: an encoder of them).
+ * `dtype` (TSD_F32 / TSD_BF16 / TSD_F16) is the type of every tensor that is not declared float or int; sums,
+ * statistics and softmax state are fp32, outputs are rounded once.  f32 products run on the bf16 matrix pipes with
+ * three-plane operands at fp32 accuracy (non-finite f32 operands of the products come out as NaN).  No atomics: the same
+ * bits on every run; no host synchronisation, capturable.
+ *
+ * Layer norm over the last dimension (1 .. 8192):  y = (x - mean) rstd weight + bias, rstd = (var + eps)^-1/2.
+ * x [rows, dim] with row stride ldx, y dense; weight / bias NULL: 1 / 0.  mean, rstd [rows] are what the backward needs
+ * (both NULL: not kept).  Backward: dx dense; dx, dweight, dbias may be NULL; scratch
+ * (tsd_layer_norm_scratch_floats(rows, dim) floats) is needed for dweight / dbias alone. */
+int tsd_layer_norm_fwd(int32_t dtype, int32_t rows, int32_t dim, const void* x, int64_t ldx, const void* weight,
+                       const void* bias, float eps, void* y, float* mean, float* rstd, void* stream);
+size_t tsd_layer_norm_scratch_floats(int32_t rows, int32_t dim);
+int tsd_layer_norm_bwd(int32_t dtype, int32_t rows, int32_t dim, const void* x, int64_t ldx, const void* weight,
+                       const void* dy, int64_t lddy, const float* mean, const float* rstd, void* dx, void* dweight,
+                       void* dbias, float* scratch, size_t scratch_floats, void* stream);
+/* h[rows,out] = act(x w_gate^T + b_gate) * (x w_up^T + b_up); weights [out, in] dense, biases [out] or NULL; `act` as in
+ * tsd_act_fwd (0 .. 3).  The backward computes both projections again; any of its outputs may be NULL (each dense, the
+ * layout of what it is the gradient of); scratch 16-byte aligned, tsd_gated_linear_scratch_floats floats. */
+int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
+                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, void* stream);
+size_t tsd_gated_linear_scratch_floats(int32_t dtype, int32_t rows, int32_t in, int32_t out);
+int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
+                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, const void* dh,
+                         int64_t lddh, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, float* scratch,
+                         size_t scratch_floats, void* stream);
+/* Attention inside the graphs of a ragged batch: query i of graph g (q_ptr[g] <= i < q_ptr[g+1]) attends to the keys
+ * k_ptr[g] .. k_ptr[g+1] whose key_mask byte is not 0 (NULL: all); head h reads key head h / (heads / kv_heads).  Offsets are
+ * int32 [num_graphs + 1], non-decreasing (clamped into the tensors, otherwise unchecked: they stay on the device).  A query
+ * without an open key, or outside of every graph, gives 0 and gradients 0; so do the gradients of masked keys and of keys
+ * outside of every graph, whatever memory holds there.  Strides are in elements, the last dimension is contiguous. */
+#define TSD_ATTENTION_MAX_DIM 128
+typedef struct tsd_attention {
+    int32_t dtype, num_graphs, num_queries, num_keys, heads, kv_heads, dim;
+    float scale;                     /* of the scores: usually dim^-1/2 */
+    const void *q, *k, *v;           /* [num_queries, heads, dim], [num_keys, kv_heads, dim] twice */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const int32_t *q_ptr, *k_ptr;
+    const uint8_t* key_mask;         /* [num_keys] or NULL */
+} tsd_attention;
+size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backward);
+/* out [num_queries, heads, dim] dense; lse [num_queries, heads]: log2 of the sum of 2^(score log2 e), what the backward needs
+ * (NULL: not kept); scratch (16-byte aligned) may be NULL where the query function says 0 floats. */
+int tsd_graph_attention_fwd(const tsd_attention* a, void* out, float* lse, float* scratch, size_t scratch_floats, void* stream);
+/* dq, dk, dv dense in the layouts of q, k, v; do_row / do_head: strides of dout */
+int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float* lse, const void* dout, int64_t do_row,
+                            int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream);
 
 #ifdef __cplusplus
 }

@@ -115,6 +115,13 @@ class Batch(C.Structure):
     ]
 
 
+class Attention(C.Structure):  # tsd_attention
+    _fields_ = [(k, C.c_int32) for k in ("dtype", "num_graphs", "num_queries", "num_keys", "heads", "kv_heads", "dim")] + [
+        ("scale", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p)] + [
+        (k, C.c_int64) for k in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + [
+        ("q_ptr", C.c_void_p), ("k_ptr", C.c_void_p), ("key_mask", C.c_void_p)]
+
+
 class Work(C.Structure):
     """tsd_work"""
     _fields_ = [(k, C.c_double) for k in ("flops_edge_embed", "flops_blocks", "flops_pair_output", "flops_other",
@@ -205,6 +212,19 @@ SIGNATURES = {
                                    _P, _P, _P]),
     "tsd_embedding_renorm": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, C.c_float, _P, _P, _P]),
     "tsd_dual_score": (C.c_int, [C.c_int32, _P, _P, C.c_float, C.c_float, C.c_float, _P, _P]),
+    "tsd_layer_norm_fwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, C.c_float, _P, _P, _P, _P]),
+    "tsd_layer_norm_scratch_floats": (C.c_size_t, [C.c_int32, C.c_int32]),
+    "tsd_layer_norm_bwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, _P, _P,
+                                     _P, C.c_size_t, _P]),
+    "tsd_gated_linear_fwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P,
+                                       _P, _P]),
+    "tsd_gated_linear_scratch_floats": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "tsd_gated_linear_bwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P,
+                                       _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "tsd_graph_attention_scratch_floats": (C.c_size_t, [C.POINTER(Attention), C.c_int32]),
+    "tsd_graph_attention_fwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_size_t, _P]),
+    "tsd_graph_attention_bwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, C.c_size_t,
+                                          _P]),
     "tsd_sampler_plan_create": (C.c_int, [_CFG, C.POINTER(Batch), C.c_int32, C.c_float, C.c_float, _P, _P, _P,
                                           C.POINTER(_P)]),
     "tsd_sampler_plan_run": (C.c_int, [_P, C.c_int32, C.POINTER(RunArgs), C.c_int32, _P]),

@@ -1,0 +1,264 @@
+// block_tile.hpp -- element types, operand tiles and the MFMA step shared by the kernels of an attention block
+// (kernels_gated.hip, kernels_attention.hip): f32, bf16 and f16 tensors, fp32 accumulation everywhere.
+//
+// One matrix instruction takes 16 x 16 outputs and 32 steps of the contraction: lane l holds 8 consecutive steps
+// (l / 16) * 8 .. + 7 of row l % 16 of either operand, and of the result the four rows (l / 16) * 4 .. + 3 of column
+// l % 16.  bf16 and f16 operands go in as they are.  An f32 operand goes in as THREE bf16 planes, x = hi + mid + lo
+// (8 + 8 + 8 bits, each the rounded rest of the one before): six of the nine plane products, smallest first, leave
+// 2^-24 of a product out.  bf16 has the exponents of f32, so nothing has to be scaled and no value leaves the range,
+// unlike f16 planes; a rate of 1/6 of the bf16 pipes is 2.6 times that of the f32 matrix instruction.  (A non-finite
+// f32 operand comes out as NaN: inf - inf in the split.)
+#pragma once
+#include "common.hpp"
+
+namespace tsd {
+namespace blk {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+using bf16x8 = bf16 __attribute__((ext_vector_type(8)));
+using f16x8 = f16 __attribute__((ext_vector_type(8)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using f32x2 = float __attribute__((ext_vector_type(2)));
+using bf16x2 = bf16 __attribute__((ext_vector_type(2)));
+
+// Chunk<T>: 8 values of the contraction, as matrix operands (P planes of 16 bytes)
+template <class T> struct Elem;
+template <> struct Elem<bf16> {
+    static constexpr int P = 1;
+    using vec = bf16x8;
+};
+template <> struct Elem<f16> {
+    static constexpr int P = 1;
+    using vec = f16x8;
+};
+template <> struct Elem<float> {
+    static constexpr int P = 3;
+    using vec = bf16x8;
+};
+template <class T> struct Chunk {
+    typename Elem<T>::vec p[Elem<T>::P];
+};
+
+__device__ __forceinline__ Chunk<bf16> to_chunk(const float (&x)[8], bf16) {
+    Chunk<bf16> c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c.p[0][j] = (bf16)x[j];
+    return c;
+}
+__device__ __forceinline__ Chunk<f16> to_chunk(const float (&x)[8], f16) {
+    Chunk<f16> c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c.p[0][j] = (f16)x[j];
+    return c;
+}
+__device__ __forceinline__ Chunk<float> to_chunk(const float (&x)[8], float) {
+    Chunk<float> c;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f32x2 r = {x[j], x[j + 1]};
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const bf16x2 h = __builtin_convertvector(r, bf16x2);
+            c.p[p][j] = h[0];
+            c.p[p][j + 1] = h[1];
+            r[0] -= (float)h[0];
+            r[1] -= (float)h[1];
+        }
+    }
+    return c;
+}
+
+__device__ __forceinline__ f32x4 mma(const Chunk<bf16>& a, const Chunk<bf16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Chunk<f16>& a, const Chunk<f16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Chunk<float>& a, const Chunk<float>& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Raw<T>: 8 values as they come from memory.  load_raw reads `n` of them (0 .. 8) and leaves zeros behind.
+// ---------------------------------------------------------------------------------------------
+template <class T> struct Raw;
+template <> struct Raw<float> {
+    f32x4 a, b;
+};
+template <> struct Raw<bf16> {
+    u32x4 a;
+};
+template <> struct Raw<f16> {
+    u32x4 a;
+};
+__device__ __forceinline__ void raw_zero(Raw<float>& r) { r.a = r.b = f32x4{0, 0, 0, 0}; }
+__device__ __forceinline__ void raw_zero(Raw<bf16>& r) { r.a = u32x4{0, 0, 0, 0}; }
+__device__ __forceinline__ void raw_zero(Raw<f16>& r) { r.a = u32x4{0, 0, 0, 0}; }
+__device__ __forceinline__ void raw_load8(Raw<float>& r, const float* p) {
+    r.a = *reinterpret_cast<const f32x4*>(p);
+    r.b = *reinterpret_cast<const f32x4*>(p + 4);
+}
+__device__ __forceinline__ void raw_load8(Raw<bf16>& r, const bf16* p) { r.a = *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ void raw_load8(Raw<f16>& r, const f16* p) { r.a = *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ void raw_put(Raw<float>& r, int j, float v) { (j < 4 ? r.a : r.b)[j & 3] = v; }
+template <class T> __device__ __forceinline__ uint32_t bits16(T v) {
+    uint16_t b;
+    __builtin_memcpy(&b, &v, 2);
+    return b;
+}
+template <class T> __device__ __forceinline__ void raw_put16(u32x4& a, int j, T v) {
+    a[j >> 1] |= bits16(v) << (16 * (j & 1));
+}
+__device__ __forceinline__ void raw_put(Raw<bf16>& r, int j, bf16 v) { raw_put16(r.a, j, v); }
+__device__ __forceinline__ void raw_put(Raw<f16>& r, int j, f16 v) { raw_put16(r.a, j, v); }
+
+// vec: p is 16-byte aligned and n is 0 or 8
+template <class T> __device__ __forceinline__ void load_raw(Raw<T>& r, const T* __restrict__ p, int n, bool vec) {
+    if (vec) {
+        if (n > 0) raw_load8(r, p);
+        else raw_zero(r);
+        return;
+    }
+    raw_zero(r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < n) raw_put(r, j, p[j]);
+}
+__device__ __forceinline__ Chunk<bf16> raw_chunk(const Raw<bf16>& r) {
+    Chunk<bf16> c;
+    c.p[0] = __builtin_bit_cast(bf16x8, r.a);
+    return c;
+}
+__device__ __forceinline__ Chunk<f16> raw_chunk(const Raw<f16>& r) {
+    Chunk<f16> c;
+    c.p[0] = __builtin_bit_cast(f16x8, r.a);
+    return c;
+}
+__device__ __forceinline__ Chunk<float> raw_chunk(const Raw<float>& r) {
+    const float x[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
+    return to_chunk(x, 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------
+// An operand tile in LDS: P planes of ROWS rows of C chunks (16 bytes each).  Chunk c of row r lies at place
+// c ^ swizzle(r), so that 16 lanes that read (or write) one chunk of 16 consecutive rows touch all 64 banks once.
+// ---------------------------------------------------------------------------------------------
+template <class T, int ROWS, int C> struct Tile {
+    static_assert(C == 4 || C == 8 || C == 16, "chunks of a row");
+    static constexpr int P = Elem<T>::P;
+    static constexpr int BYTES = P * ROWS * C * 16;
+    __device__ __forceinline__ static int at(int row, int c) {
+        return (row * C + (c ^ ((row / (16 / C)) & (C - 1)))) * 16;
+    }
+    __device__ __forceinline__ static void put(char* lds, int row, int c, const Chunk<T>& v) {
+        const int o = at(row, c);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            *reinterpret_cast<typename Elem<T>::vec*>(lds + p * (ROWS * C * 16) + o) = v.p[p];
+    }
+    __device__ __forceinline__ static Chunk<T> get(const char* lds, int row, int c) {
+        Chunk<T> v;
+        const int o = at(row, c);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            v.p[p] = *reinterpret_cast<const typename Elem<T>::vec*>(lds + p * (ROWS * C * 16) + o);
+        return v;
+    }
+};
+
+// Two neighbouring columns of 8 rows (16-bit types) or one column (f32): how a tile is turned on its way to LDS.
+// W columns a unit; w[j] holds row j's W values.
+template <class T> struct ColRaw {
+    static constexpr int W = 2;
+    uint32_t w[8];
+};
+template <> struct ColRaw<float> {
+    static constexpr int W = 1;
+    float w[8];
+};
+// p + row[j] .. : row j at p + off[j]; n rows valid through the mask `ok` (bit j), `cols` columns exist
+template <class T> __device__ __forceinline__ void col_load(uint32_t& w, const T* p, int cols, bool vec) {
+    if (vec) {  // 4-byte aligned, both columns exist
+        w = *reinterpret_cast<const uint32_t*>(p);
+        return;
+    }
+    w = bits16(p[0]);
+    if (cols > 1) w |= bits16(p[1]) << 16;
+}
+__device__ __forceinline__ void col_load(float& w, const float* p, int, bool) { w = *p; }
+
+template <class T> __device__ __forceinline__ Chunk<T> col_chunk(const ColRaw<T>& r, int which) {
+    u32x4 a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        a[j] = which ? (r.w[2 * j] >> 16) | (r.w[2 * j + 1] & 0xffff0000u) : (r.w[2 * j] & 0xffffu) | (r.w[2 * j + 1] << 16);
+    Chunk<T> c;
+    c.p[0] = __builtin_bit_cast(typename Elem<T>::vec, a);
+    return c;
+}
+template <> __device__ __forceinline__ Chunk<float> col_chunk<float>(const ColRaw<float>& r, int) {
+    return to_chunk(r.w, 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------
+// stores of four neighbouring outputs, rounded once
+// ---------------------------------------------------------------------------------------------
+template <class T> __device__ __forceinline__ void store4(T* p, f32x4 v, int n, bool vec) {
+    if (vec && n >= 4) {
+        T t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = (T)v[i];
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<f32x4*>(p) = v;
+        } else {
+            uint2 u;
+            u.x = bits16(t[0]) | bits16(t[1]) << 16;
+            u.y = bits16(t[2]) | bits16(t[3]) << 16;
+            *reinterpret_cast<uint2*>(p) = u;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) p[i] = (T)v[i];
+}
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(bf16 v) { return (float)v; }
+__device__ __forceinline__ float to_f(f16 v) { return (float)v; }
+
+template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n, bool vec) {
+    f32x4 r = {0, 0, 0, 0};
+    if (vec && n >= 4) {
+        if constexpr (sizeof(T) == 4) return *reinterpret_cast<const f32x4*>(p);
+        T t[4];
+        __builtin_memcpy(t, __builtin_assume_aligned(p, 8), 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = to_f(t[i]);
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) r[i] = to_f(p[i]);
+    return r;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// C entry -> instance: TSD_F32 / TSD_BF16 / TSD_F16
+#define TSD_BY_DTYPE(dtype, T, ...)                                          \
+    switch (dtype) {                                                         \
+        case TSD_F32: { using T = float; __VA_ARGS__; } break;               \
+        case TSD_BF16: { using T = ::tsd::blk::bf16; __VA_ARGS__; } break;   \
+        case TSD_F16: { using T = ::tsd::blk::f16; __VA_ARGS__; } break;     \
+        default: break;                                                      \
+    }
+
+}  // namespace blk
+}  // namespace tsd
