@@ -118,17 +118,45 @@ template <class T> __device__ __forceinline__ void raw_put16(u32x4& a, int j, T 
 __device__ __forceinline__ void raw_put(Raw<bf16>& r, int j, bf16 v) { raw_put16(r.a, j, v); }
 __device__ __forceinline__ void raw_put(Raw<f16>& r, int j, f16 v) { raw_put16(r.a, j, v); }
 
-// vec: p is 16-byte aligned and n is 0 or 8
-template <class T> __device__ __forceinline__ void load_raw(Raw<T>& r, const T* __restrict__ p, int n, bool vec) {
-    if (vec) {
-        if (n > 0) raw_load8(r, p);
-        else raw_zero(r);
-        return;
-    }
+// vw: values a load may take (p aligned to as many, n a multiple of it): 8, 4, 2 or 1
+template <class T> __device__ __forceinline__ void load_raw(Raw<T>& r, const T* __restrict__ p, int n, int vw) {
     raw_zero(r);
+    if constexpr (sizeof(T) == 2) {
+        if (vw == 8) {
+            if (n > 0) raw_load8(r, p);
+        } else if (vw == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < n) raw_put(r, j, p[j]);
+            for (int j = 0; j < 2; ++j)
+                if (4 * j < n) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(p + 4 * j);
+                    r.a[2 * j] = v.x;
+                    r.a[2 * j + 1] = v.y;
+                }
+        } else if (vw == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (2 * j < n) r.a[j] = *reinterpret_cast<const uint32_t*>(p + 2 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) raw_put(r, j, p[j]);
+        }
+    } else {
+        if (vw >= 4) {
+            if (n > 0) r.a = *reinterpret_cast<const f32x4*>(p);
+            if (n > 4) r.b = *reinterpret_cast<const f32x4*>(p + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) raw_put(r, j, p[j]);
+        }
+    }
+}
+// the widest such load for rows of `n` values `ld` apart from p on (strides of further dimensions: any common factor of ld)
+inline int load_width(size_t size, int64_t n, int64_t ld, const void* p) {
+    for (int v = 8; v > 1; v /= 2)
+        if (n % v == 0 && ld % v == 0 && (reinterpret_cast<uintptr_t>(p) & (v * size < 16 ? v * size - 1 : 15)) == 0) return v;
+    return 1;
 }
 __device__ __forceinline__ Chunk<bf16> raw_chunk(const Raw<bf16>& r) {
     Chunk<bf16> c;
@@ -146,64 +174,85 @@ __device__ __forceinline__ Chunk<float> raw_chunk(const Raw<float>& r) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// An operand tile in LDS: P planes of ROWS rows of C chunks (16 bytes each).  Chunk c of row r lies at place
-// c ^ swizzle(r), so that 16 lanes that read (or write) one chunk of 16 consecutive rows touch all 64 banks once.
+// An operand tile in LDS: P planes of ROWS rows of C chunks (16 bytes each).  It is read along its rows (get: chunk c of
+// row r) or across them (get_across: 8 rows of one column, by the LDS's transposing read), so a tensor is brought in as it
+// lies in memory whichever way a product goes over it.  Chunk c of row r lies at place c ^ swizzle(r): 16 lanes that read
+// one chunk of 16 rows (consecutive ones, or 0-3, 8-11, 16-19, 24-27) touch all 64 banks once, and so do the 32 lanes
+// that read two chunks of rows 0-3 and 8-11 across.
 // ---------------------------------------------------------------------------------------------
-template <class T, int ROWS, int C> struct Tile {
+using s16x4 = short __attribute__((ext_vector_type(4)));
+using s16x8 = short __attribute__((ext_vector_type(8)));
+template <class T, int ROWS_, int C_> struct Tile {
+    static constexpr int ROWS = ROWS_, C = C_;
     static_assert(C == 4 || C == 8 || C == 16, "chunks of a row");
     static constexpr int P = Elem<T>::P;
-    static constexpr int BYTES = P * ROWS * C * 16;
-    __device__ __forceinline__ static int at(int row, int c) {
-        return (row * C + (c ^ ((row / (16 / C)) & (C - 1)))) * 16;
+    static constexpr int PLANE = ROWS * C * 16, BYTES = P * PLANE;
+    using vec = typename Elem<T>::vec;
+    __device__ __forceinline__ static int swizzle(int r) {
+        const int low = ((r >> 2) ^ (r >> 4)) & 1, b3 = (r >> 3) & 1;
+        if constexpr (C == 16) return low | (r & 3) << 1 | b3 << 3;
+        if constexpr (C == 8) return low | ((r >> 1) & 1) << 1 | b3 << 2;
+        return low | b3 << 1;
     }
+    __device__ __forceinline__ static int at(int row, int c) { return (row * C + (c ^ swizzle(row))) * 16; }
     __device__ __forceinline__ static void put(char* lds, int row, int c, const Chunk<T>& v) {
         const int o = at(row, c);
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-            *reinterpret_cast<typename Elem<T>::vec*>(lds + p * (ROWS * C * 16) + o) = v.p[p];
+        for (int p = 0; p < P; ++p) *reinterpret_cast<vec*>(lds + p * PLANE + o) = v.p[p];
     }
     __device__ __forceinline__ static Chunk<T> get(const char* lds, int row, int c) {
         Chunk<T> v;
         const int o = at(row, c);
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-            v.p[p] = *reinterpret_cast<const typename Elem<T>::vec*>(lds + p * (ROWS * C * 16) + o);
+        for (int p = 0; p < P; ++p) v.p[p] = *reinterpret_cast<const vec*>(lds + p * PLANE + o);
+        return v;
+    }
+    // rows row0 + 8 (lane / 16) .. + 7 of column 16 t + lane % 16; row0 a multiple of 32
+    __device__ __forceinline__ static Chunk<T> get_across(const char* lds, int row0, int t) {
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        const int lane = threadIdx.x & 63, i = lane & 15, r = row0 + (lane >> 4) * 8 + (i >> 2), c = 2 * t + ((i & 3) >> 1);
+        const int o0 = at(r, c) + (i & 1) * 8, o1 = at(r + 4, c) + (i & 1) * 8;
+        Chunk<T> v;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lds + p * PLANE + o0));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lds + p * PLANE + o1));
+            v.p[p] = __builtin_bit_cast(vec, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
         return v;
     }
 };
 
-// Two neighbouring columns of 8 rows (16-bit types) or one column (f32): how a tile is turned on its way to LDS.
-// W columns a unit; w[j] holds row j's W values.
-template <class T> struct ColRaw {
-    static constexpr int W = 2;
-    uint32_t w[8];
-};
-template <> struct ColRaw<float> {
-    static constexpr int W = 1;
-    float w[8];
-};
-// p + row[j] .. : row j at p + off[j]; n rows valid through the mask `ok` (bit j), `cols` columns exist
-template <class T> __device__ __forceinline__ void col_load(uint32_t& w, const T* p, int cols, bool vec) {
-    if (vec) {  // 4-byte aligned, both columns exist
-        w = *reinterpret_cast<const uint32_t*>(p);
-        return;
-    }
-    w = bits16(p[0]);
-    if (cols > 1) w |= bits16(p[1]) << 16;
+// ---------------------------------------------------------------------------------------------
+// Loads from memory to LDS that pass no register (16-bit types): lane l of a wave writes 16 bytes at the wave's base +
+// 16 l (m0 holds the base: nothing else in these kernels uses it); an offset past the buffer's end (NOWHERE) writes zeros.  The compiler does not see them: dma_wait<N> waits until
+// at most the N youngest loads of the wave are under way, behind it stands a barrier.
+// ---------------------------------------------------------------------------------------------
+using i32x4 = int __attribute__((ext_vector_type(4)));
+constexpr uint32_t DMA_NOWHERE = 0x80000000u;
+__device__ __forceinline__ i32x4 dma_buffer(const void* p) {  // 2 GiB from p on; p the same in all lanes
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff),
+                 0x7fffffff, 0x00027000};
 }
-__device__ __forceinline__ void col_load(float& w, const float* p, int, bool) { w = *p; }
-
-template <class T> __device__ __forceinline__ Chunk<T> col_chunk(const ColRaw<T>& r, int which) {
-    u32x4 a;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        a[j] = which ? (r.w[2 * j] >> 16) | (r.w[2 * j + 1] & 0xffff0000u) : (r.w[2 * j] & 0xffffu) | (r.w[2 * j + 1] << 16);
-    Chunk<T> c;
-    c.p[0] = __builtin_bit_cast(typename Elem<T>::vec, a);
-    return c;
+__device__ __forceinline__ void dma_load(i32x4 buf, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(buf)
+                 : "memory");
 }
-template <> __device__ __forceinline__ Chunk<float> col_chunk<float>(const ColRaw<float>& r, int) {
-    return to_chunk(r.w, 0.f);
+// 4 bytes a lane: lane l writes the wave's base + 4 l
+__device__ __forceinline__ void dma_load4(i32x4 buf, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(buf)
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+// every wave's LDS reads are done and its awaited loads have landed
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
 // ---------------------------------------------------------------------------------------------

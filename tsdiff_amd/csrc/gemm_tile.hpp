@@ -1,5 +1,6 @@
 // gemm_tile.hpp -- C[m][n] = sum_k M(m, k) N(n, k) on operand tiles in LDS (block_tile.hpp), for the kernels of the gated
-// linear layer.  Either operand is read as it lies (k contiguous) or turned (the tile's rows contiguous) on its way to LDS.
+// linear layer.  An operand is a matrix whose rows are the output's (k contiguous: RowOperand) or whose rows are the
+// contraction's (ColOperand); its tiles are copied as they lie and read along or across.
 // The instruction's first operand is the n side: a lane then holds four neighbouring n of one m, which is how a
 // row-major result is stored and how the epilogues read what belongs to it.
 #pragma once
@@ -11,131 +12,204 @@ namespace blk {
 constexpr int GEMM_WG = 256;  // four waves, two by two over the output tile
 constexpr int GEMM_K = 32;    // steps of the contraction a tile
 
-// rows x kmax values, k contiguous; rows from `split` on are rows of a second matrix
-template <class T> struct RowSource {
+// Tile row r is matrix row first + r (r < split) or row first2 + r - split of a second matrix; k along the rows
+template <class T> struct RowOperand {
+    static constexpr bool ACROSS = false;
     const T *p, *p2;
     int64_t ld;
-    int rows, kmax, first, split, first2;  // tile row r < split: row first + r of p; else row first2 + r - split of p2
-    bool vec;
-    __device__ __forceinline__ void load(Raw<T>& raw, int r, int k) const {
+    int rows, kmax, first, split, first2;
+    int vw;  // load_raw's
+    template <int N> using TileOf = Tile<T, N, GEMM_K / 8>;
+    __device__ __forceinline__ void load(Raw<T>& raw, int r, int c, int k) const {
         const bool two = r >= split;
-        const int row = two ? first2 + r - split : first + r;
-        const int n = row < rows ? kmax - k : 0;
-        load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)row * ld + k : 0), n < 0 ? 0 : n > 8 ? 8 : n, vec);
+        const int row = two ? first2 + r - split : first + r, kk = k + c * 8, n = row < rows ? kmax - kk : 0;
+        load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)row * ld + kk : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
     }
+    // bytes from the tile's first matrix (both matrices' tiles fit 2 GiB: the caller has seen to it)
+    __device__ __forceinline__ uint32_t offset(int r, int c) const {
+        const bool two = r >= split;
+        return (two ? first2 + r - split : first + r) < rows ? (uint32_t)(((two ? r - split : r) * ld + c * 8) * (int)sizeof(T))
+                                                              : DMA_NOWHERE;
+    }
+    __device__ __forceinline__ bool inside(int, int c, int k) const { return k + c * 8 < kmax; }
+    __device__ __forceinline__ const T* base(bool two, int k) const {
+        return (two ? p2 + (int64_t)first2 * ld : p + (int64_t)first * ld) + k;
+    }
+    __device__ __forceinline__ bool second(int r, int) const { return r >= split; }
 };
-// kmax x cols values, columns contiguous; k from `ksplit` on are rows k - ksplit of a second matrix
-template <class T> struct ColSource {
+// Rows of the contraction, from `ksplit` on those of a second matrix (kmax rows each); columns first ..
+template <class T> struct ColOperand {
+    static constexpr bool ACROSS = true;
     const T *p, *p2;
     int64_t ld;
-    int cols, kmax, first, ksplit;  // kmax: rows of either matrix
-    bool vec;                       // two columns a load: even ld and first, 4-byte aligned
-    __device__ __forceinline__ void load(ColRaw<T>& raw, int c, int k) const {
-        const bool two = k >= ksplit;
-        const int kk = two ? k - ksplit : k, col = first + c;
-        const T* q = (two ? p2 : p) + col;
+    int cols, kmax, first, ksplit;
+    int vw;  // load_raw's
+    template <int N> using TileOf = Tile<T, GEMM_K, N / 8>;
+    __device__ __forceinline__ void load(Raw<T>& raw, int r, int c, int k) const {
+        const bool two = k + r >= ksplit;
+        const int kk = k + r - (two ? ksplit : 0), col = first + c * 8, n = kk < kmax ? cols - col : 0;
+        load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)kk * ld + col : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
+    }
+};
+
+// How a tile of N output rows (or columns) comes in.  Registers: U chunks a thread, DEPTH tiles under way.
+template <class T, int N, class Op, int DEPTH> struct RegStage {
+    using Lds = typename Op::template TileOf<N>;
+    static constexpr int UNITS = Lds::ROWS * Lds::C, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
+    Raw<T> raw[DEPTH][U];
+    __device__ __forceinline__ void load(int d, const Op& op, int k) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            raw.w[j] = 0;
-            if (col < cols && kk + j < kmax) col_load(raw.w[j], q + (int64_t)(kk + j) * ld, cols - col, vec && col + 1 < cols);
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * GEMM_WG;
+            if (UNITS % GEMM_WG == 0 || u < UNITS) op.load(raw[d][i], u / Lds::C, u % Lds::C, k);
+        }
+    }
+    __device__ __forceinline__ void store(int d, char* lds) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * GEMM_WG;
+            if (UNITS % GEMM_WG == 0 || u < UNITS) Lds::put(lds, u / Lds::C, u % Lds::C, raw_chunk(raw[d][i]));
+        }
+    }
+};
+// Straight to LDS: a wave's 64 lanes fill 64 neighbouring places, so the lane of place p of row r fetches chunk
+// p ^ swizzle(r).  One matrix a load: the 64 places of a wave lie on one side of the operand's split.
+template <class T, int N, class Op> struct DmaStage {
+    using Lds = typename Op::template TileOf<N>;
+    static constexpr int UNITS = Lds::ROWS * Lds::C, U = UNITS < GEMM_WG ? 1 : UNITS / GEMM_WG;
+    // (a tile smaller than the workgroup is loaded by several waves alike: every wave counts the same loads)
+    static_assert(UNITS % GEMM_WG == 0 || (GEMM_WG % UNITS == 0 && UNITS % 64 == 0), "whole loads");
+    uint32_t off[U];
+    int row[U], chunk[U];
+    __device__ __forceinline__ void init(const Op& op) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = (threadIdx.x + i * GEMM_WG) % UNITS;
+            row[i] = u / Lds::C;
+            chunk[i] = (u % Lds::C) ^ Lds::swizzle(row[i]);
+            if constexpr (!Op::ACROSS) {
+                off[i] = op.offset(row[i], chunk[i]);
+            } else {
+                const int col = op.first + chunk[i] * 8;
+                off[i] = col < op.cols ? (uint32_t)((row[i] * op.ld + chunk[i] * 8) * (int)sizeof(T)) : DMA_NOWHERE;
+            }
+        }
+    }
+    __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int wave_row = __builtin_amdgcn_readfirstlane(row[i]);
+            const uint32_t to = lds + (threadIdx.x / 64 * 64 + i * GEMM_WG) % UNITS * 16;
+            if constexpr (!Op::ACROSS) {
+                dma_load(dma_buffer(op.base(wave_row >= op.split, k)), k + chunk[i] * 8 < op.kmax ? off[i] : DMA_NOWHERE, to);
+            } else {  // ksplit is a multiple of 8, as few rows as a wave's load may hold: it lies on one side
+                const bool two = k + wave_row >= op.ksplit;
+                const int kk = k - (two ? op.ksplit : 0);
+                dma_load(dma_buffer((two ? op.p2 : op.p) + (int64_t)kk * op.ld + op.first),
+                         kk + row[i] < op.kmax ? off[i] : DMA_NOWHERE, to);
+            }
         }
     }
 };
 
-template <class T, int ROWS> struct RowStage {
-    static constexpr int UNITS = ROWS * 4, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
-    using Lds = Tile<T, ROWS, 4>;
-    Raw<T> raw[U];
-    __device__ __forceinline__ void load(const RowSource<T>& s, int k) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) s.load(raw[i], u >> 2, k + (u & 3) * 8);
-        }
-    }
-    __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) Lds::put(lds, u >> 2, u & 3, raw_chunk(raw[i]));
-        }
-    }
-};
-template <class T, int ROWS> struct ColStage {
-    static constexpr int W = ColRaw<T>::W, COLS = ROWS / W, UNITS = COLS * 4, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
-    using Lds = Tile<T, ROWS, 4>;
-    ColRaw<T> raw[U];
-    __device__ __forceinline__ void load(const ColSource<T>& s, int k) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) s.load(raw[i], (u % COLS) * W, k + (u / COLS) * 8);
-        }
-    }
-    __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS)
-#pragma unroll
-                for (int c = 0; c < W; ++c) Lds::put(lds, (u % COLS) * W + c, u / COLS, col_chunk<T>(raw[i], c));
-        }
-    }
-};
-template <class T, int ROWS, class Source> struct StageOf;
-template <class T, int ROWS> struct StageOf<T, ROWS, RowSource<T>> { using type = RowStage<T, ROWS>; };
-template <class T, int ROWS> struct StageOf<T, ROWS, ColSource<T>> { using type = ColStage<T, ROWS>; };
+template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
+    using NT = typename NS::template TileOf<BN>;
+    using MT = typename MS::template TileOf<BM>;
+    static constexpr int BUF = NT::BYTES + MT::BYTES;
+    using Acc = f32x4[BN / 32][BM / 32];
 
-template <class T, int BM, int BN> constexpr int gemm_lds() { return 2 * (Tile<T, BM, 4>::BYTES + Tile<T, BN, 4>::BYTES); }
-
-// One output tile: acc[jn][im] of the calling wave, n rows nrow(jn) and m rows mrow + im * 16 of the tile.
-// The next tile's values are on their way into registers while this tile's products run; two LDS buffers, one barrier a tile.
-template <class T, int BM, int BN, class NS, class MS, class NRow>
-__device__ __forceinline__ void gemm_tile(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow, NRow nrow,
-                                          f32x4 (&acc)[BN / 32][BM / 32]) {
-    using NT = Tile<T, BN, 4>;
-    using MT = Tile<T, BM, 4>;
-    constexpr int BUF = NT::BYTES + MT::BYTES;
-    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
-    typename StageOf<T, BN, NS>::type nst;
-    typename StageOf<T, BM, MS>::type mst;
-#pragma unroll
-    for (int j = 0; j < BN / 32; ++j)
-#pragma unroll
-        for (int i = 0; i < BM / 32; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
-    if (kbegin >= kend) return;
-    nst.load(ns, kbegin);
-    mst.load(ms, kbegin);
-    nst.store(lds);
-    mst.store(lds + NT::BYTES);
-    __syncthreads();
-    int cur = 0;
-    for (int k = kbegin; k < kend; k += GEMM_K) {
-        const bool more = k + GEMM_K < kend;
-        if (more) {
-            nst.load(ns, k + GEMM_K);
-            mst.load(ms, k + GEMM_K);
-        }
-        const char* nb = lds + cur * BUF;
+    template <class NRow>
+    __device__ __forceinline__ static void products(const char* nb, int mrow, NRow nrow, Acc& acc) {
+        const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
         const char* mb = nb + NT::BYTES;
         Chunk<T> mf[BM / 32];
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) mf[i] = MT::get(mb, mrow + i * 16 + r, c);
+        for (int i = 0; i < BM / 32; ++i) {
+            if constexpr (MS::ACROSS) mf[i] = MT::get_across(mb, 0, mrow / 16 + i);
+            else mf[i] = MT::get(mb, mrow + i * 16 + r, c);
+        }
 #pragma unroll
         for (int j = 0; j < BN / 32; ++j) {
-            const Chunk<T> nf = NT::get(nb, nrow(j) + r, c);
+            Chunk<T> nf;
+            if constexpr (NS::ACROSS) nf = NT::get_across(nb, 0, nrow(j) / 16);
+            else nf = NT::get(nb, nrow(j) + r, c);
 #pragma unroll
             for (int i = 0; i < BM / 32; ++i) acc[j][i] = mma(nf, mf[i], acc[j][i]);
         }
-        if (more) {
-            char* next = lds + (cur ^ 1) * BUF;
-            nst.store(next);
-            mst.store(next + NT::BYTES);
-        }
-        __syncthreads();
-        cur ^= 1;
     }
-}
+    __device__ __forceinline__ static void clear(Acc& acc) {
+#pragma unroll
+        for (int j = 0; j < BN / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < BM / 32; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    }
+    // One output tile: acc[jn][im] of the calling wave, n rows nrow(jn) and m rows mrow + im * 16 of the tile; ends behind a
+    // barrier.  The next DEPTH tiles' values are on their way into registers; two LDS buffers, one barrier a tile.
+    template <int DEPTH, class NRow>
+    __device__ __forceinline__ static void by_registers(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow,
+                                                        NRow nrow, Acc& acc) {
+        RegStage<T, BN, NS, DEPTH> nst;
+        RegStage<T, BM, MS, DEPTH> mst;
+        clear(acc);
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d)
+            if (kbegin + d * GEMM_K < kend) {
+                nst.load(d, ns, kbegin + d * GEMM_K);
+                mst.load(d, ms, kbegin + d * GEMM_K);
+            }
+        nst.store(0, lds);
+        mst.store(0, lds + NT::BYTES);
+        __syncthreads();
+        int cur = 0;
+        for (int k0 = kbegin; k0 < kend; k0 += DEPTH * GEMM_K) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const int k = k0 + d * GEMM_K;
+                if (k >= kend) break;
+                if (k + DEPTH * GEMM_K < kend) {
+                    nst.load(d, ns, k + DEPTH * GEMM_K);
+                    mst.load(d, ms, k + DEPTH * GEMM_K);
+                }
+                products(lds + cur * BUF, mrow, nrow, acc);
+                cur ^= 1;
+                if (k + GEMM_K < kend) {
+                    nst.store((d + 1) % DEPTH, lds + cur * BUF);
+                    mst.store((d + 1) % DEPTH, lds + cur * BUF + NT::BYTES);
+                }
+                __syncthreads();
+            }
+        }
+    }
+    // The same with loads straight to LDS: STAGES buffers, STAGES - 1 tiles under way, one barrier a tile.
+    template <int STAGES, class NRow>
+    __device__ __forceinline__ static void by_dma(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow, NRow nrow,
+                                                  Acc& acc) {
+        DmaStage<T, BN, NS> nst;
+        DmaStage<T, BM, MS> mst;
+        constexpr int LOADS = DmaStage<T, BN, NS>::U + DmaStage<T, BM, MS>::U;
+        nst.init(ns);
+        mst.init(ms);
+        clear(acc);
+        const uint32_t base = lds_offset(lds);
+#pragma unroll
+        for (int d = 0; d < STAGES - 1; ++d) {  // (tiles past the end load zeros: the count of loads stays the same)
+            nst.issue(ns, kbegin + d * GEMM_K, base + d * BUF);
+            mst.issue(ms, kbegin + d * GEMM_K, base + d * BUF + NT::BYTES);
+        }
+        int buf = 0, ahead = STAGES - 1;
+        for (int k = kbegin; k < kend; k += GEMM_K) {
+            dma_wait<(STAGES - 2) * LOADS>();
+            lds_barrier();
+            nst.issue(ns, k + (STAGES - 1) * GEMM_K, base + ahead * BUF);
+            mst.issue(ms, k + (STAGES - 1) * GEMM_K, base + ahead * BUF + NT::BYTES);
+            products(lds + buf * BUF, mrow, nrow, acc);
+            buf = buf + 1 == STAGES ? 0 : buf + 1;
+            ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+        }
+        dma_wait<0>();  // nothing may land in LDS that is used otherwise, or belongs to the next workgroup
+        lds_barrier();
+    }
+};
 
 // Workgroup b of a grid over (long side) x (short side) tiles: consecutive workgroups go to the eight XCDs in turn, so the
 // tiles of one long-side row are given to one XCD, whose L2 then holds that row's operand once.

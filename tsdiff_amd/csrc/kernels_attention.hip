@@ -11,24 +11,25 @@
 // dV; every gradient is summed by one workgroup in a fixed order, without atomics.
 //
 // Rows are (query, query head of the key head's group), so heads that share keys share their tiles.  Tiles never cross a
-// graph: workgroup s looks its graph up, tile slot(v) = floor(start_v / T) + v being where graph v's tiles begin -- a bound
-// on the tiles before it that needs no prefix sum and no lengths on the host, at most one idle workgroup a graph.  Offsets
-// are clamped into the tensors.  Rows and keys outside of every graph count as graphs without keys / rows: they are written
+// graph: workgroup s looks its graph up, slot(v) = floor((start_v + v (T - 1)) / T) being where graph v's tiles begin -- a
+// bound on the tiles before it that needs no prefix sum and no lengths on the host, less than one idle workgroup a graph.
+// The key heads of a slot are neighbouring workgroups: they go to the eight XCDs in turn, and share lines of memory in time.
+// Offsets are clamped into the tensors.  Rows and keys outside of every graph count as graphs without keys / rows: they are written
 // as zeros.  Masked and missing keys are zeros in LDS whatever memory holds there, so that no NaN meets a zero weight.
 #include "block_tile.hpp"
 
 namespace tsd {
 namespace blk {
 
-constexpr int ATT_KT = 64;  // keys (forward, dQ) a tile in LDS
 constexpr float LOG2E = 1.44269504088896341f;
 
 struct AttDims {
     int graphs, rows_q, rows_k, heads, kv_heads, group, dim;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
     float scale, scale2;  // scale2 = scale * log2 e
-    int splits;
-    bool qvec, kvec, vvec, dovec, ovec;
+    int splits, slots;
+    int qvw, kvw, vvw, dovw;  // values a load of each may take (load_raw)
+    bool ovec;
     const int32_t *q_ptr, *k_ptr;
     const uint8_t* mask;
 };
@@ -40,95 +41,146 @@ struct Span {
 __device__ __forceinline__ int clamp_to(int v, int n) { return v < 0 ? 0 : v > n ? n : v; }
 // boundary v of the list 0, ptr[0], .., ptr[G], n
 __device__ __forceinline__ int bound_at(const int32_t* ptr, int graphs, int n, int v) {
-    return v == 0 ? 0 : v > graphs + 1 ? n : clamp_to(ptr[v - 1], n);
+    return v <= 0 ? 0 : v > graphs + 1 ? n : clamp_to(ptr[v - 1], n);
 }
-// the graph whose tiles hold slot s (64 lanes look at a time); tiles of T rows, `times` rows an entry
+// The graph whose tiles (T rows, `times` rows an entry) hold slot s.  slot(v) = floor((start_v times + v (T - 1)) / T) leaves
+// every graph the tiles it needs.  64 lanes look at a time, first where equal graphs would have it.
 __device__ __forceinline__ Span find_span(const AttDims& d, bool by_key, int T, int times, int s) {
     const int32_t* ptr = by_key ? d.k_ptr : d.q_ptr;
-    const int n = by_key ? d.rows_k : d.rows_q, lane = threadIdx.x & 63;
-    int lo = 0, count = d.graphs + 2;  // slot(lo) <= s, and the answer is below lo + count
-    while (count > 1) {
-        const int step = (count + 63) / 64, v = lo + lane * step;
-        const bool in = lane * step < count && (int64_t)bound_at(ptr, d.graphs, n, v) * times / T + v <= s;
-        const unsigned long long m = __ballot(in);
-        const int last = 63 - __builtin_clzll(m | 1);
-        lo += last * step;
-        count = count - last * step < step ? count - last * step : step;
+    const int32_t* other = by_key ? d.q_ptr : d.k_ptr;
+    const int n = by_key ? d.rows_k : d.rows_q, on = by_key ? d.rows_q : d.rows_k, lane = threadIdx.x & 63, all = d.graphs + 2;
+    auto slot = [&](int b, int v) { return ((int64_t)b * times + (int64_t)v * (T - 1)) / T; };
+    int lo = (int)((int64_t)s * all / d.slots) - 32;
+    lo = lo > all - 64 ? all - 64 : lo;
+    lo = lo < 0 ? 0 : lo;
+    int b = bound_at(ptr, d.graphs, n, lo + lane);
+    unsigned long long m = __ballot(lo + lane < all && slot(b, lo + lane) <= s);
+    if (!(m & 1) || (m == ~0ull && lo + 64 < all)) {  // not here: narrow the whole list down
+        lo = 0;
+        int count = all;  // slot(lo) <= s < slot(lo + count)
+        while (count > 64) {
+            const int step = (count + 63) / 64, v = lo + lane * step;
+            m = __ballot(lane * step < count && slot(bound_at(ptr, d.graphs, n, v), v) <= s);
+            const int last = 63 - __builtin_clzll(m | 1);
+            lo += last * step;
+            count = count - last * step < step ? count - last * step : step;
+        }
+        b = bound_at(ptr, d.graphs, n, lo + lane);
+        m = __ballot(lane < count && slot(b, lo + lane) <= s);
+    }
+    const int last = 63 - __builtin_clzll(m | 1), v = lo + last;
+    const int start = __builtin_amdgcn_readlane(b, last);
+    int end = last < 63 ? __builtin_amdgcn_readlane(b, last < 63 ? last + 1 : 63) : bound_at(ptr, d.graphs, n, v + 1);
+    int os = 0, oe = 0;
+    if (v >= 1 && v <= d.graphs) {
+        if (other == ptr && on == n) {
+            os = start;
+            oe = end;
+        } else {
+            os = bound_at(other, d.graphs, on, v);
+            oe = bound_at(other, d.graphs, on, v + 1);
+        }
     }
     Span sp;
-    const int start = bound_at(ptr, d.graphs, n, lo);
-    sp.tile = s - (int)((int64_t)start * times / T) - lo;
-    const bool real = lo >= 1 && lo <= d.graphs;
-    const int end = bound_at(ptr, d.graphs, n, lo + 1);
-    const int ostart = real ? bound_at(by_key ? d.q_ptr : d.k_ptr, d.graphs, by_key ? d.rows_q : d.rows_k, lo) : 0;
-    const int oend = real ? bound_at(by_key ? d.q_ptr : d.k_ptr, d.graphs, by_key ? d.rows_q : d.rows_k, lo + 1) : 0;
-    sp.qs = by_key ? ostart : start;
-    sp.qe = by_key ? oend : end;
-    sp.ks = by_key ? start : ostart;
-    sp.ke = by_key ? end : oend;
-    if (sp.qe < sp.qs) sp.qe = sp.qs;
-    if (sp.ke < sp.ks) sp.ke = sp.ks;
+    sp.tile = s - (int)slot(start, v);
+    end = end < start ? start : end;
+    oe = oe < os ? os : oe;
+    sp.qs = by_key ? os : start;
+    sp.qe = by_key ? oe : end;
+    sp.ks = by_key ? start : os;
+    sp.ke = by_key ? end : oe;
     return sp;
 }
 
 // Values (row, d) of a graph's rows or keys
 template <class T> struct Rows {
-    const T* p;        // row 0 of the graph, this head (the first of the group)
-    int64_t row, head; // strides
-    int n, group, dim; // rows
+    const T* p;         // row 0 of the graph, this head (the first of the group)
+    int64_t row, head;  // strides
+    int n, group, dim;  // n: rows
     const uint8_t* mask;
-    bool vec;
+    int vw;
     __device__ __forceinline__ bool has(int r) const { return r < n && (mask == nullptr || mask[r] != 0); }
     __device__ __forceinline__ const T* at(int r) const {
         if (group == 1) return p + (int64_t)r * row;
         const int q = r / group;
         return p + (int64_t)q * row + (r - q * group) * head;
     }
+    // bit i: row r0 + i (i < ROWS <= 64) is there and open; the same in every lane
+    template <int ROWS> __device__ __forceinline__ uint64_t open(int r0) const {
+        if (mask == nullptr) return n - r0 >= 64 ? ~0ull : n > r0 ? (1ull << (n - r0)) - 1 : 0;
+        const int lane = threadIdx.x & 63;
+        return __ballot(lane < ROWS && has(r0 + lane));
+    }
 };
 
-// tile rows r0 .. r0 + ROWS as they lie: chunk c of row r
-template <class T, int ROWS, int DP, int NT>
-__device__ __forceinline__ void stage_rows(char* lds, const Rows<T>& s, int r0) {
-    constexpr int C = DP / 8;
-    for (int u = threadIdx.x; u < ROWS * C; u += NT) {
-        const int r = u / C, c = u % C, n = s.dim - c * 8;
-        Raw<T> raw;
-        if (n > 0 && s.has(r0 + r)) load_raw(raw, s.at(r0 + r) + c * 8, n > 8 ? 8 : n, s.vec);
-        else raw_zero(raw);
-        Tile<T, ROWS, C>::put(lds, r, c, raw_chunk(raw));
-    }
-}
-// The same values turned: row d, the tile's rows along it.  Chunk 4 b + g of a row holds rows 32 b + 4 g .. + 3 and
-// 32 b + 16 + 4 g .. + 3: the order in which two neighbouring 16 x 16 results leave lane group g.
-template <class T, int ROWS, int DP, int NT>
-__device__ __forceinline__ void stage_cols(char* lds, const Rows<T>& s, int r0) {
-    constexpr int W = ColRaw<T>::W, COLS = DP / W, C = ROWS / 8;
-    for (int u = threadIdx.x; u < COLS * C; u += NT) {
-        const int d = (u % COLS) * W, c = u / COLS, base = r0 + (c >> 2) * 32 + (c & 3) * 4;
-        ColRaw<T> raw;
+// A tile of ROWS rows on its way to LDS; rows that are not open become zeros.  DMA: straight there; registers otherwise.
+template <class T, int ROWS, int DP, int NT, bool DMA> struct RowStage {
+    using Lds = Tile<T, ROWS, DP / 8>;
+    static constexpr int C = DP / 8, UNITS = ROWS * C, U = (UNITS + NT - 1) / NT;
+    static_assert(!DMA || UNITS % NT == 0 || (NT % UNITS == 0 && UNITS % 64 == 0), "whole loads");
+    Raw<T> raw[DMA ? 1 : U];
+    __device__ __forceinline__ void load(const Rows<T>& s, int r0, uint64_t open, uint32_t lds) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = base + (j & 3) + (j >> 2) * 16;
-            raw.w[j] = 0;
-            if (d < s.dim && s.has(r)) col_load(raw.w[j], s.at(r) + d, s.dim - d, s.vec);
+        for (int i = 0; i < U; ++i) {
+            int u = threadIdx.x + i * NT;
+            if constexpr (DMA) {
+                u %= UNITS;  // (a small tile is loaded by several waves alike: every wave counts the same loads)
+                const int r = u / C, c = (u % C) ^ Lds::swizzle(r);
+                const T* base = s.group == 1 ? s.p + (int64_t)r0 * s.row : s.p + (int64_t)(r0 / s.group) * s.row;
+                uint32_t off = DMA_NOWHERE;
+                if ((open >> r & 1) && c * 8 < s.dim) off = (uint32_t)((s.at(r0 + r) - base + c * 8) * (int)sizeof(T));
+                dma_load(dma_buffer(base), off, lds + (threadIdx.x / 64 * 64 + i * NT) % UNITS * 16);
+            } else if (UNITS % NT == 0 || u < UNITS) {
+                const int r = u / C, c = u % C, n = (open >> r & 1) ? s.dim - c * 8 : 0;
+                load_raw(raw[i], n > 0 ? s.at(r0 + r) + c * 8 : s.p, n < 0 ? 0 : n > 8 ? 8 : n, s.vw);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < W; ++k) Tile<T, DP, C>::put(lds, d + k, c, col_chunk<T>(raw, k));
     }
-}
+    __device__ __forceinline__ void store(char* lds) const {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int u = threadIdx.x + i * NT;
+                if (UNITS % NT == 0 || u < UNITS) Lds::put(lds, u / C, u % C, raw_chunk(raw[i]));
+            }
+        }
+    }
+};
+
 // one row's operand, kept in registers: chunk (lane / 16) of each 32 values
-template <class T, int DP> __device__ __forceinline__ void row_chunks(Chunk<T> (&f)[DP / 32], const Rows<T>& s, int r) {
-    const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b) {
-        const int d0 = b * 32 + g * 8, n = s.dim - d0;
-        Raw<T> raw;
-        if (n > 0 && s.has(r)) load_raw(raw, s.at(r) + d0, n > 8 ? 8 : n, s.vec);
-        else raw_zero(raw);
-        f[b] = raw_chunk(raw);
-    }
+template <class T> __device__ __forceinline__ void row_raw(Raw<T>& raw, const Rows<T>& s, int r, bool has, int b) {
+    const int d0 = b * 32 + ((threadIdx.x & 63) >> 4) * 8, n = has ? s.dim - d0 : 0;
+    load_raw(raw, n > 0 ? s.at(r) + d0 : s.p, n < 0 ? 0 : n > 8 ? 8 : n, s.vw);
 }
-// two 16 x 16 results of neighbouring subtiles as the operand of the next product
+template <class T, int DP> __device__ __forceinline__ void row_chunks(Chunk<T> (&f)[DP / 32], const Rows<T>& s, int r) {
+    const bool has = s.has(r);
+    Raw<T> raw[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) row_raw(raw[b], s, r, has, b);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) f[b] = raw_chunk(raw[b]);
+}
+__device__ __forceinline__ float raw_dot(const Raw<float>& a, const Raw<float>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += a.a[j] * b.a[j] + a.b[j] * b.b[j];
+    return s;
+}
+template <class T> __device__ __forceinline__ float raw_dot(const Raw<T>& a, const Raw<T>& b) {
+    T x[8], y[8];
+    __builtin_memcpy(x, &a, 16);
+    __builtin_memcpy(y, &b, 16);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += to_f(x[j]) * to_f(y[j]);
+    return s;
+}
+// Of a block of 32 tile rows, row i of 16 x 16 subtile t is row 8 (i / 4) + 4 t + i % 4: lane group g then holds rows
+// 8 g .. + 7 of the block, in order, in the results of t = 0 and 1 -- chunk g of the next product's operand.
+__device__ __forceinline__ int sub_row(int t) {
+    const int i = threadIdx.x & 15;
+    return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
+}
 template <class T> __device__ __forceinline__ Chunk<T> joined(const f32x4& a, const f32x4& b) {
     const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return to_chunk(x, T());
@@ -144,107 +196,197 @@ __device__ __forceinline__ float over_groups_sum(float v) {
 }
 template <class T>
 __device__ __forceinline__ Rows<T> rows_of(const T* p, int64_t row, int64_t head, int start, int n, int first_head, int group,
-                                           int dim, const uint8_t* mask, bool vec) {
+                                           int dim, const uint8_t* mask, int vw) {
     return {p + (int64_t)start * row + (int64_t)first_head * head, row, head, n, group, dim,
-            mask == nullptr ? nullptr : mask + start, vec};
+            mask == nullptr ? nullptr : mask + start, vw};
 }
-// keys of split z: whole tiles, in equal shares
+// tiles of split z, in equal shares
 __device__ __forceinline__ void split_range(int n, int tile, int splits, int z, int* b, int* e) {
     const int tiles = (n + tile - 1) / tile, per = (tiles + splits - 1) / splits;
-    *b = z * per * tile;
-    *e = (z + 1) * per * tile;
-    if (*b > n) *b = n;
-    if (*e > n) *e = n;
+    *b = z * per < tiles ? z * per : tiles;
+    *e = (z + 1) * per < tiles ? (z + 1) * per : tiles;
 }
 
+// The tiles b .. e - 1 of one pair of row sets, one after the other in LDS: stage(i, open, buffer) starts tile i's loads,
+// step(i, open, buffer) is its work.  DMA: three buffers, two tiles under way; registers: two buffers, one tile under way.
+// LOADS: the loads of a wave a tile.
+template <int LOADS, bool DMA, class Open, class Load, class Store, class Step>
+__device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, Store store, Step step) {
+    if (b >= e) return;
+    if constexpr (DMA) {
+        uint64_t m0 = open(b), m1 = b + 1 < e ? open(b + 1) : 0;
+        load(b, m0, 0);
+        if (b + 1 < e) load(b + 1, m1, 1);
+        int buf = 0;
+        for (int i = b; i < e; ++i) {
+            const uint64_t m2 = i + 2 < e ? open(i + 2) : 0;
+            if (i + 1 < e) dma_wait<LOADS>();
+            else dma_wait<0>();
+            lds_barrier();
+            if (i + 2 < e) load(i + 2, m2, buf == 0 ? 2 : buf - 1);
+            step(i, m0, buf);
+            m0 = m1;
+            m1 = m2;
+            buf = buf == 2 ? 0 : buf + 1;
+        }
+    } else {
+        uint64_t m0 = open(b);
+        load(b, m0, 0);
+        store(0);
+        int buf = 0;
+        for (int i = b; i < e; ++i) {
+            __syncthreads();
+            const uint64_t m1 = i + 1 < e ? open(i + 1) : 0;
+            if (i + 1 < e) load(i + 1, m1, buf ^ 1);
+            step(i, m0, buf);
+            if (i + 1 < e) store(buf ^ 1);
+            m0 = m1;
+            buf ^= 1;
+        }
+    }
+}
+template <bool DMA> constexpr int att_buffers() { return DMA ? 3 : 2; }
+
 // ---------------------------------------------------------------------------------------------
-// forward: WAVES waves of 16 rows each share the key tiles
+// forward: WAVES waves of RS x 16 rows each share the key tiles
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int KT>
+template <class T, int DP, int WAVES, int RS, int KT, bool DMA>
 __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, T* __restrict__ out,
                                                              float* __restrict__ lse, float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TR = WAVES * 16;
-    using KTile = Tile<T, KT, DP / 8>;
-    using VTile = Tile<T, DP, KT / 8>;
+    constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
+    using Stage = RowStage<T, KT, DP, NT, DMA>;
+    using KTile = typename Stage::Lds;
+    constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
-    char* kl = lds;
-    char* vl = kl + KTile::BYTES;
-    const Span sp = find_span(d, false, TR, d.group, blockIdx.x);
-    const int hk = blockIdx.y, r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
+    const int hk = blockIdx.x % d.kv_heads;
+    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / d.kv_heads);
+    const int r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
     if (r0 >= nrows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int row = r0 + wave * 16 + c;
-    const uint8_t* mask = d.mask;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.qvec);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, mask, d.kvec);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, mask, d.vvec);
-    Chunk<T> qf[DP / 32];
-    row_chunks<T, DP>(qf, qr, row);
-    f32x4 o[DP / 16];
+    const int row0 = r0 + wave * RS * 16 + c;
+    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, (const uint8_t*)nullptr, d.qvw);
+    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
+    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
+    Chunk<T> qf[RS][DP / 32];
+    f32x4 o[RS][DP / 16];
+    float m[RS], l[RS];
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.f;
-    int kb, ke;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &kb, &ke);
-    for (int k0 = kb; k0 < ke; k0 += KT) {
-        __syncthreads();
-        stage_rows<T, KT, DP, NT>(kl, kr, k0);
-        stage_cols<T, KT, DP, NT>(vl, vr, k0);
-        __syncthreads();
-        f32x4 s[KT / 16];
-        float top = -INFINITY;
+    for (int x = 0; x < RS; ++x) {
+        row_chunks<T, DP>(qf[x], qr, row0 + x * 16);
 #pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-            s[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < DP / 32; ++b) s[t] = mma(KTile::get(kl, t * 16 + c, b * 4 + g), qf[b], s[t]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] = kr.has(k0 + t * 16 + g * 4 + e) ? s[t][e] * d.scale2 : -INFINITY;
-                top = fmaxf(top, s[t][e]);
-            }
-        }
-        top = fmaxf(m, over_groups_max(top));
-        const float safe = top == -INFINITY ? 0.f : top, a = exp2_fast(m - safe);
-        m = top;
-        l *= a;
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] = exp2_fast(s[t][e] - safe);
-                l += s[t][e];
-            }
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) o[t] *= a;
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
-            const Chunk<T> p = joined<T>(s[2 * b], s[2 * b + 1]);
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) o[t] = mma(VTile::get(vl, t * 16 + c, b * 4 + g), p, o[t]);
-        }
+        for (int t = 0; t < DP / 16; ++t) o[x][t] = f32x4{0, 0, 0, 0};
+        m[x] = -INFINITY;
+        l[x] = 0.f;
     }
-    l = over_groups_sum(l);
-    if (row >= nrows) return;
-    const int qi = sp.qs + row / d.group, h = hk * d.group + row % d.group;
-    const int64_t at = (int64_t)qi * d.heads + h;
-    if (d.splits > 1) {  // unnormalised sums and their statistics: att_join_kernel ends the work
-        const int64_t all = (int64_t)d.rows_q * d.heads, i = blockIdx.z * all + at;
-        float* po = part + i * d.dim;
+    Stage ks, vs;
+    const uint32_t at_lds = lds_offset(lds);
+    int tb, te;
+    split_range(kr.n, KT, d.splits, blockIdx.z, &tb, &te);
+    over_tiles<2 * Stage::U, DMA>(
+        tb, te, [&](int i) { return kr.template open<KT>(i * KT); },
+        [&](int i, uint64_t open, int buf) {
+            ks.load(kr, i * KT, open, at_lds + buf * BUF);
+            vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
+        },
+        [&](int buf) {
+            ks.store(lds + buf * BUF);
+            vs.store(lds + buf * BUF + KTile::BYTES);
+        },
+        [&](int, uint64_t open, int buf) {
+            const char* kl = lds + buf * BUF;
+            const char* vl = kl + KTile::BYTES;
+            f32x4 s[RS][KT / 16];
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) store4(po + t * 16 + g * 4, o[t], d.dim - t * 16 - g * 4, d.dim % 4 == 0);
-        if (g == 0) {
-            float* ps = part + d.splits * all * d.dim + 2 * i;
-            ps[0] = m;
-            ps[1] = l;
+            for (int t = 0; t < KT / 16; ++t) {
+#pragma unroll
+                for (int x = 0; x < RS; ++x) s[x][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) {
+                    const Chunk<T> kf = KTile::get(kl, sub_row(t), b * 4 + g);
+#pragma unroll
+                    for (int x = 0; x < RS; ++x) s[x][t] = mma(kf, qf[x][b], s[x][t]);
+                }
+            }
+            const bool whole = KT == 64 ? open == ~0ull : (uint32_t)open == 0xffffffffu;
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < KT / 16; ++t) {
+                    const uint32_t bits = (uint32_t)(open >> (32 * (t >> 1) + 8 * g + 4 * (t & 1)));
+#pragma unroll
+                    for (int x = 0; x < RS; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[x][t][e] = bits >> e & 1 ? s[x][t][e] * d.scale2 : -INFINITY;
+                }
+            }
+            const float sc = whole ? d.scale2 : 1.f;  // the scores' unit: a whole tile's are still to be scaled
+#pragma unroll
+            for (int x = 0; x < RS; ++x) {
+                float hi = -INFINITY;
+                if (sc >= 0.f) {
+#pragma unroll
+                    for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, s[x][t][e]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, -s[x][t][e]);
+                }
+                const float top = fmaxf(m[x], over_groups_max(hi * fabsf(sc)));
+                const float safe = top == -INFINITY ? 0.f : top, a = exp2_fast(m[x] - safe);
+                m[x] = top;
+                l[x] *= a;
+#pragma unroll
+                for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[x][t][e] = exp2_fast(__builtin_fmaf(s[x][t][e], sc, -safe));
+                        l[x] += s[x][t][e];
+                    }
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) o[x][t] *= a;
+            }
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) {
+                Chunk<T> p[RS];
+#pragma unroll
+                for (int x = 0; x < RS; ++x) p[x] = joined<T>(s[x][2 * b], s[x][2 * b + 1]);
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    const Chunk<T> vf = KTile::get_across(vl, b * 32, t);
+#pragma unroll
+                    for (int x = 0; x < RS; ++x) o[x][t] = mma(vf, p[x], o[x][t]);
+                }
+            }
+        });
+#pragma unroll
+    for (int x = 0; x < RS; ++x) {
+        const float ls = over_groups_sum(l[x]);
+        const int row = row0 + x * 16;
+        if (row >= nrows) continue;
+        const int qi = sp.qs + row / d.group, h = hk * d.group + row % d.group;
+        const int64_t at = (int64_t)qi * d.heads + h;
+        if (d.splits > 1) {  // unnormalised sums and their statistics: att_join_kernel ends the work
+            const int64_t all = (int64_t)d.rows_q * d.heads, i = blockIdx.z * all + at;
+            float* po = part + i * d.dim;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) store4(po + t * 16 + g * 4, o[x][t], d.dim - t * 16 - g * 4, d.dim % 4 == 0);
+            if (g == 0) {
+                float* ps = part + d.splits * all * d.dim + 2 * i;
+                ps[0] = m[x];
+                ps[1] = ls;
+            }
+            continue;
         }
-        return;
-    }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) store4(out + at * d.dim + t * 16 + g * 4, o[t] * inv, d.dim - t * 16 - g * 4, d.ovec);
-    if (lse != nullptr && g == 0) lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+        for (int t = 0; t < DP / 16; ++t)
+            store4(out + at * d.dim + t * 16 + g * 4, o[x][t] * inv, d.dim - t * 16 - g * 4, d.ovec);
+        if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? -INFINITY : m[x] + log2f(ls);
+    }
 }
 
 // The parts of a row: out = sum_z 2^(m_z - m) O_z / sum_z 2^(m_z - m) l_z, 64 rows' values a workgroup
@@ -284,191 +426,268 @@ __global__ __launch_bounds__(256) void att_sum_kernel(int64_t n, int splits, con
 // ---------------------------------------------------------------------------------------------
 // dQ: the forward's tiles again; delta on the way
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int KT>
+template <class T, int DP, int WAVES, int RS, int KT, bool DMA>
 __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                             const T* __restrict__ v, const T* __restrict__ out,
                                                             const T* __restrict__ dout, const float* __restrict__ lse,
                                                             float* __restrict__ delta, T* __restrict__ dq,
                                                             float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TR = WAVES * 16;
-    using KTile = Tile<T, KT, DP / 8>;
-    using KCols = Tile<T, DP, KT / 8>;
+    constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
+    using Stage = RowStage<T, KT, DP, NT, DMA>;
+    using KTile = typename Stage::Lds;
+    constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
-    char* kl = lds;
-    char* vl = kl + KTile::BYTES;
-    char* kc = vl + KTile::BYTES;
-    const Span sp = find_span(d, false, TR, d.group, blockIdx.x);
-    const int hk = blockIdx.y, r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
+    const int hk = blockIdx.x % d.kv_heads;
+    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / d.kv_heads);
+    const int r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
     if (r0 >= nrows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int row = r0 + wave * 16 + c;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.qvec);
-    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.dovec);
-    const Rows<T> orow = rows_of(out, (int64_t)d.heads * d.dim, d.dim, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.ovec);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvec);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvec);
-    Chunk<T> qf[DP / 32], gf[DP / 32];
-    row_chunks<T, DP>(qf, qr, row);
-    row_chunks<T, DP>(gf, gr, row);
-    const bool mine = row < nrows;
-    const int qi = sp.qs + (mine ? row / d.group : 0), h = hk * d.group + (mine ? row % d.group : 0);
-    const int64_t at = (int64_t)qi * d.heads + h;
-    float del = 0.f;
-    if (mine) {
-        const T *po = orow.at(row), *pg = gr.at(row);
+    const int row0 = r0 + wave * RS * 16 + c;
+    const uint8_t* no = nullptr;
+    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
+    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
+    const Rows<T> orow = rows_of(out, (int64_t)d.heads * d.dim, d.dim, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.ovec ? 8 : 1);
+    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
+    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
+    Chunk<T> qf[RS][DP / 32], gf[RS][DP / 32];
+    float del[RS], L[RS], safe[RS];
+    f32x4 acc[RS][DP / 16];
 #pragma unroll
-        for (int b = 0; b < DP / 32; ++b)
+    for (int x = 0; x < RS; ++x) {
+        const int row = row0 + x * 16;
+        const bool mine = row < nrows;
+        row_chunks<T, DP>(qf[x], qr, row);
+        float s = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int x = b * 32 + g * 8 + e;
-                if (x < d.dim) del += to_f(po[x]) * to_f(pg[x]);
-            }
-    }
-    del = over_groups_sum(del);
-    const float L = mine ? lse[at] : INFINITY, safe = L == -INFINITY ? INFINITY : L;  // no open key: every weight is 0
-    if (mine && g == 0 && blockIdx.z == 0) delta[at] = del;
-    f32x4 acc[DP / 16];
-#pragma unroll
-    for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
-    int kb, ke;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &kb, &ke);
-    for (int k0 = kb; k0 < ke; k0 += KT) {
-        __syncthreads();
-        stage_rows<T, KT, DP, NT>(kl, kr, k0);
-        stage_rows<T, KT, DP, NT>(vl, vr, k0);
-        stage_cols<T, KT, DP, NT>(kc, kr, k0);
-        __syncthreads();
-#pragma unroll
-        for (int p = 0; p < KT / 32; ++p) {
-            f32x4 ds[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = 2 * p + u;
-                f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < DP / 32; ++b) {
-                    s = mma(KTile::get(kl, t * 16 + c, b * 4 + g), qf[b], s);
-                    dp = mma(KTile::get(vl, t * 16 + c, b * 4 + g), gf[b], dp);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float w = kr.has(k0 + t * 16 + g * 4 + e) ? exp2_fast(s[e] * d.scale2 - safe) : 0.f;
-                    ds[u][e] = w * (dp[e] - del);
-                }
-            }
-            const Chunk<T> f = joined<T>(ds[0], ds[1]);
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) acc[t] = mma(KCols::get(kc, t * 16 + c, p * 4 + g), f, acc[t]);
+        for (int b = 0; b < DP / 32; ++b) {
+            Raw<T> a, o;
+            row_raw(a, gr, row, mine, b);
+            row_raw(o, orow, row, mine, b);
+            gf[x][b] = raw_chunk(a);
+            s += raw_dot(a, o);
         }
-    }
-    if (!mine) return;
-    // a row without an open key has dQ = 0 whatever dO and O hold
+        del[x] = over_groups_sum(s);
+        const int64_t at = (int64_t)(sp.qs + (mine ? row / d.group : 0)) * d.heads + hk * d.group + (mine ? row % d.group : 0);
+        L[x] = mine ? lse[at] : INFINITY;
+        safe[x] = L[x] == -INFINITY ? INFINITY : L[x];  // no open key: every weight is 0
+        if (mine && g == 0 && blockIdx.z == 0) delta[at] = del[x];
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-        const f32x4 r = L == -INFINITY ? f32x4{0, 0, 0, 0} : acc[t] * d.scale;
-        const int n = d.dim - t * 16 - g * 4;
-        if (d.splits > 1)
-            store4(part + (blockIdx.z * (int64_t)d.rows_q * d.heads + at) * d.dim + t * 16 + g * 4, r, n, d.dim % 4 == 0);
-        else
-            store4(dq + at * d.dim + t * 16 + g * 4, r, n, d.ovec);
+        for (int t = 0; t < DP / 16; ++t) acc[x][t] = f32x4{0, 0, 0, 0};
+    }
+    Stage ks, vs;
+    const uint32_t at_lds = lds_offset(lds);
+    int tb, te;
+    split_range(kr.n, KT, d.splits, blockIdx.z, &tb, &te);
+    over_tiles<2 * Stage::U, DMA>(
+        tb, te, [&](int i) { return kr.template open<KT>(i * KT); },
+        [&](int i, uint64_t open, int buf) {
+            ks.load(kr, i * KT, open, at_lds + buf * BUF);
+            vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
+        },
+        [&](int buf) {
+            ks.store(lds + buf * BUF);
+            vs.store(lds + buf * BUF + KTile::BYTES);
+        },
+        [&](int, uint64_t open, int buf) {
+            const char* kl = lds + buf * BUF;
+            const char* vl = kl + KTile::BYTES;
+#pragma unroll
+            for (int p = 0; p < KT / 32; ++p) {
+                f32x4 s[RS][2], dp[RS][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int x = 0; x < RS; ++x) s[x][u] = dp[x][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int b = 0; b < DP / 32; ++b) {
+                        const Chunk<T> kf = KTile::get(kl, sub_row(2 * p + u), b * 4 + g);
+                        const Chunk<T> vf = KTile::get(vl, sub_row(2 * p + u), b * 4 + g);
+#pragma unroll
+                        for (int x = 0; x < RS; ++x) {
+                            s[x][u] = mma(kf, qf[x][b], s[x][u]);
+                            dp[x][u] = mma(vf, gf[x][b], dp[x][u]);
+                        }
+                    }
+                }
+                const uint32_t bits = (uint32_t)(open >> (32 * p + 8 * g));
+                Chunk<T> f[RS];
+#pragma unroll
+                for (int x = 0; x < RS; ++x) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float w = exp2_fast(__builtin_fmaf(s[x][u][e], d.scale2, -safe[x])) * (dp[x][u][e] - del[x]);
+                            s[x][u][e] = bits >> (4 * u + e) & 1 ? w : 0.f;
+                        }
+                    f[x] = joined<T>(s[x][0], s[x][1]);
+                }
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    const Chunk<T> kc = KTile::get_across(kl, p * 32, t);
+#pragma unroll
+                    for (int x = 0; x < RS; ++x) acc[x][t] = mma(kc, f[x], acc[x][t]);
+                }
+            }
+        });
+#pragma unroll
+    for (int x = 0; x < RS; ++x) {
+        const int row = row0 + x * 16;
+        if (row >= nrows) continue;
+        const int64_t at = (int64_t)(sp.qs + row / d.group) * d.heads + hk * d.group + row % d.group;
+        // a row without an open key has dQ = 0 whatever dO and O hold
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            const f32x4 r = L[x] == -INFINITY ? f32x4{0, 0, 0, 0} : acc[x][t] * d.scale;
+            const int n = d.dim - t * 16 - g * 4;
+            if (d.splits > 1)
+                store4(part + (blockIdx.z * (int64_t)d.rows_q * d.heads + at) * d.dim + t * 16 + g * 4, r, n, d.dim % 4 == 0);
+            else
+                store4(dq + at * d.dim + t * 16 + g * 4, r, n, d.ovec);
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// dK, dV: WAVES waves of 16 keys each; all rows (of all heads that read the keys) go by in tiles of RT
+// dK, dV: WAVES waves of KS x 16 keys each; all rows (of all heads that read the keys) go by in tiles of RT
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int RT>
+template <class T, int DP, int WAVES, int KS, int RT, bool DMA>
 __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const T* __restrict__ dout,
                                                              const float* __restrict__ lse, const float* __restrict__ delta,
                                                              T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TK = WAVES * 16;
-    using RTile = Tile<T, RT, DP / 8>;
-    using CTile = Tile<T, DP, RT / 8>;
+    constexpr int NT = WAVES * 64, TK = WAVES * KS * 16;
+    using Stage = RowStage<T, RT, DP, NT, DMA>;
+    using RTile = typename Stage::Lds;
+    constexpr int STAT = 2 * RTile::BYTES, BUF = STAT + 2 * 64 * 4;  // Q, dO, then 64 values of L and of delta each
+    constexpr int STATS = WAVES > 1 ? 1 : 2;                         // stat loads of a wave a tile
     extern __shared__ __align__(16) char lds[];
-    char* ql = lds;
-    char* gl = ql + RTile::BYTES;
-    char* qc = gl + RTile::BYTES;
-    char* gc = qc + CTile::BYTES;
-    float* stat = reinterpret_cast<float*>(gc + CTile::BYTES);  // [2][RT]: L, delta
-    const Span sp = find_span(d, true, TK, 1, blockIdx.x);
-    const int hk = blockIdx.y, k0 = sp.tile * TK, nkeys = sp.ke - sp.ks, nrows = (sp.qe - sp.qs) * d.group;
+    const int hk = blockIdx.x % d.kv_heads;
+    const Span sp = find_span(d, true, TK, 1, blockIdx.x / d.kv_heads);
+    const int k0 = sp.tile * TK, nkeys = sp.ke - sp.ks, nrows = (sp.qe - sp.qs) * d.group;
     if (k0 >= nkeys) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int key = k0 + wave * 16 + c;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.qvec);
-    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, nullptr, d.dovec);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.kvec);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.vvec);
-    Chunk<T> kf[DP / 32], vf[DP / 32];
-    row_chunks<T, DP>(kf, kr, key);
-    row_chunks<T, DP>(vf, vr, key);
-    const bool open = kr.has(key);
-    f32x4 ak[DP / 16], av[DP / 16];
+    const int key0 = k0 + wave * KS * 16 + c;
+    const uint8_t* no = nullptr;
+    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
+    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
+    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.kvw);
+    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.vvw);
+    // row r's statistics lie at (qs + r / group) heads + hk group + r % group
+    const int64_t stat0 = (int64_t)sp.qs * d.heads + hk * d.group;
+    auto stat_at = [&](int r) { return (int64_t)(r / d.group) * d.heads + r % d.group; };
+    Chunk<T> kf[KS][DP / 32], vf[KS][DP / 32];
+    bool open_key[KS];
+    f32x4 ak[KS][DP / 16], av[KS][DP / 16];
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) ak[t] = av[t] = f32x4{0, 0, 0, 0};
-    int rb, re;
-    split_range(nrows, RT, d.splits, blockIdx.z, &rb, &re);
-    for (int r0 = rb; r0 < re; r0 += RT) {
-        __syncthreads();
-        stage_rows<T, RT, DP, NT>(ql, qr, r0);
-        stage_rows<T, RT, DP, NT>(gl, gr, r0);
-        stage_cols<T, RT, DP, NT>(qc, qr, r0);
-        stage_cols<T, RT, DP, NT>(gc, gr, r0);
-        for (int u = threadIdx.x; u < RT; u += NT) {
-            const int r = r0 + u;
-            float L = INFINITY, del = 0.f;  // a missing row's weights are 0
-            if (r < nrows) {
-                const int64_t at = (int64_t)(sp.qs + r / d.group) * d.heads + hk * d.group + r % d.group;
-                L = lse[at];
-                L = L == -INFINITY ? INFINITY : L;
-                del = delta[at];
-            }
-            stat[u] = L;
-            stat[RT + u] = del;
-        }
-        __syncthreads();
+    for (int x = 0; x < KS; ++x) {
+        row_chunks<T, DP>(kf[x], kr, key0 + x * 16);
+        row_chunks<T, DP>(vf[x], vr, key0 + x * 16);
+        open_key[x] = kr.has(key0 + x * 16);
 #pragma unroll
-        for (int p = 0; p < RT / 32; ++p) {
-            f32x4 w[2], ds[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = 2 * p + u;
-                f32x4 s = {0, 0, 0, 0}, dp = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < DP / 32; ++b) {
-                    s = mma(RTile::get(ql, t * 16 + c, b * 4 + g), kf[b], s);
-                    dp = mma(RTile::get(gl, t * 16 + c, b * 4 + g), vf[b], dp);
-                }
-                const f32x4 L = *reinterpret_cast<const f32x4*>(stat + t * 16 + g * 4);
-                const f32x4 del = *reinterpret_cast<const f32x4*>(stat + RT + t * 16 + g * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[u][e] = open ? exp2_fast(s[e] * d.scale2 - L[e]) : 0.f;
-                    ds[u][e] = open ? w[u][e] * (dp[e] - del[e]) : 0.f;
-                }
-            }
-            const Chunk<T> pf = joined<T>(w[0], w[1]), df = joined<T>(ds[0], ds[1]);
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) {
-                av[t] = mma(CTile::get(gc, t * 16 + c, p * 4 + g), pf, av[t]);
-                ak[t] = mma(CTile::get(qc, t * 16 + c, p * 4 + g), df, ak[t]);
-            }
-        }
+        for (int t = 0; t < DP / 16; ++t) ak[x][t] = av[x][t] = f32x4{0, 0, 0, 0};
     }
-    if (key >= nkeys) return;
-    const int64_t all = (int64_t)d.rows_k * d.kv_heads, at = (int64_t)(sp.ks + key) * d.kv_heads + hk;
+    Stage qs, gs;
+    float stat_reg = 0.f;
+    const uint32_t at_lds = lds_offset(lds);
+    int tb, te;
+    split_range(nrows, RT, d.splits, blockIdx.z, &tb, &te);
+    over_tiles<2 * Stage::U + STATS, DMA>(
+        tb, te, [&](int i) { return qr.template open<RT>(i * RT); },
+        [&](int i, uint64_t open, int buf) {
+            qs.load(qr, i * RT, open, at_lds + buf * BUF);
+            gs.load(gr, i * RT, open, at_lds + buf * BUF + RTile::BYTES);
+            // a missing row: its Q, dO, L and delta are zeros, and so is what it adds
+            if constexpr (DMA) {
+                const int64_t first = stat_at(i * RT);
+                const uint32_t off = (open >> lane & 1) && lane < RT ? (uint32_t)((stat_at(i * RT + lane) - first) * 4) : DMA_NOWHERE;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
-        const int x = t * 16 + g * 4, n = d.dim - x;
-        // a masked key's gradients are 0 whatever the rows that do not read it hold
-        const f32x4 rk = open ? ak[t] * d.scale : f32x4{0, 0, 0, 0}, rv = open ? av[t] : f32x4{0, 0, 0, 0};
-        if (d.splits > 1) {
-            store4(part + (blockIdx.z * all + at) * d.dim + x, rk, n, d.dim % 4 == 0);
-            store4(part + ((d.splits + blockIdx.z) * all + at) * d.dim + x, rv, n, d.dim % 4 == 0);
-        } else {
-            store4(dk + at * d.dim + x, rk, n, d.ovec);
-            store4(dv + at * d.dim + x, rv, n, d.ovec);
+                for (int w = 0; w < STATS; ++w) {
+                    const int which = STATS == 2 ? w : wave & 1;
+                    dma_load4(dma_buffer((which ? delta : lse) + stat0 + first), off, at_lds + buf * BUF + STAT + which * 256);
+                }
+            } else if (threadIdx.x < 2 * RT || NT < 2 * RT) {
+                static_assert(NT >= 2 * RT, "a thread a value");
+                const int r = threadIdx.x % RT;
+                stat_reg = open >> r & 1 ? (threadIdx.x / RT ? delta : lse)[stat0 + stat_at(i * RT + r)] : 0.f;
+            }
+        },
+        [&](int buf) {
+            qs.store(lds + buf * BUF);
+            gs.store(lds + buf * BUF + RTile::BYTES);
+            if (!DMA && threadIdx.x < 2 * RT)
+                reinterpret_cast<float*>(lds + buf * BUF + STAT)[threadIdx.x / RT * 64 + threadIdx.x % RT] = stat_reg;
+        },
+        [&](int, uint64_t, int buf) {
+            const char* ql = lds + buf * BUF;
+            const char* gl = ql + RTile::BYTES;
+            const float* stat = reinterpret_cast<const float*>(ql + STAT);
+#pragma unroll
+            for (int p = 0; p < RT / 32; ++p) {
+                f32x4 s[KS][2], dp[KS][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) s[x][u] = dp[x][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int b = 0; b < DP / 32; ++b) {
+                        const Chunk<T> qf = RTile::get(ql, sub_row(2 * p + u), b * 4 + g);
+                        const Chunk<T> gf = RTile::get(gl, sub_row(2 * p + u), b * 4 + g);
+#pragma unroll
+                        for (int x = 0; x < KS; ++x) {
+                            s[x][u] = mma(qf, kf[x][b], s[x][u]);
+                            dp[x][u] = mma(gf, vf[x][b], dp[x][u]);
+                        }
+                    }
+                }
+                Chunk<T> pf[KS], df[KS];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const f32x4 L = *reinterpret_cast<const f32x4*>(stat + 32 * p + 8 * g + 4 * u);
+                    const f32x4 del = *reinterpret_cast<const f32x4*>(stat + 64 + 32 * p + 8 * g + 4 * u);
+#pragma unroll
+                    for (int x = 0; x < KS; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float w = exp2_fast(__builtin_fmaf(s[x][u][e], d.scale2, -L[e]));
+                            s[x][u][e] = open_key[x] ? w : 0.f;
+                            dp[x][u][e] = open_key[x] ? w * (dp[x][u][e] - del[e]) : 0.f;
+                        }
+                }
+#pragma unroll
+                for (int x = 0; x < KS; ++x) {
+                    pf[x] = joined<T>(s[x][0], s[x][1]);
+                    df[x] = joined<T>(dp[x][0], dp[x][1]);
+                }
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    const Chunk<T> gc = RTile::get_across(gl, p * 32, t);
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) av[x][t] = mma(gc, pf[x], av[x][t]);
+                    const Chunk<T> qc = RTile::get_across(ql, p * 32, t);
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) ak[x][t] = mma(qc, df[x], ak[x][t]);
+                }
+            }
+        });
+    const int64_t all = (int64_t)d.rows_k * d.kv_heads;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+        const int key = key0 + x * 16;
+        if (key >= nkeys) continue;
+        const int64_t at = (int64_t)(sp.ks + key) * d.kv_heads + hk;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            const int y = t * 16 + g * 4, n = d.dim - y;
+            // a masked key's gradients are 0 whatever the rows that do not read it hold
+            const f32x4 zero = {0, 0, 0, 0}, rk = open_key[x] ? ak[x][t] * d.scale : zero, rv = open_key[x] ? av[x][t] : zero;
+            if (d.splits > 1) {
+                store4(part + (blockIdx.z * all + at) * d.dim + y, rk, n, d.dim % 4 == 0);
+                store4(part + ((d.splits + blockIdx.z) * all + at) * d.dim + y, rv, n, d.dim % 4 == 0);
+            } else {
+                store4(dk + at * d.dim + y, rk, n, d.ovec);
+                store4(dv + at * d.dim + y, rv, n, d.ovec);
+            }
         }
     }
 }
@@ -476,9 +695,18 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-// One wave a tile where the graphs are small (its 16 rows fill it at least as well as 64 would), four otherwise.
-static int att_waves(int64_t rows, int graphs) { return rows <= 32 * (int64_t)(graphs < 1 ? 1 : graphs) ? 1 : 4; }
-static int att_slots(int64_t rows, int graphs, int tile) { return (int)(rows / tile) + graphs + 2; }
+// How a side (queries of all heads of a group, or keys) is cut into tiles
+enum { SIDE_16, SIDE_64, SIDE_128 };
+static const int SIDE_ROWS[3] = {16, 64, 128};
+// One wave of 16 rows where the graphs are small (its tile is filled at least as well as one of 64 rows), 32 rows a wave where
+// they are long (each tile of the other side then feeds twice the products an LDS read).  Values that no 16-byte load fits
+// have the middle instance alone; f32 has no 128 (its three planes of twice the rows do not fit the registers).
+static int att_side(int64_t rows, int graphs, bool f32, bool aligned) {
+    const int64_t each = rows / (graphs < 1 ? 1 : graphs);
+    if (!f32 && !aligned) return SIDE_64;
+    return each <= 32 ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
+}
+static int att_slots(int64_t rows, int graphs, int tile) { return (int)((rows + (int64_t)(graphs + 2) * (tile - 1)) / tile); }
 // Shares of the other side's tiles: enough workgroups for the 256 CUs, and four tiles of 64 a share at least.
 static int att_splits(int64_t workgroups, int64_t other, int graphs) {
     const int64_t want = 1024 / (workgroups < 1 ? 1 : workgroups), most = other / (graphs < 1 ? 1 : graphs) / 256;
@@ -486,19 +714,37 @@ static int att_splits(int64_t workgroups, int64_t other, int graphs) {
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
+static int att_width(const void* p, int64_t row, int64_t head, int dim, int es) {
+    int w = load_width(es, dim, row, p);
+    while (w > 1 && head % w != 0) w /= 2;
+    return w;
+}
+// 16-byte loads, and what a tile spans within the 2 GiB that a buffer's offsets reach
+static bool att_aligned(const tsd_attention& a, const void* dout, int64_t do_row, int64_t do_head) {
+    const int es = a.dtype == TSD_F32 ? 4 : 2, group = a.heads / a.kv_heads;
+    auto near = [&](int64_t row, int64_t head) { return row >= 0 && head >= 0 && 129 * row + group * head < (1ll << 29); };
+    return att_width(a.q, a.q_row, a.q_head, a.dim, es) == 8 && att_width(a.k, a.k_row, a.k_head, a.dim, es) == 8 &&
+           att_width(a.v, a.v_row, a.v_head, a.dim, es) == 8 && near(a.q_row, a.q_head) && near(a.k_row, a.k_head) &&
+           near(a.v_row, a.v_head) &&
+           (dout == nullptr || (att_width(dout, do_row, do_head, a.dim, es) == 8 && near(do_row, do_head)));
+}
+
 struct AttPlan {
-    int wq, wk, splits_q, splits_k;  // waves a tile; shares of the keys (forward, dQ) and of the rows (dK, dV)
-    size_t fwd, bwd;                 // scratch floats
-    size_t part;                     // where the backward's parts begin (behind delta)
+    int side_q, side_k, splits_q, splits_k;  // tiles; shares of the keys (forward, dQ) and of the rows (dK, dV)
+    size_t fwd, bwd;                         // scratch floats
+    size_t part;                             // where the backward's parts begin (behind delta)
 };
-static AttPlan att_plan(const tsd_attention& a) {
+// (the sizes of the scratch do not depend on strides or addresses: the query function sees the same)
+static AttPlan att_plan(const tsd_attention& a, bool aligned) {
     AttPlan p = {};
     const int group = a.heads / a.kv_heads;
+    const bool f32 = a.dtype == TSD_F32;
     const int64_t rows = (int64_t)a.num_queries * group, keys = a.num_keys;
-    p.wq = att_waves(rows, a.num_graphs);
-    p.wk = att_waves(keys, a.num_graphs);
-    p.splits_q = att_splits((rows / (16 * p.wq) + a.num_graphs) * a.kv_heads, keys, a.num_graphs);
-    p.splits_k = att_splits((keys / (16 * p.wk) + a.num_graphs) * a.kv_heads, rows, a.num_graphs);
+    auto tiles = [&](int64_t n) { return (n / SIDE_ROWS[att_side(n, a.num_graphs, f32, true)] + a.num_graphs) * a.kv_heads; };
+    p.side_q = att_side(rows, a.num_graphs, f32, aligned);
+    p.side_k = att_side(keys, a.num_graphs, f32, aligned);
+    p.splits_q = att_splits(tiles(rows), keys, a.num_graphs);
+    p.splits_k = att_splits(tiles(keys), rows, a.num_graphs);
     const size_t nq = (size_t)a.num_queries * a.heads, nk = (size_t)keys * a.kv_heads;
     p.fwd = p.splits_q > 1 ? p.splits_q * nq * (a.dim + 2) : 0;
     const size_t q = p.splits_q > 1 ? p.splits_q * nq * a.dim : 0, k = p.splits_k > 1 ? 2 * p.splits_k * nk * a.dim : 0;
@@ -514,8 +760,8 @@ static int att_check(const char* name, const tsd_attention* a) {
                     a->heads % a->kv_heads == 0 && a->dim >= 1,
                 "%s: bad sizes: %d graphs, %d queries, %d keys, %d heads, %d key heads, dim %d", name, a->num_graphs,
                 a->num_queries, a->num_keys, a->heads, a->kv_heads, a->dim);
-    if (a->dim > TSD_ATTENTION_MAX_DIM || a->kv_heads > 65535 || (int64_t)a->num_queries * a->heads > (1 << 30) ||
-        (int64_t)a->num_keys * a->heads > (1 << 30) || a->num_graphs > (1 << 22)) {
+    if (a->dim > TSD_ATTENTION_MAX_DIM || (int64_t)a->num_queries * a->heads > (1 << 30) ||
+        (int64_t)a->num_keys * a->heads > (1 << 30) || (int64_t)a->num_graphs * a->kv_heads > (1 << 22)) {
         set_error("%s: head dim %d (at most %d), %d queries, %d keys, %d heads, %d graphs", name, a->dim, TSD_ATTENTION_MAX_DIM,
                   a->num_queries, a->num_keys, a->heads, a->num_graphs);
         return TSD_ERR_UNSUPPORTED;
@@ -524,10 +770,6 @@ static int att_check(const char* name, const tsd_attention* a) {
     TSD_REQUIRE(a->num_queries == 0 || a->q != nullptr, "%s: null pointer", name);
     TSD_REQUIRE(a->num_keys == 0 || (a->k != nullptr && a->v != nullptr), "%s: null pointer", name);
     return TSD_OK;
-}
-static bool att_vec(const void* p, int64_t row, int64_t head, int dim, int es) {
-    const int v = 16 / es;
-    return dim % 8 == 0 && row % v == 0 && head % v == 0 && aligned16(p);
 }
 static AttDims att_dims(const tsd_attention& a) {
     AttDims d = {};
@@ -547,100 +789,121 @@ static AttDims att_dims(const tsd_attention& a) {
     d.v_head = a.v_head;
     d.scale = a.scale;
     d.scale2 = a.scale * LOG2E;
-    d.qvec = att_vec(a.q, a.q_row, a.q_head, a.dim, es);
-    d.kvec = att_vec(a.k, a.k_row, a.k_head, a.dim, es);
-    d.vvec = att_vec(a.v, a.v_row, a.v_head, a.dim, es);
+    d.qvw = att_width(a.q, a.q_row, a.q_head, a.dim, es);
+    d.kvw = att_width(a.k, a.k_row, a.k_head, a.dim, es);
+    d.vvw = att_width(a.v, a.v_row, a.v_head, a.dim, es);
     d.q_ptr = a.q_ptr;
     d.k_ptr = a.k_ptr;
     d.mask = a.key_mask;
     return d;
 }
 
-template <class T, int DP, int WAVES>
+// rows of a tile of the other side: what keeps three workgroups (f32 of 128 values: one) on a CU
+template <class T, int DP, int WAVES> constexpr int att_tile() {
+    return WAVES == 1 || DP == 128 || (sizeof(T) == 4 && DP > 32) ? 32 : 64;
+}
+template <class T, int DP, int WAVES, int RS, bool DMA>
 static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse, float* scratch, hipStream_t st) {
-    constexpr int KT = WAVES == 1 ? 32 : ATT_KT;
-    constexpr int lds = Tile<T, KT, DP / 8>::BYTES + Tile<T, DP, KT / 8>::BYTES;
+    constexpr int KT = att_tile<T, DP, WAVES>();
+    constexpr int lds = att_buffers<DMA>() * 2 * Tile<T, KT, DP / 8>::BYTES;
     static DeviceOnce once;
-    auto k = att_fwd_kernel<T, DP, WAVES, KT>;
+    auto k = att_fwd_kernel<T, DP, WAVES, RS, KT, DMA>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * 16), d.kv_heads, d.splits),
-                       dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k, (const T*)a.v, out, lse, scratch);
+    d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
+    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+                       (const T*)a.v, out, lse, scratch);
     TSD_LAUNCH_CHECK("attention_fwd");
-    if (d.splits > 1) {
-        const int64_t all = (int64_t)d.rows_q * d.heads;
-        hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((all * d.dim + 255) / 256)), dim3(256), 0, st, all, d.dim, d.splits,
-                           scratch, out, lse);
-        TSD_LAUNCH_CHECK("attention_join");
-    }
     return TSD_OK;
 }
-template <class T, int DP, int WAVES>
+template <class T, int DP, int WAVES, int RS, bool DMA>
 static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* dout, const float* lse, float* delta, T* dq,
                          float* part, hipStream_t st) {
-    constexpr int KT = WAVES == 1 || DP == 128 ? 32 : ATT_KT;
-    constexpr int lds = 2 * Tile<T, KT, DP / 8>::BYTES + Tile<T, DP, KT / 8>::BYTES;
+    constexpr int KT = att_tile<T, DP, WAVES>();
+    constexpr int lds = att_buffers<DMA>() * 2 * Tile<T, KT, DP / 8>::BYTES;
     static DeviceOnce once;
-    auto k = att_dq_kernel<T, DP, WAVES, KT>;
+    auto k = att_dq_kernel<T, DP, WAVES, RS, KT, DMA>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * 16), d.kv_heads, d.splits),
-                       dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k, (const T*)a.v, out, dout, lse, delta, dq, part);
+    d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
+    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+                       (const T*)a.v, out, dout, lse, delta, dq, part);
     TSD_LAUNCH_CHECK("attention_dq");
-    if (d.splits > 1) {
-        const int64_t n = (int64_t)d.rows_q * d.heads * d.dim;
-        hipLaunchKernelGGL(att_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, n, d.splits, part, dq,
-                           (const float*)nullptr, (T*)nullptr);
-        TSD_LAUNCH_CHECK("attention_dq_sum");
-    }
     return TSD_OK;
 }
-template <class T, int DP, int WAVES>
+template <class T, int DP, int WAVES, int KS, bool DMA>
 static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, const float* lse, const float* delta, T* dk, T* dv,
                           float* part, hipStream_t st) {
     constexpr int RT = 32;
-    constexpr int lds = 2 * Tile<T, RT, DP / 8>::BYTES + 2 * Tile<T, DP, RT / 8>::BYTES + 2 * RT * 4;
+    constexpr int lds = att_buffers<DMA>() * (2 * Tile<T, RT, DP / 8>::BYTES + 512);
     static DeviceOnce once;
-    auto k = att_dkv_kernel<T, DP, WAVES, RT>;
+    auto k = att_dkv_kernel<T, DP, WAVES, KS, RT, DMA>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_slots(d.rows_k, d.graphs, WAVES * 16), d.kv_heads, d.splits), dim3(WAVES * 64), lds, st, d,
-                       (const T*)a.q, (const T*)a.k, (const T*)a.v, dout, lse, delta, dk, dv, part);
+    d.slots = att_slots(d.rows_k, d.graphs, WAVES * KS * 16);
+    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+                       (const T*)a.v, dout, lse, delta, dk, dv, part);
     TSD_LAUNCH_CHECK("attention_dkv");
-    if (d.splits > 1) {
-        const int64_t n = (int64_t)d.rows_k * d.kv_heads * d.dim;
-        hipLaunchKernelGGL(att_sum_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, st, n, d.splits, part, dk,
-                           part + d.splits * n, dv);
-        TSD_LAUNCH_CHECK("attention_dkv_sum");
-    }
     return TSD_OK;
 }
+// launch<T, DP, waves, subtiles of 16 a wave, DMA> of a side
+#define ATT_BY_SIDE(rc, side, aligned, launch, ...)                                      \
+    if constexpr (sizeof(T) == 4) {                                                      \
+        if (side == SIDE_16) rc = launch<T, DP, 1, 1, false>(__VA_ARGS__);               \
+        else rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                               \
+    } else {                                                                             \
+        if (!(aligned)) rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                    \
+        else if (side == SIDE_16) rc = launch<T, DP, 1, 1, true>(__VA_ARGS__);           \
+        else if (side == SIDE_64) rc = launch<T, DP, 4, 1, true>(__VA_ARGS__);           \
+        else rc = launch<T, DP, 4, 2, true>(__VA_ARGS__);                                \
+    }
 
 template <class T, int DP>
-static int att_fwd(AttDims d, const AttPlan& p, const tsd_attention& a, void* out, float* lse, float* scratch, hipStream_t st) {
+static int att_fwd(AttDims d, const tsd_attention& a, void* out, float* lse, float* scratch, hipStream_t st) {
+    const bool aligned = att_aligned(a, nullptr, 0, 0);
+    const AttPlan p = att_plan(a, aligned);
     d.splits = p.splits_q;
     d.ovec = d.dim % 4 == 0 && aligned16(out);
-    return p.wq == 1 ? att_launch_fwd<T, DP, 1>(d, a, (T*)out, lse, scratch, st)
-                     : att_launch_fwd<T, DP, 4>(d, a, (T*)out, lse, scratch, st);
+    int rc;
+    ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_fwd, d, a, (T*)out, lse, scratch, st);
+    if (rc == TSD_OK && d.splits > 1) {
+        const int64_t all = (int64_t)d.rows_q * d.heads;
+        hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((all * d.dim + 255) / 256)), dim3(256), 0, st, all, d.dim, d.splits,
+                           scratch, (T*)out, lse);
+        TSD_LAUNCH_CHECK("attention_join");
+    }
+    return rc;
 }
 template <class T, int DP>
-static int att_bwd(AttDims d, const AttPlan& p, const tsd_attention& a, const void* out, const void* dout, int64_t do_row,
-                   int64_t do_head, const float* lse, void* dq, void* dk, void* dv, float* scratch, hipStream_t st) {
+static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const void* dout, int64_t do_row, int64_t do_head,
+                   const float* lse, void* dq, void* dk, void* dv, float* scratch, hipStream_t st) {
+    const bool aligned = att_aligned(a, dout, do_row, do_head);
+    const AttPlan p = att_plan(a, aligned);
     float *delta = scratch, *part = scratch + p.part;
     d.do_row = do_row;
     d.do_head = do_head;
-    d.dovec = att_vec(dout, do_row, do_head, d.dim, sizeof(T));
+    d.dovw = att_width(dout, do_row, do_head, d.dim, sizeof(T));
     d.ovec = d.dim % 8 == 0 && aligned16(out) && aligned16(dq) && aligned16(dk) && aligned16(dv);
     int rc = TSD_OK;
     if (d.rows_q > 0) {
         d.splits = p.splits_q;
-        rc = p.wq == 1 ? att_launch_dq<T, DP, 1>(d, a, (const T*)out, (const T*)dout, lse, delta, (T*)dq, part, st)
-                       : att_launch_dq<T, DP, 4>(d, a, (const T*)out, (const T*)dout, lse, delta, (T*)dq, part, st);
+        ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_dq, d, a, (const T*)out, (const T*)dout, lse, delta, (T*)dq, part, st);
+        if (rc == TSD_OK && d.splits > 1) {
+            const int64_t n = (int64_t)d.rows_q * d.heads * d.dim;
+            hipLaunchKernelGGL(att_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, n, d.splits, part, (T*)dq,
+                               (const float*)nullptr, (T*)nullptr);
+            TSD_LAUNCH_CHECK("attention_dq_sum");
+        }
     }
     if (rc == TSD_OK && d.rows_k > 0) {
         d.splits = p.splits_k;
-        rc = p.wk == 1 ? att_launch_dkv<T, DP, 1>(d, a, (const T*)dout, lse, delta, (T*)dk, (T*)dv, part, st)
-                       : att_launch_dkv<T, DP, 4>(d, a, (const T*)dout, lse, delta, (T*)dk, (T*)dv, part, st);
+        ATT_BY_SIDE(rc, p.side_k, aligned, att_launch_dkv, d, a, (const T*)dout, lse, delta, (T*)dk, (T*)dv, part, st);
+        if (rc == TSD_OK && d.splits > 1) {
+            const int64_t n = (int64_t)d.rows_k * d.kv_heads * d.dim;
+            hipLaunchKernelGGL(att_sum_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, st, n, d.splits, part, (T*)dk,
+                               part + d.splits * n, (T*)dv);
+            TSD_LAUNCH_CHECK("attention_dkv_sum");
+        }
     }
     return rc;
 }
@@ -655,7 +918,7 @@ extern "C" {
 
 size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backward) {
     if (att_check("tsd_graph_attention_scratch_floats", a) != TSD_OK) return 0;
-    const AttPlan p = att_plan(*a);
+    const AttPlan p = att_plan(*a, true);
     return backward ? p.bwd : p.fwd;
 }
 
@@ -663,16 +926,16 @@ int tsd_graph_attention_fwd(const tsd_attention* a, void* out, float* lse, float
     const int rc = att_check("tsd_graph_attention_fwd", a);
     if (rc != TSD_OK) return rc;
     if (a->num_queries == 0) return TSD_OK;
-    const AttPlan p = att_plan(*a);
+    const AttPlan p = att_plan(*a, true);
     TSD_REQUIRE(out != nullptr, "tsd_graph_attention_fwd: null pointer");
     TSD_REQUIRE(p.fwd == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats >= p.fwd),
                 "tsd_graph_attention_fwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, p.fwd);
     const AttDims d = att_dims(*a);
     hipStream_t st = (hipStream_t)stream;
     TSD_BY_DTYPE(a->dtype, T, {
-        if (d.dim <= 32) return att_fwd<T, 32>(d, p, *a, out, lse, scratch, st);
-        if (d.dim <= 64) return att_fwd<T, 64>(d, p, *a, out, lse, scratch, st);
-        return att_fwd<T, 128>(d, p, *a, out, lse, scratch, st);
+        if (d.dim <= 32) return att_fwd<T, 32>(d, *a, out, lse, scratch, st);
+        if (d.dim <= 64) return att_fwd<T, 64>(d, *a, out, lse, scratch, st);
+        return att_fwd<T, 128>(d, *a, out, lse, scratch, st);
     });
     return TSD_OK;
 }
@@ -681,7 +944,7 @@ int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float
                             int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream) {
     const int rc = att_check("tsd_graph_attention_bwd", a);
     if (rc != TSD_OK) return rc;
-    const AttPlan p = att_plan(*a);
+    const AttPlan p = att_plan(*a, true);
     TSD_REQUIRE(a->num_queries == 0 || (out != nullptr && lse != nullptr && dout != nullptr && dq != nullptr),
                 "tsd_graph_attention_bwd: null pointer");
     TSD_REQUIRE(a->num_keys == 0 || (dk != nullptr && dv != nullptr), "tsd_graph_attention_bwd: null pointer");
@@ -690,9 +953,9 @@ int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float
     const AttDims d = att_dims(*a);
     hipStream_t st = (hipStream_t)stream;
     TSD_BY_DTYPE(a->dtype, T, {
-        if (d.dim <= 32) return att_bwd<T, 32>(d, p, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
-        if (d.dim <= 64) return att_bwd<T, 64>(d, p, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
-        return att_bwd<T, 128>(d, p, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        if (d.dim <= 32) return att_bwd<T, 32>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        if (d.dim <= 64) return att_bwd<T, 64>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        return att_bwd<T, 128>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
     });
     return TSD_OK;
 }

@@ -32,10 +32,65 @@ struct GatedDims {
     int rows, in, out, outp;  // outp: out rounded up to 8, the width of each half of D
     int64_t ldx, lddh;
     int kind;
-    bool xvec, wvec, hvec, dhvec;
+    int xvw, wvw, dhvw, hvw, dxvw;  // values a load or store of x, the weights, dh, h, dx may take
 };
 
-template <class T, int BM, int BN, bool BWD>
+// A tile of BM rows x BC columns in LDS on its way to (from) memory, so that neighbouring lanes touch neighbouring bytes
+template <class T, int BM, int BC> struct OutTile {
+    static constexpr int LD = BC * (int)sizeof(T) + 16, BYTES = BM * LD, CH = BC / 8, UNITS = BM * CH;
+    static constexpr int U = (UNITS + GEMM_WG - 1) / GEMM_WG;
+    __device__ __forceinline__ static T* at(char* lds, int row, int col) { return reinterpret_cast<T*>(lds + row * LD) + col; }
+    __device__ __forceinline__ static void fetch(Raw<T> (&raw)[U], const T* p, int64_t ld, int rows, int cols, int vw) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * GEMM_WG, r = u / CH, c = (u % CH) * 8, n = u < UNITS && r < rows ? cols - c : 0;
+            load_raw(raw[i], p + (n > 0 ? r * ld + c : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
+        }
+    }
+    __device__ __forceinline__ static void keep(const Raw<T> (&raw)[U], char* lds) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * GEMM_WG;
+            if (UNITS % GEMM_WG == 0 || u < UNITS)
+                __builtin_memcpy(__builtin_assume_aligned(at(lds, u / CH, (u % CH) * 8), 16), &raw[i], sizeof(Raw<T>));
+        }
+    }
+    __device__ __forceinline__ static void write(char* lds, T* p, int64_t ld, int rows, int cols, int vw) {
+        if (vw * sizeof(T) >= 16) {
+            constexpr int V = 16 / sizeof(T), CV = BC / V;
+            for (int u = threadIdx.x; u < BM * CV; u += GEMM_WG) {
+                const int r = u / CV, c = (u % CV) * V;
+                if (r < rows && c < cols)
+                    *reinterpret_cast<u32x4*>(p + r * ld + c) = *reinterpret_cast<const u32x4*>(at(lds, r, c));
+            }
+            return;
+        }
+        for (int u = threadIdx.x; u < BM * BC; u += GEMM_WG) {
+            const int r = u / BC, c = u % BC;
+            if (r < rows && c < cols) p[r * ld + c] = *at(lds, r, c);
+        }
+    }
+};
+
+// Registers for f32 (its planes are made there) and for rows that no 16-byte load fits; LDS directly otherwise.
+template <int BM> constexpr int gated_depth() { return BM == 128 ? 1 : BM == 64 ? 2 : 4; }
+constexpr int GATED_STAGES = 4;
+template <class T, int BM, int BN, bool DMA, class NS, class MS, class NRow>
+__device__ __forceinline__ void gated_gemm(char* lds, const NS& ns, const MS& ms, int k, int mrow, NRow nrow,
+                                           f32x4 (&acc)[BN / 32][BM / 32]) {
+    using G = GemmTile<T, BM, BN, NS, MS>;
+    if constexpr (DMA) G::template by_dma<GATED_STAGES>(lds, ns, ms, 0, k, mrow, nrow, acc);
+    else G::template by_registers<gated_depth<BM>()>(lds, ns, ms, 0, k, mrow, nrow, acc);
+}
+template <class T, int BM, int BN, bool DMA> constexpr int gated_lds(int behind) {
+    const int g = (BM + BN) * 64 * Elem<T>::P * (DMA ? GATED_STAGES : 2);
+    return g > behind ? g : behind;
+}
+template <class T, int BM, int BN> constexpr int gated_behind(bool bwd) {
+    return (bwd ? 2 : 1) * OutTile<T, BM, BN / 2>::BYTES + (bwd ? 4 * (BN / 2) * 4 : 0);
+}
+
+template <class T, int BM, int BN, bool DMA, bool BWD>
 __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
                                                         const T* __restrict__ wg, const T* __restrict__ wu,
                                                         const T* __restrict__ bg, const T* __restrict__ bu,
@@ -43,18 +98,26 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
                                                         float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
     constexpr int FT = BN / 2, TN = BN / 64, TM = BM / 32;  // columns a tile; gate (and up) subtiles, row subtiles of a wave
+    using Out = OutTile<T, BM, FT>;
     const TileAt at = tile_at(blockIdx.x, ftiles);
     if (at.lo >= mtiles) return;
     const int m0 = at.lo * BM, f0 = at.sh * FT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave & 1, wm = wave >> 1;
     const int nbase = wn * (FT / 2), mrow = wm * (BM / 2);
-    const RowSource<T> ns = {wg, wu, d.in, d.out, d.in, f0, FT, f0, d.wvec};
-    const RowSource<T> ms = {x, x, d.ldx, d.rows, d.in, m0, BM, 0, d.xvec};
+    const RowOperand<T> ns = {wg, wu, d.in, d.out, d.in, f0, FT, f0, d.wvw};
+    const RowOperand<T> ms = {x, x, d.ldx, d.rows, d.in, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
-    gemm_tile<T, BM, BN>(lds, ns, ms, 0, d.in, mrow,
-                         [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
+    Raw<T> dhr[BWD ? Out::U : 1];
+    if constexpr (BWD) Out::fetch(dhr, dh + (int64_t)m0 * d.lddh + f0, d.lddh, d.rows - m0, d.out - f0, d.dhvw);
+    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, d.in, mrow,
+                               [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
-    float* red = reinterpret_cast<float*>(lds);  // [2 (wm)][2][FT] column sums
+    char* second = lds + Out::BYTES;
+    float* red = reinterpret_cast<float*>(lds + 2 * Out::BYTES);  // [2 (wm)][2][FT] column sums
+    if constexpr (BWD) {
+        Out::keep(dhr, lds);
+        __syncthreads();
+    }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
         const int fl = nbase + j * 16 + c4, f = f0 + fl, nf = d.out - f;
@@ -64,27 +127,26 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
         f32x4 sg = zero, su = zero;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const int m = m0 + mrow + i * 16 + r;
+            const int ml = mrow + i * 16 + r;
             const f32x4 g = acc[j][i] + vbg, u = acc[j + TN][i] + vbu;
+            T* o = Out::at(lds, ml, fl);
             if constexpr (!BWD) {
-                f32x4 o;
+                f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = act_value(d.kind, g[e]) * u[e];
-                if (m < d.rows) store4(h + (int64_t)m * d.out + f, o, nf, d.hvec);
-            } else {
+                for (int e = 0; e < 4; ++e) v[e] = act_value(d.kind, g[e]) * u[e];
+                store4(o, v, 4, true);
+            } else {  // dh's place takes dg; columns and rows outside hold zeros, whatever g and u are there
+                const f32x4 v = load4(o, 4, true);
+                const bool real = m0 + ml < d.rows;
                 f32x4 og = zero, ou = zero;
-                if (m < d.rows) {
-                    const f32x4 v = load4(dh + (int64_t)m * d.lddh + f, nf, d.dhvec);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < nf) {
-                            ou[e] = v[e] * act_value(d.kind, g[e]);
-                            og[e] = v[e] * u[e] * act_slope(d.kind, g[e]);
-                        }
-                    T* o = D + (int64_t)m * 2 * d.outp + f;
-                    store4(o, og, d.outp - f, true);
-                    store4(o + d.outp, ou, d.outp - f, true);
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (real && e < nf) {
+                        ou[e] = v[e] * act_value(d.kind, g[e]);
+                        og[e] = v[e] * u[e] * act_slope(d.kind, g[e]);
+                    }
+                store4(o, og, 4, true);
+                store4(Out::at(second, ml, fl), ou, 4, true);
                 sg += og;
                 su += ou;
             }
@@ -97,16 +159,21 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
                     sg[e] += __shfl_xor(sg[e], s, 64);
                     su[e] += __shfl_xor(su[e], s, 64);
                 }
-                if (r == 0) {  // (gemm_tile ends behind a barrier: the operand tiles are free)
+                if (r == 0) {
                     red[(wm * 2) * FT + fl + e] = sg[e];
                     red[(wm * 2 + 1) * FT + fl + e] = su[e];
                 }
             }
         }
     }
-    if constexpr (BWD) {
+    __syncthreads();
+    if constexpr (!BWD) {
+        Out::write(lds, h + (int64_t)m0 * d.out + f0, d.out, d.rows - m0, d.out - f0, d.hvw);
+    } else {
+        T* o = D + (int64_t)m0 * 2 * d.outp + f0;
+        Out::write(lds, o, 2 * d.outp, d.rows - m0, d.outp - f0, 8);
+        Out::write(second, o + d.outp, 2 * d.outp, d.rows - m0, d.outp - f0, 8);
         if (part == nullptr) return;
-        __syncthreads();
         for (int t = threadIdx.x; t < 2 * FT; t += GEMM_WG) {
             const int f = f0 + t % FT;
             if (f < d.outp) part[(int64_t)at.lo * 2 * d.outp + (t / FT) * d.outp + f] = red[t] + red[2 * FT + t];
@@ -115,45 +182,44 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
 }
 
 // dx[m][k] = sum over f < 2 outp of D[m][f] [Wg; Wu][f][k]
-template <class T, int BM, int BN>
+template <class T, int BM, int BN, bool DMA>
 __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktiles, int mtiles, const T* __restrict__ D,
                                                            const T* __restrict__ wg, const T* __restrict__ wu,
                                                            T* __restrict__ dx) {
     extern __shared__ __align__(16) char lds[];
+    using Out = OutTile<T, BM, BN>;
     const TileAt at = tile_at(blockIdx.x, ktiles);
     if (at.lo >= mtiles) return;
     const int m0 = at.lo * BM, k0 = at.sh * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
-    const ColSource<T> ns = {wg, wu, d.in, d.in, d.out, k0, d.outp, d.wvec};
-    const RowSource<T> ms = {D, D, 2 * d.outp, d.rows, 2 * d.outp, m0, BM, 0, true};
+    const ColOperand<T> ns = {wg, wu, d.in, d.in, d.out, k0, d.outp, d.wvw};
+    const RowOperand<T> ms = {D, D, 2 * d.outp, d.rows, 2 * d.outp, m0, BM, 0, 8};
     f32x4 acc[BN / 32][BM / 32];
-    gemm_tile<T, BM, BN>(lds, ns, ms, 0, 2 * d.outp, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, 2 * d.outp, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
 #pragma unroll
     for (int j = 0; j < BN / 32; ++j)
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
-            const int m = m0 + mrow + i * 16 + r, k = k0 + nbase + j * 16 + c4;
-            if (m < d.rows) store4(dx + (int64_t)m * d.in + k, acc[j][i], d.in - k, d.wvec);
-        }
+        for (int i = 0; i < BM / 32; ++i) store4(Out::at(lds, mrow + i * 16 + r, nbase + j * 16 + c4), acc[j][i], 4, true);
+    __syncthreads();
+    Out::write(lds, dx + (int64_t)m0 * d.in + k0, d.in, d.rows - m0, d.in - k0, d.dxvw);
 }
 
 // part[s][f][k] = sum over the rows of split s of D[m][f] x[m][k]
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktiles, int ftiles, int rows_a_split,
-                                                           const T* __restrict__ D, const T* __restrict__ x,
-                                                           float* __restrict__ part) {
+template <class T, int BM, int BN, bool DMA>
+__global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktiles, int rows_a_split, const T* __restrict__ D,
+                                                           const T* __restrict__ x, float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
     const int k0 = (blockIdx.x % ktiles) * BN, f0 = (blockIdx.x / ktiles) * BM;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
     const int64_t rb = (int64_t)blockIdx.y * rows_a_split;
     const int n = (int)(d.rows - rb < rows_a_split ? d.rows - rb : rows_a_split);
-    const ColSource<T> ns = {x + rb * d.ldx, x, d.ldx, d.in, n, k0, 1 << 30, d.xvec};
-    const ColSource<T> ms = {D + rb * 2 * d.outp, D, 2 * d.outp, 2 * d.outp, n, f0, 1 << 30, true};
+    const ColOperand<T> ns = {x + rb * d.ldx, x, d.ldx, d.in, n, k0, 1 << 30, d.xvw};
+    const ColOperand<T> ms = {D + rb * 2 * d.outp, D, 2 * d.outp, 2 * d.outp, n, f0, 1 << 30, 8};
     f32x4 acc[BN / 32][BM / 32];
-    gemm_tile<T, BM, BN>(lds, ns, ms, 0, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + (int64_t)blockIdx.y * 2 * d.outp * d.in;
 #pragma unroll
@@ -202,31 +268,43 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int wblo
     }
 }
 
-constexpr int GATED_BM = 128, GATED_BN = 128;
-
-static int gated_splits(int rows, int in, int outp, int* rows_a_split) {
-    const int tiles = ((2 * outp + GATED_BM - 1) / GATED_BM) * ((in + GATED_BN - 1) / GATED_BN);
-    int s = (512 + tiles - 1) / tiles;
-    const int most = (rows + 255) / 256;
-    s = s < most ? s : most;
-    s = s < 1 ? 1 : s;
-    int per = (rows + s - 1) / s;
-    per = (per + GEMM_K - 1) / GEMM_K * GEMM_K;
-    per = per < GEMM_K ? GEMM_K : per;
-    if (rows_a_split) *rows_a_split = per;
-    return rows > 0 ? (rows + per - 1) / per : 0;
+// Tiles of an output of m x n: 128 x 128 where they fill the 256 CUs, else 64 x 64, else 32 x 64.
+enum { TILE_128, TILE_64, TILE_32 };
+static const int TILE_M[3] = {128, 64, 32}, TILE_N[3] = {128, 64, 64};
+static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+static int gated_tile(int64_t m, int64_t n, int64_t times) {
+    for (int t = TILE_128; t < TILE_32; ++t)
+        if (times * div_up(m, TILE_M[t]) * div_up(n, TILE_N[t]) >= 256) return t;
+    return TILE_32;
 }
+#define GATED_BY_TILE(tile, BM, BN, ...)                                               \
+    switch (tile) {                                                                    \
+        case TILE_128: { constexpr int BM = 128, BN = 128; __VA_ARGS__; } break;       \
+        case TILE_64: { constexpr int BM = 64, BN = 64; __VA_ARGS__; } break;          \
+        default: { constexpr int BM = 32, BN = 64; __VA_ARGS__; } break;               \
+    }
 
 struct GatedScratch {  // bytes from the start
     size_t D, bpart, wpart, total;
-    int mtiles, splits, rows_a_split;
+    int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
+    int wtile, splits, rows_a_split;   // of dW
 };
 static GatedScratch gated_scratch(int dtype, int rows, int in, int out) {
     GatedScratch s = {};
     const size_t outp = ((size_t)out + 7) / 8 * 8, es = dtype == TSD_F32 ? 4 : 2;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    s.mtiles = (rows + GATED_BM - 1) / GATED_BM;
-    s.splits = gated_splits(rows, in, (int)outp, &s.rows_a_split);
+    s.tile = gated_tile(rows, 2 * outp, 1);
+    s.mtiles = div_up(rows, TILE_M[s.tile]);
+    // dW: the rows in shares of at least 256, about two workgroups a CU
+    const int most = div_up(rows, 256);
+    s.wtile = gated_tile(2 * outp, in, most);
+    if (s.wtile == TILE_32) s.wtile = TILE_64;
+    const int tiles = div_up(2 * outp, TILE_M[s.wtile]) * div_up(in, TILE_N[s.wtile]);
+    int n = div_up(512, tiles);
+    n = n < most ? n : most;
+    n = n < 1 ? 1 : n;
+    s.rows_a_split = div_up(div_up(rows > 0 ? rows : 1, n), GEMM_K) * GEMM_K;
+    s.splits = div_up(rows, s.rows_a_split);
     s.D = 0;
     s.bpart = up((size_t)rows * 2 * outp * es);
     s.wpart = s.bpart + up((size_t)s.mtiles * 2 * outp * 4);
@@ -249,9 +327,7 @@ static int gated_check(const char* name, int32_t dtype, int32_t act, int32_t row
 }
 
 template <class T>
-static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, int64_t ldx, const void* wg, const void* wu,
-                            const void* dx) {
-    const int v = (int)(16 / sizeof(T)) > 8 ? 8 : 8;  // chunks of 8 values: a row of a whole number of them
+static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, int64_t ldx, const void* wg, const void* wu) {
     GatedDims d = {};
     d.rows = rows;
     d.in = in;
@@ -259,71 +335,106 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
     d.outp = (out + 7) / 8 * 8;
     d.ldx = ldx;
     d.kind = act;
-    d.xvec = in % v == 0 && ldx % v == 0 && aligned16(x);
-    d.wvec = in % v == 0 && aligned16(wg) && aligned16(wu) && aligned16(dx);
+    d.xvw = load_width(sizeof(T), in, ldx, x);
+    const int a = load_width(sizeof(T), in, in, wg), b = load_width(sizeof(T), in, in, wu);
+    d.wvw = a < b ? a : b;
     return d;
 }
+// 16-byte loads everywhere, and a tile's rows within the 2 GiB that a buffer's offsets reach
+static bool gated_dma(const GatedDims& d) { return d.xvw == 8 && d.wvw == 8 && d.ldx <= (1 << 22); }
 
-template <class T>
-static int gated_fwd(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, void* h,
-                     hipStream_t st) {
+template <class T, int BM, int BN, bool DMA, bool BWD>
+static int gated_first(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
+                       void* h, void* D, float* part, hipStream_t st) {
     static DeviceOnce once;
-    constexpr int lds = gemm_lds<T, GATED_BM, GATED_BN>();
-    auto k = gated_kernel<T, GATED_BM, GATED_BN, false>;
+    constexpr int lds = gated_lds<T, BM, BN, DMA>(gated_behind<T, BM, BN>(BWD));
+    auto k = gated_kernel<T, BM, BN, DMA, BWD>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    const int ft = (d.out + GATED_BN / 2 - 1) / (GATED_BN / 2), mt = (d.rows + GATED_BM - 1) / GATED_BM;
-    d.hvec = d.out % 4 == 0 && aligned16(h);
+    const int ft = div_up(BWD ? d.outp : d.out, BN / 2), mt = div_up(d.rows, BM);
     hipLaunchKernelGGL(k, dim3(tile_grid(mt, ft)), dim3(GEMM_WG), lds, st, d, ft, mt, (const T*)x, (const T*)wg, (const T*)wu,
-                       (const T*)bg, (const T*)bu, (const T*)nullptr, (T*)h, (T*)nullptr, (float*)nullptr);
-    TSD_LAUNCH_CHECK("gated_fwd");
+                       (const T*)bg, (const T*)bu, (const T*)dh, (T*)h, (T*)D, part);
+    TSD_LAUNCH_CHECK("gated_linear");
     return TSD_OK;
+}
+template <class T, int BM, int BN, bool DMA>
+static int gated_dx(GatedDims d, const T* D, const void* wg, const void* wu, void* dx, hipStream_t st) {
+    static DeviceOnce once;
+    constexpr int lds = gated_lds<T, BM, BN, DMA>(OutTile<T, BM, BN>::BYTES);
+    auto k = gated_dx_kernel<T, BM, BN, DMA>;
+    const int rc = allow_lds(k, lds, once);
+    if (rc != TSD_OK) return rc;
+    const int kt = div_up(d.in, BN), mt = div_up(d.rows, BM);
+    hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt)), dim3(GEMM_WG), lds, st, d, kt, mt, D, (const T*)wg, (const T*)wu, (T*)dx);
+    TSD_LAUNCH_CHECK("gated_dx");
+    return TSD_OK;
+}
+template <class T, int BM, int BN, bool DMA>
+static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* x, float* wpart, hipStream_t st) {
+    static DeviceOnce once;
+    constexpr int lds = gated_lds<T, BM, BN, DMA>(0);
+    auto k = gated_dw_kernel<T, BM, BN, DMA>;
+    const int rc = allow_lds(k, lds, once);
+    if (rc != TSD_OK) return rc;
+    const int kt = div_up(d.in, BN), ft = div_up(2 * d.outp, BM);
+    hipLaunchKernelGGL(k, dim3(kt * ft, s.splits), dim3(GEMM_WG), lds, st, d, kt, s.rows_a_split, D, (const T*)x, wpart);
+    TSD_LAUNCH_CHECK("gated_dw");
+    return TSD_OK;
+}
+// f32 has no instance with loads straight to LDS
+template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
+    GATED_BY_TILE(tile, BM, BN, {
+        if constexpr (sizeof(T) == 2) {
+            if (gated_dma(d)) return gated_first<T, BM, BN, true, BWD>(d, a...);
+        }
+        return gated_first<T, BM, BN, false, BWD>(d, a...);
+    });
 }
 
 template <class T>
 static int gated_bwd(GatedDims d, const GatedScratch& s, const void* x, const void* wg, const void* wu, const void* bg,
                      const void* bu, const void* dh, int64_t lddh, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
                      char* scratch, hipStream_t st) {
-    static DeviceOnce once_d, once_x, once_w;
-    constexpr int lds = gemm_lds<T, GATED_BM, GATED_BN>();
     T* D = reinterpret_cast<T*>(scratch + s.D);
     float* bpart = reinterpret_cast<float*>(scratch + s.bpart);
     float* wpart = reinterpret_cast<float*>(scratch + s.wpart);
     const bool sums = dbg != nullptr || dbu != nullptr, weights = dwg != nullptr || dwu != nullptr;
-    int rc;
+    int rc = TSD_OK;
     if (d.rows > 0) {
         d.lddh = lddh;
-        d.dhvec = d.out % 4 == 0 && lddh % 4 == 0 && aligned16(dh);
-        auto k1 = gated_kernel<T, GATED_BM, GATED_BN, true>;
-        if ((rc = allow_lds(k1, lds, once_d)) != TSD_OK) return rc;
-        const int ft = (d.outp + GATED_BN / 2 - 1) / (GATED_BN / 2);
-        hipLaunchKernelGGL(k1, dim3(tile_grid(s.mtiles, ft)), dim3(GEMM_WG), lds, st, d, ft, s.mtiles, (const T*)x, (const T*)wg,
-                           (const T*)wu, (const T*)bg, (const T*)bu, (const T*)dh, (T*)nullptr, D, sums ? bpart : nullptr);
-        TSD_LAUNCH_CHECK("gated_bwd");
-        const int kt = (d.in + GATED_BN - 1) / GATED_BN;
-        if (dx != nullptr) {
-            auto k2 = gated_dx_kernel<T, GATED_BM, GATED_BN>;
-            if ((rc = allow_lds(k2, lds, once_x)) != TSD_OK) return rc;
-            hipLaunchKernelGGL(k2, dim3(tile_grid(s.mtiles, kt)), dim3(GEMM_WG), lds, st, d, kt, s.mtiles, D, (const T*)wg,
-                               (const T*)wu, (T*)dx);
-            TSD_LAUNCH_CHECK("gated_dx");
+        d.dhvw = load_width(sizeof(T), d.out, lddh, dh);
+        d.dxvw = load_width(sizeof(T), d.in, d.in, dx);
+        rc = gated_first_by<T, true>(s.tile, d, x, wg, wu, bg, bu, dh, (void*)nullptr, (void*)D, sums ? bpart : (float*)nullptr, st);
+        if (rc == TSD_OK && dx != nullptr) {
+            GATED_BY_TILE(gated_tile(d.rows, d.in, 1), BM, BN, {
+                if constexpr (sizeof(T) == 2) {
+                    if (gated_dma(d)) {
+                        rc = gated_dx<T, BM, BN, true>(d, D, wg, wu, dx, st);
+                        break;
+                    }
+                }
+                rc = gated_dx<T, BM, BN, false>(d, D, wg, wu, dx, st);
+            });
         }
-        if (weights) {
-            auto k3 = gated_dw_kernel<T, GATED_BM, GATED_BN>;
-            if ((rc = allow_lds(k3, lds, once_w)) != TSD_OK) return rc;
-            const int f2 = (2 * d.outp + GATED_BM - 1) / GATED_BM;
-            hipLaunchKernelGGL(k3, dim3(kt * f2, s.splits), dim3(GEMM_WG), lds, st, d, kt, f2, s.rows_a_split, D, (const T*)x,
-                               wpart);
-            TSD_LAUNCH_CHECK("gated_dw");
+        if (rc == TSD_OK && weights) {
+            GATED_BY_TILE(s.wtile, BM, BN, {
+                if constexpr (sizeof(T) == 2) {
+                    if (gated_dma(d)) {
+                        rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st);
+                        break;
+                    }
+                }
+                rc = gated_dw<T, BM, BN, false>(d, s, D, x, wpart, st);
+            });
         }
     }
-    if (weights || sums) {
+    if (rc == TSD_OK && (weights || sums)) {
         const int wb = weights ? (int)(((int64_t)2 * d.outp * d.in + 255) / 256) : 0, bb = sums ? (2 * d.outp + 15) / 16 : 0;
         hipLaunchKernelGGL(gated_reduce_kernel<T>, dim3(wb + bb), dim3(256), 0, st, d, wb, s.splits, s.mtiles, wpart, bpart,
                            (T*)dwg, (T*)dwu, (T*)dbg, (T*)dbu);
         TSD_LAUNCH_CHECK("gated_reduce");
     }
-    return TSD_OK;
+    return rc;
 }
 
 }  // namespace blk
@@ -340,8 +451,12 @@ int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
     if (rc != TSD_OK) return rc;
     if (rows == 0) return TSD_OK;
     TSD_REQUIRE(h != nullptr, "tsd_gated_linear_fwd: null pointer");
-    TSD_BY_DTYPE(dtype, T, return gated_fwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, nullptr), x, w_gate,
-                                               w_up, b_gate, b_up, h, (hipStream_t)stream));
+    TSD_BY_DTYPE(dtype, T, {
+        GatedDims d = gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up);
+        d.hvw = load_width(sizeof(T), out, out, h);
+        return gated_first_by<T, false>(gated_tile(rows, 2 * (int64_t)d.outp, 1), d, x, w_gate, w_up, b_gate, b_up,
+                                        (const void*)nullptr, h, (void*)nullptr, (float*)nullptr, (hipStream_t)stream);
+    });
     return TSD_OK;
 }
 
@@ -360,7 +475,7 @@ int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
     TSD_REQUIRE(rows == 0 || (dh != nullptr && lddh >= out), "tsd_gated_linear_bwd: null pointer or row stride");
     TSD_REQUIRE(rows == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats * 4 >= s.total),
                 "tsd_gated_linear_bwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, s.total / 4);
-    TSD_BY_DTYPE(dtype, T, return gated_bwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, dx), s, x, w_gate, w_up,
+    TSD_BY_DTYPE(dtype, T, return gated_bwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up), s, x, w_gate, w_up,
                                                b_gate, b_up, dh, lddh, dx, dw_gate, dw_up, db_gate, db_up, (char*)scratch,
                                                (hipStream_t)stream));
     return TSD_OK;
