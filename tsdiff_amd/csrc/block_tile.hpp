@@ -235,6 +235,12 @@ __device__ __forceinline__ i32x4 dma_buffer(const void* p) {  // 2 GiB from p on
     return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff),
                  0x7fffffff, 0x00027000};
 }
+// the same bounds for loads to registers
+__device__ __forceinline__ f32x4 buffer_load(i32x4 buf, uint32_t off) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+        __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)(uint32_t)buf[0] | (uint64_t)(uint32_t)buf[1] << 32), 0, buf[2], buf[3]),
+        (int)off, 0, 0));
+}
 __device__ __forceinline__ void dma_load(i32x4 buf, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :

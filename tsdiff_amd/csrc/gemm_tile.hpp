@@ -52,29 +52,10 @@ template <class T> struct ColOperand {
     }
 };
 
-// How a tile of N output rows (or columns) comes in.  Registers: U chunks a thread, DEPTH tiles under way.
-template <class T, int N, class Op, int DEPTH> struct RegStage {
-    using Lds = typename Op::template TileOf<N>;
-    static constexpr int UNITS = Lds::ROWS * Lds::C, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
-    Raw<T> raw[DEPTH][U];
-    __device__ __forceinline__ void load(int d, const Op& op, int k) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) op.load(raw[d][i], u / Lds::C, u % Lds::C, k);
-        }
-    }
-    __device__ __forceinline__ void store(int d, char* lds) const {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) Lds::put(lds, u / Lds::C, u % Lds::C, raw_chunk(raw[d][i]));
-        }
-    }
-};
-// Straight to LDS: a wave's 64 lanes fill 64 neighbouring places, so the lane of place p of row r fetches chunk
-// p ^ swizzle(r).  One matrix a load: the 64 places of a wave lie on one side of the operand's split.
-template <class T, int N, class Op> struct DmaStage {
+// Where the chunks of a tile of N output rows (or columns) lie, for 32-bit offsets from a base that is the same for a wave;
+// places outside of the matrix are NOWHERE.  LDS places for loads straight to LDS (PERMUTED): a wave's 64 lanes fill 64
+// neighbouring places, so the lane of place p of row r fetches chunk p ^ swizzle(r).
+template <class T, int N, class Op, bool PERMUTED> struct Places {
     using Lds = typename Op::template TileOf<N>;
     static constexpr int UNITS = Lds::ROWS * Lds::C, U = UNITS < GEMM_WG ? 1 : UNITS / GEMM_WG;
     // (a tile smaller than the workgroup is loaded by several waves alike: every wave counts the same loads)
@@ -86,7 +67,7 @@ template <class T, int N, class Op> struct DmaStage {
         for (int i = 0; i < U; ++i) {
             const int u = (threadIdx.x + i * GEMM_WG) % UNITS;
             row[i] = u / Lds::C;
-            chunk[i] = (u % Lds::C) ^ Lds::swizzle(row[i]);
+            chunk[i] = PERMUTED ? (u % Lds::C) ^ Lds::swizzle(row[i]) : u % Lds::C;
             if constexpr (!Op::ACROSS) {
                 off[i] = op.offset(row[i], chunk[i]);
             } else {
@@ -95,20 +76,64 @@ template <class T, int N, class Op> struct DmaStage {
             }
         }
     }
-    __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) const {
+    // One matrix a load: the 64 places of a wave lie on one side of the operand's split
+    template <class F> __device__ __forceinline__ void each(const Op& op, int k, F f) const {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int wave_row = __builtin_amdgcn_readfirstlane(row[i]);
-            const uint32_t to = lds + (threadIdx.x / 64 * 64 + i * GEMM_WG) % UNITS * 16;
             if constexpr (!Op::ACROSS) {
-                dma_load(dma_buffer(op.base(wave_row >= op.split, k)), k + chunk[i] * 8 < op.kmax ? off[i] : DMA_NOWHERE, to);
+                f(i, dma_buffer(op.base(wave_row >= op.split, k)), k + chunk[i] * 8 < op.kmax ? off[i] : DMA_NOWHERE);
             } else {  // ksplit is a multiple of 8, as few rows as a wave's load may hold: it lies on one side
                 const bool two = k + wave_row >= op.ksplit;
                 const int kk = k - (two ? op.ksplit : 0);
-                dma_load(dma_buffer((two ? op.p2 : op.p) + (int64_t)kk * op.ld + op.first),
-                         kk + row[i] < op.kmax ? off[i] : DMA_NOWHERE, to);
+                f(i, dma_buffer((two ? op.p2 : op.p) + (int64_t)kk * op.ld + op.first),
+                  kk + row[i] < op.kmax ? off[i] : DMA_NOWHERE);
             }
         }
+    }
+};
+
+// A tile by way of registers, DEPTH tiles under way.  FAST (f32): branch-free loads with the bounds in the buffer.
+template <class T, int N, class Op, int DEPTH, bool FAST> struct RegStage {
+    using Lds = typename Op::template TileOf<N>;
+    static constexpr int UNITS = Lds::ROWS * Lds::C, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
+    Raw<T> raw[DEPTH][U];
+    Places<T, N, Op, false> places;
+    __device__ __forceinline__ void init(const Op& op) {
+        if constexpr (FAST) places.init(op);
+    }
+    __device__ __forceinline__ void load(int d, const Op& op, int k) {
+        if constexpr (FAST) {
+            places.each(op, k, [&](int i, i32x4 buf, uint32_t off) {
+                raw[d][i].a = buffer_load(buf, off);
+                raw[d][i].b = buffer_load(buf, off + 16);
+            });
+        } else {
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int u = threadIdx.x + i * GEMM_WG;
+                if (UNITS % GEMM_WG == 0 || u < UNITS) op.load(raw[d][i], u / Lds::C, u % Lds::C, k);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(int d, char* lds) const {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = threadIdx.x + i * GEMM_WG;
+            if (UNITS % GEMM_WG == 0 || u < UNITS) Lds::put(lds, u / Lds::C, u % Lds::C, raw_chunk(raw[d][i]));
+        }
+    }
+};
+// Straight to LDS
+template <class T, int N, class Op> struct DmaStage {
+    using At = Places<T, N, Op, true>;
+    static constexpr int U = At::U;
+    At places;
+    __device__ __forceinline__ void init(const Op& op) { places.init(op); }
+    __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) const {
+        places.each(op, k, [&](int i, i32x4 buf, uint32_t off) {
+            dma_load(buf, off, lds + (threadIdx.x / 64 * 64 + i * GEMM_WG) % At::UNITS * 16);
+        });
     }
 };
 
@@ -144,12 +169,15 @@ template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
             for (int i = 0; i < BM / 32; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
     }
     // One output tile: acc[jn][im] of the calling wave, n rows nrow(jn) and m rows mrow + im * 16 of the tile; ends behind a
-    // barrier.  The next DEPTH tiles' values are on their way into registers; two LDS buffers, one barrier a tile.
-    template <int DEPTH, class NRow>
+    // barrier.  The next DEPTH tiles' values are on their way into registers.  BUFS 2: two LDS buffers, one barrier a tile;
+    // 1: one buffer, two barriers, and twice the workgroups on a CU where LDS is what limits them.
+    template <int DEPTH, int BUFS, bool FAST, class NRow>
     __device__ __forceinline__ static void by_registers(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow,
                                                         NRow nrow, Acc& acc) {
-        RegStage<T, BN, NS, DEPTH> nst;
-        RegStage<T, BM, MS, DEPTH> mst;
+        RegStage<T, BN, NS, DEPTH, FAST> nst;
+        RegStage<T, BM, MS, DEPTH, FAST> mst;
+        nst.init(ns);
+        mst.init(ms);
         clear(acc);
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
@@ -171,7 +199,8 @@ template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
                     mst.load(d, ms, k + DEPTH * GEMM_K);
                 }
                 products(lds + cur * BUF, mrow, nrow, acc);
-                cur ^= 1;
+                if constexpr (BUFS == 2) cur ^= 1;
+                else __syncthreads();
                 if (k + GEMM_K < kend) {
                     nst.store((d + 1) % DEPTH, lds + cur * BUF);
                     mst.store((d + 1) % DEPTH, lds + cur * BUF + NT::BYTES);

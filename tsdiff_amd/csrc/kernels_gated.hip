@@ -8,6 +8,8 @@
 // inputs reading them back in f32 costs more than the products) and writes D = [dg | du] in the tensors' type -- the one
 // rounding of an intermediate, since D is the next two products' matrix operand -- with each row tile's column sums in fp32;
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
+#include <type_traits>
+
 #include "gemm_tile.hpp"
 
 namespace tsd {
@@ -17,12 +19,15 @@ namespace blk {
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-g)); }
 __device__ __forceinline__ float softplus(float g) { return fmaxf(g, 0.f) + log1pf(fast_exp(-fabsf(g))); }
-__device__ __forceinline__ float act_value(int kind, float g) {
+// KIND < 0: any of them, by `kind` (the same in all lanes)
+template <int KIND> __device__ __forceinline__ float act_value(int kind, float g) {
+    if constexpr (KIND >= 0) kind = KIND;
     if (kind == 0) return g * sigmoid(g);
     if (kind == 2) return g < 0.f ? 0.f : g;
     return softplus(g) - (kind == 1 ? 0.693147180559945309f : 0.f);
 }
-__device__ __forceinline__ float act_slope(int kind, float g) {
+template <int KIND> __device__ __forceinline__ float act_slope(int kind, float g) {
+    if constexpr (KIND >= 0) kind = KIND;
     if (kind == 2) return g > 0.f ? 1.f : 0.f;
     const float s = sigmoid(g);
     return kind == 0 ? s * (1.f + g * (1.f - s)) : s;
@@ -32,6 +37,7 @@ struct GatedDims {
     int rows, in, out, outp;  // outp: out rounded up to 8, the width of each half of D
     int64_t ldx, lddh;
     int kind;
+    bool bvec;  // both biases: four values a load
     int xvw, wvw, dhvw, hvw, dxvw;  // values a load or store of x, the weights, dh, h, dx may take
 };
 
@@ -72,26 +78,28 @@ template <class T, int BM, int BC> struct OutTile {
     }
 };
 
-// Registers for f32 (its planes are made there) and for rows that no 16-byte load fits; LDS directly otherwise.
+// FAST: 16-byte loads with bounds in the buffer, straight to LDS for the 16-bit types, by way of registers for f32 (its planes
+// are made there).  Otherwise guarded loads of what width the rows allow.
 template <int BM> constexpr int gated_depth() { return BM == 128 ? 1 : BM == 64 ? 2 : 4; }
-constexpr int GATED_STAGES = 4;
-template <class T, int BM, int BN, bool DMA, class NS, class MS, class NRow>
-__device__ __forceinline__ void gated_gemm(char* lds, const NS& ns, const MS& ms, int k, int mrow, NRow nrow,
+constexpr int GATED_STAGES = 3;
+template <class T, int BM> constexpr int gated_bufs() { return sizeof(T) == 4 && BM == 128 ? 1 : 2; }
+template <class T, int BM, int BN, bool FAST, class NS, class MS, class NRow>
+__device__ __forceinline__ void gated_gemm(char* lds, const NS& ns, const MS& ms, int kb, int ke, int mrow, NRow nrow,
                                            f32x4 (&acc)[BN / 32][BM / 32]) {
     using G = GemmTile<T, BM, BN, NS, MS>;
-    if constexpr (DMA) G::template by_dma<GATED_STAGES>(lds, ns, ms, 0, k, mrow, nrow, acc);
-    else G::template by_registers<gated_depth<BM>()>(lds, ns, ms, 0, k, mrow, nrow, acc);
+    if constexpr (FAST && sizeof(T) == 2) G::template by_dma<GATED_STAGES>(lds, ns, ms, kb, ke, mrow, nrow, acc);
+    else G::template by_registers<gated_depth<BM>(), gated_bufs<T, BM>(), FAST>(lds, ns, ms, kb, ke, mrow, nrow, acc);
 }
-template <class T, int BM, int BN, bool DMA> constexpr int gated_lds(int behind) {
-    const int g = (BM + BN) * 64 * Elem<T>::P * (DMA ? GATED_STAGES : 2);
+template <class T, int BM, int BN, bool FAST> constexpr int gated_lds(int behind) {
+    const int g = (BM + BN) * 64 * Elem<T>::P * (FAST && sizeof(T) == 2 ? GATED_STAGES : gated_bufs<T, BM>());
     return g > behind ? g : behind;
 }
 template <class T, int BM, int BN> constexpr int gated_behind(bool bwd) {
     return (bwd ? 2 : 1) * OutTile<T, BM, BN / 2>::BYTES + (bwd ? 4 * (BN / 2) * 4 : 0);
 }
 
-template <class T, int BM, int BN, bool DMA, bool BWD>
-__global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
+template <class T, int BM, int BN, bool FAST, bool BWD>
+__global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
                                                         const T* __restrict__ wg, const T* __restrict__ wu,
                                                         const T* __restrict__ bg, const T* __restrict__ bu,
                                                         const T* __restrict__ dh, T* __restrict__ h, T* __restrict__ D,
@@ -107,65 +115,77 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
     const RowOperand<T> ns = {wg, wu, d.in, d.out, d.in, f0, FT, f0, d.wvw};
     const RowOperand<T> ms = {x, x, d.ldx, d.rows, d.in, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
+    const int r = lane & 15, c4 = (lane >> 4) * 4;
+    f32x4 vbg[TN], vbu[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int f = f0 + nbase + j * 16 + c4, nf = d.out - f;
+        const f32x4 zero = {0, 0, 0, 0};
+        vbg[j] = bg != nullptr ? load4(bg + f, nf, d.bvec) : zero;
+        vbu[j] = bu != nullptr ? load4(bu + f, nf, d.bvec) : zero;
+    }
     Raw<T> dhr[BWD ? Out::U : 1];
     if constexpr (BWD) Out::fetch(dhr, dh + (int64_t)m0 * d.lddh + f0, d.lddh, d.rows - m0, d.out - f0, d.dhvw);
-    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, d.in, mrow,
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.in, mrow,
                                [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
-    const int r = lane & 15, c4 = (lane >> 4) * 4;
     char* second = lds + Out::BYTES;
     float* red = reinterpret_cast<float*>(lds + 2 * Out::BYTES);  // [2 (wm)][2][FT] column sums
     if constexpr (BWD) {
         Out::keep(dhr, lds);
         __syncthreads();
     }
+    // (swish has code of its own: with all kinds' in every place of the unrolled loops the code outgrows its cache)
+    auto epilogue = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int fl = nbase + j * 16 + c4, f = f0 + fl, nf = d.out - f;
-        const f32x4 zero = {0, 0, 0, 0};
-        const f32x4 vbg = bg != nullptr ? load4(bg + f, nf, false) : zero;
-        const f32x4 vbu = bu != nullptr ? load4(bu + f, nf, false) : zero;
-        f32x4 sg = zero, su = zero;
+        for (int j = 0; j < TN; ++j) {
+            const int fl = nbase + j * 16 + c4, f = f0 + fl, nf = d.out - f;
+            const f32x4 zero = {0, 0, 0, 0};
+            f32x4 sg = zero, su = zero;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int ml = mrow + i * 16 + r;
-            const f32x4 g = acc[j][i] + vbg, u = acc[j + TN][i] + vbu;
-            T* o = Out::at(lds, ml, fl);
-            if constexpr (!BWD) {
-                f32x4 v;
+            for (int i = 0; i < TM; ++i) {
+                const int ml = mrow + i * 16 + r;
+                const f32x4 g = acc[j][i] + vbg[j], u = acc[j + TN][i] + vbu[j];
+                T* o = Out::at(lds, ml, fl);
+                if constexpr (!BWD) {
+                    f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = act_value(d.kind, g[e]) * u[e];
-                store4(o, v, 4, true);
-            } else {  // dh's place takes dg; columns and rows outside hold zeros, whatever g and u are there
-                const f32x4 v = load4(o, 4, true);
-                const bool real = m0 + ml < d.rows;
-                f32x4 og = zero, ou = zero;
+                    for (int e = 0; e < 4; ++e) v[e] = act_value<KIND>(d.kind, g[e]) * u[e];
+                    store4(o, v, 4, true);
+                } else {  // dh's place takes dg; columns and rows outside hold zeros, whatever g and u are there
+                    const f32x4 v = load4(o, 4, true);
+                    const bool real = m0 + ml < d.rows;
+                    f32x4 og = zero, ou = zero;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (real && e < nf) {
-                        ou[e] = v[e] * act_value(d.kind, g[e]);
-                        og[e] = v[e] * u[e] * act_slope(d.kind, g[e]);
+                    for (int e = 0; e < 4; ++e)
+                        if (real && e < nf) {
+                            ou[e] = v[e] * act_value<KIND>(d.kind, g[e]);
+                            og[e] = v[e] * u[e] * act_slope<KIND>(d.kind, g[e]);
+                        }
+                    store4(o, og, 4, true);
+                    store4(Out::at(second, ml, fl), ou, 4, true);
+                    sg += og;
+                    su += ou;
+                }
+            }
+            if constexpr (BWD) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int s = 1; s < 16; s *= 2) {
+                        sg[e] += __shfl_xor(sg[e], s, 64);
+                        su[e] += __shfl_xor(su[e], s, 64);
                     }
-                store4(o, og, 4, true);
-                store4(Out::at(second, ml, fl), ou, 4, true);
-                sg += og;
-                su += ou;
-            }
-        }
-        if constexpr (BWD) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int s = 1; s < 16; s *= 2) {
-                    sg[e] += __shfl_xor(sg[e], s, 64);
-                    su[e] += __shfl_xor(su[e], s, 64);
-                }
-                if (r == 0) {
-                    red[(wm * 2) * FT + fl + e] = sg[e];
-                    red[(wm * 2 + 1) * FT + fl + e] = su[e];
+                    if (r == 0) {
+                        red[(wm * 2) * FT + fl + e] = sg[e];
+                        red[(wm * 2 + 1) * FT + fl + e] = su[e];
+                    }
                 }
             }
         }
-    }
+    };
+    if (d.kind == 0) epilogue(std::integral_constant<int, 0>());
+    else epilogue(std::integral_constant<int, -1>());
     __syncthreads();
     if constexpr (!BWD) {
         Out::write(lds, h + (int64_t)m0 * d.out + f0, d.out, d.rows - m0, d.out - f0, d.hvw);
@@ -181,11 +201,11 @@ __global__ __launch_bounds__(GEMM_WG) void gated_kernel(GatedDims d, int ftiles,
     }
 }
 
-// dx[m][k] = sum over f < 2 outp of D[m][f] [Wg; Wu][f][k]
-template <class T, int BM, int BN, bool DMA>
+// dx[m][k] = sum over f < 2 outp of D[m][f] [Wg; Wu][f][k]; several shares of f (blockIdx.y): their sums in fp32 to part
+template <class T, int BM, int BN, bool FAST>
 __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktiles, int mtiles, const T* __restrict__ D,
                                                            const T* __restrict__ wg, const T* __restrict__ wu,
-                                                           T* __restrict__ dx) {
+                                                           T* __restrict__ dx, int share, float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
     using Out = OutTile<T, BM, BN>;
     const TileAt at = tile_at(blockIdx.x, ktiles);
@@ -196,8 +216,20 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktil
     const ColOperand<T> ns = {wg, wu, d.in, d.in, d.out, k0, d.outp, d.wvw};
     const RowOperand<T> ms = {D, D, 2 * d.outp, d.rows, 2 * d.outp, m0, BM, 0, 8};
     f32x4 acc[BN / 32][BM / 32];
-    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, 2 * d.outp, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    const int fb = blockIdx.y * share, fe = fb + share < 2 * d.outp ? fb + share : 2 * d.outp;
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
+    if (gridDim.y > 1) {
+        float* o = part + (int64_t)blockIdx.y * d.rows * d.in;
+#pragma unroll
+        for (int j = 0; j < BN / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < BM / 32; ++i) {
+                const int m = m0 + mrow + i * 16 + r, k = k0 + nbase + j * 16 + c4;
+                if (m < d.rows) store4(o + (int64_t)m * d.in + k, acc[j][i], d.in - k, d.in % 4 == 0);
+            }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < BN / 32; ++j)
 #pragma unroll
@@ -207,7 +239,7 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktil
 }
 
 // part[s][f][k] = sum over the rows of split s of D[m][f] x[m][k]
-template <class T, int BM, int BN, bool DMA>
+template <class T, int BM, int BN, bool FAST>
 __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktiles, int rows_a_split, const T* __restrict__ D,
                                                            const T* __restrict__ x, float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
@@ -219,7 +251,7 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
     const ColOperand<T> ns = {x + rb * d.ldx, x, d.ldx, d.in, n, k0, 1 << 30, d.xvw};
     const ColOperand<T> ms = {D + rb * 2 * d.outp, D, 2 * d.outp, 2 * d.outp, n, f0, 1 << 30, 8};
     f32x4 acc[BN / 32][BM / 32];
-    gated_gemm<T, BM, BN, DMA>(lds, ns, ms, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + (int64_t)blockIdx.y * 2 * d.outp * d.in;
 #pragma unroll
@@ -231,14 +263,26 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
         }
 }
 
-// the parts of dW (workgroups below wblocks) and of the column sums, added in order
+// the parts of dx (workgroups below xblocks), of dW (wblocks more) and of the column sums, added in order
 template <class T>
-__global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int wblocks, int splits, int mtiles,
+__global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblocks, int xsplits, const float* __restrict__ xpart,
+                                                           T* __restrict__ dx, int wblocks, int splits, int mtiles,
                                                            const float* __restrict__ wpart, const float* __restrict__ bpart,
                                                            T* __restrict__ dwg, T* __restrict__ dwu, T* __restrict__ dbg,
                                                            T* __restrict__ dbu) {
-    if ((int)blockIdx.x < wblocks) {
-        const int64_t size = (int64_t)2 * d.outp * d.in, i = ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    int b = blockIdx.x;
+    if (b < xblocks) {
+        const int64_t size = (int64_t)d.rows * d.in, i = (int64_t)b * 256 + threadIdx.x;
+        if (i >= size) return;
+        float s = 0.f;
+#pragma unroll 8
+        for (int p = 0; p < xsplits; ++p) s += xpart[p * size + i];
+        dx[i] = (T)s;
+        return;
+    }
+    b -= xblocks;
+    if (b < wblocks) {
+        const int64_t size = (int64_t)2 * d.outp * d.in, i = ((int64_t)b * 256 + threadIdx.x);
         if (i >= size) return;
         const int f = (int)(i / d.in), k = (int)(i % d.in), half = f >= d.outp, ff = f - half * d.outp;
         if (ff >= d.out) return;
@@ -249,8 +293,9 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int wblo
         if (o != nullptr) o[(int64_t)ff * d.in + k] = (T)s;
         return;
     }
+    b -= wblocks;
     __shared__ float red[16][17];
-    const int cx = threadIdx.x & 15, q = threadIdx.x >> 4, c = ((int)blockIdx.x - wblocks) * 16 + cx, W = 2 * d.outp;
+    const int cx = threadIdx.x & 15, q = threadIdx.x >> 4, c = b * 16 + cx, W = 2 * d.outp;
     float s = 0.f;
     if (c < W) {
 #pragma unroll 8
@@ -285,9 +330,10 @@ static int gated_tile(int64_t m, int64_t n, int64_t times) {
     }
 
 struct GatedScratch {  // bytes from the start
-    size_t D, bpart, wpart, total;
+    size_t D, bpart, wpart, xpart, total;
     int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
     int wtile, splits, rows_a_split;   // of dW
+    int xtile, xsplits, share;         // of dx
 };
 static GatedScratch gated_scratch(int dtype, int rows, int in, int out) {
     GatedScratch s = {};
@@ -305,10 +351,22 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out) {
     n = n < 1 ? 1 : n;
     s.rows_a_split = div_up(div_up(rows > 0 ? rows : 1, n), GEMM_K) * GEMM_K;
     s.splits = div_up(rows, s.rows_a_split);
+    // dx: the largest tiles that fill the chip with shares of at least eight steps of the contraction
+    const int steps = div_up(2 * outp, GEMM_K);
+    for (s.xtile = TILE_128;; ++s.xtile) {
+        const int t = div_up(rows, TILE_M[s.xtile]) * div_up(in, TILE_N[s.xtile]);
+        int x = div_up(512, t > 0 ? t : 1);
+        x = x < steps / 8 ? x : steps / 8;
+        x = x < 1 ? 1 : x;
+        s.share = div_up(steps, x) * GEMM_K;
+        s.xsplits = div_up(2 * outp, s.share);
+        if (s.xtile == TILE_32 || (int64_t)t * s.xsplits >= 256) break;
+    }
     s.D = 0;
     s.bpart = up((size_t)rows * 2 * outp * es);
     s.wpart = s.bpart + up((size_t)s.mtiles * 2 * outp * 4);
-    s.total = s.wpart + up((size_t)s.splits * 2 * outp * in * 4);
+    s.xpart = s.wpart + up((size_t)s.splits * 2 * outp * in * 4);
+    s.total = s.xpart + (s.xsplits > 1 ? up((size_t)s.xsplits * rows * in * 4) : 0);
     return s;
 }
 
@@ -327,7 +385,8 @@ static int gated_check(const char* name, int32_t dtype, int32_t act, int32_t row
 }
 
 template <class T>
-static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, int64_t ldx, const void* wg, const void* wu) {
+static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, int64_t ldx, const void* wg, const void* wu,
+                            const void* bg, const void* bu) {
     GatedDims d = {};
     d.rows = rows;
     d.in = in;
@@ -338,17 +397,18 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
     d.xvw = load_width(sizeof(T), in, ldx, x);
     const int a = load_width(sizeof(T), in, in, wg), b = load_width(sizeof(T), in, in, wu);
     d.wvw = a < b ? a : b;
+    d.bvec = aligned16(bg) && aligned16(bu);
     return d;
 }
 // 16-byte loads everywhere, and a tile's rows within the 2 GiB that a buffer's offsets reach
-static bool gated_dma(const GatedDims& d) { return d.xvw == 8 && d.wvw == 8 && d.ldx <= (1 << 22); }
+static bool gated_fast(const GatedDims& d) { return d.xvw == 8 && d.wvw == 8 && d.ldx <= (1 << 21); }
 
-template <class T, int BM, int BN, bool DMA, bool BWD>
+template <class T, int BM, int BN, bool FAST, bool BWD>
 static int gated_first(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
                        void* h, void* D, float* part, hipStream_t st) {
     static DeviceOnce once;
-    constexpr int lds = gated_lds<T, BM, BN, DMA>(gated_behind<T, BM, BN>(BWD));
-    auto k = gated_kernel<T, BM, BN, DMA, BWD>;
+    constexpr int lds = gated_lds<T, BM, BN, FAST>(gated_behind<T, BM, BN>(BWD));
+    auto k = gated_kernel<T, BM, BN, FAST, BWD>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int ft = div_up(BWD ? d.outp : d.out, BN / 2), mt = div_up(d.rows, BM);
@@ -357,23 +417,25 @@ static int gated_first(GatedDims d, const void* x, const void* wg, const void* w
     TSD_LAUNCH_CHECK("gated_linear");
     return TSD_OK;
 }
-template <class T, int BM, int BN, bool DMA>
-static int gated_dx(GatedDims d, const T* D, const void* wg, const void* wu, void* dx, hipStream_t st) {
+template <class T, int BM, int BN, bool FAST>
+static int gated_dx(GatedDims d, const GatedScratch& s, const T* D, const void* wg, const void* wu, void* dx, float* part,
+                    hipStream_t st) {
     static DeviceOnce once;
-    constexpr int lds = gated_lds<T, BM, BN, DMA>(OutTile<T, BM, BN>::BYTES);
-    auto k = gated_dx_kernel<T, BM, BN, DMA>;
+    constexpr int lds = gated_lds<T, BM, BN, FAST>(OutTile<T, BM, BN>::BYTES);
+    auto k = gated_dx_kernel<T, BM, BN, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), mt = div_up(d.rows, BM);
-    hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt)), dim3(GEMM_WG), lds, st, d, kt, mt, D, (const T*)wg, (const T*)wu, (T*)dx);
+    hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt), s.xsplits), dim3(GEMM_WG), lds, st, d, kt, mt, D, (const T*)wg,
+                       (const T*)wu, (T*)dx, s.share, part);
     TSD_LAUNCH_CHECK("gated_dx");
     return TSD_OK;
 }
-template <class T, int BM, int BN, bool DMA>
+template <class T, int BM, int BN, bool FAST>
 static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* x, float* wpart, hipStream_t st) {
     static DeviceOnce once;
-    constexpr int lds = gated_lds<T, BM, BN, DMA>(0);
-    auto k = gated_dw_kernel<T, BM, BN, DMA>;
+    constexpr int lds = gated_lds<T, BM, BN, FAST>(0);
+    auto k = gated_dw_kernel<T, BM, BN, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), ft = div_up(2 * d.outp, BM);
@@ -381,12 +443,9 @@ static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* 
     TSD_LAUNCH_CHECK("gated_dw");
     return TSD_OK;
 }
-// f32 has no instance with loads straight to LDS
 template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
     GATED_BY_TILE(tile, BM, BN, {
-        if constexpr (sizeof(T) == 2) {
-            if (gated_dma(d)) return gated_first<T, BM, BN, true, BWD>(d, a...);
-        }
+        if (gated_fast(d)) return gated_first<T, BM, BN, true, BWD>(d, a...);
         return gated_first<T, BM, BN, false, BWD>(d, a...);
     });
 }
@@ -398,6 +457,7 @@ static int gated_bwd(GatedDims d, const GatedScratch& s, const void* x, const vo
     T* D = reinterpret_cast<T*>(scratch + s.D);
     float* bpart = reinterpret_cast<float*>(scratch + s.bpart);
     float* wpart = reinterpret_cast<float*>(scratch + s.wpart);
+    float* xpart = reinterpret_cast<float*>(scratch + s.xpart);
     const bool sums = dbg != nullptr || dbu != nullptr, weights = dwg != nullptr || dwu != nullptr;
     int rc = TSD_OK;
     if (d.rows > 0) {
@@ -406,32 +466,22 @@ static int gated_bwd(GatedDims d, const GatedScratch& s, const void* x, const vo
         d.dxvw = load_width(sizeof(T), d.in, d.in, dx);
         rc = gated_first_by<T, true>(s.tile, d, x, wg, wu, bg, bu, dh, (void*)nullptr, (void*)D, sums ? bpart : (float*)nullptr, st);
         if (rc == TSD_OK && dx != nullptr) {
-            GATED_BY_TILE(gated_tile(d.rows, d.in, 1), BM, BN, {
-                if constexpr (sizeof(T) == 2) {
-                    if (gated_dma(d)) {
-                        rc = gated_dx<T, BM, BN, true>(d, D, wg, wu, dx, st);
-                        break;
-                    }
-                }
-                rc = gated_dx<T, BM, BN, false>(d, D, wg, wu, dx, st);
+            GATED_BY_TILE(s.xtile, BM, BN, {
+                rc = gated_fast(d) ? gated_dx<T, BM, BN, true>(d, s, D, wg, wu, dx, xpart, st) : gated_dx<T, BM, BN, false>(d, s, D, wg, wu, dx, xpart, st);
             });
         }
         if (rc == TSD_OK && weights) {
             GATED_BY_TILE(s.wtile, BM, BN, {
-                if constexpr (sizeof(T) == 2) {
-                    if (gated_dma(d)) {
-                        rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st);
-                        break;
-                    }
-                }
-                rc = gated_dw<T, BM, BN, false>(d, s, D, x, wpart, st);
+                rc = gated_fast(d) ? gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st) : gated_dw<T, BM, BN, false>(d, s, D, x, wpart, st);
             });
         }
     }
-    if (rc == TSD_OK && (weights || sums)) {
+    const bool parts = d.rows > 0 && dx != nullptr && s.xsplits > 1;
+    if (rc == TSD_OK && (weights || sums || parts)) {
+        const int xb = parts ? (int)(((int64_t)d.rows * d.in + 255) / 256) : 0;
         const int wb = weights ? (int)(((int64_t)2 * d.outp * d.in + 255) / 256) : 0, bb = sums ? (2 * d.outp + 15) / 16 : 0;
-        hipLaunchKernelGGL(gated_reduce_kernel<T>, dim3(wb + bb), dim3(256), 0, st, d, wb, s.splits, s.mtiles, wpart, bpart,
-                           (T*)dwg, (T*)dwu, (T*)dbg, (T*)dbu);
+        hipLaunchKernelGGL(gated_reduce_kernel<T>, dim3(xb + wb + bb), dim3(256), 0, st, d, xb, s.xsplits, xpart, (T*)dx, wb, s.splits,
+                           s.mtiles, wpart, bpart, (T*)dwg, (T*)dwu, (T*)dbg, (T*)dbu);
         TSD_LAUNCH_CHECK("gated_reduce");
     }
     return rc;
@@ -452,7 +502,7 @@ int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
     if (rows == 0) return TSD_OK;
     TSD_REQUIRE(h != nullptr, "tsd_gated_linear_fwd: null pointer");
     TSD_BY_DTYPE(dtype, T, {
-        GatedDims d = gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up);
+        GatedDims d = gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, b_gate, b_up);
         d.hvw = load_width(sizeof(T), out, out, h);
         return gated_first_by<T, false>(gated_tile(rows, 2 * (int64_t)d.outp, 1), d, x, w_gate, w_up, b_gate, b_up,
                                         (const void*)nullptr, h, (void*)nullptr, (float*)nullptr, (hipStream_t)stream);
@@ -475,7 +525,7 @@ int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
     TSD_REQUIRE(rows == 0 || (dh != nullptr && lddh >= out), "tsd_gated_linear_bwd: null pointer or row stride");
     TSD_REQUIRE(rows == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats * 4 >= s.total),
                 "tsd_gated_linear_bwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, s.total / 4);
-    TSD_BY_DTYPE(dtype, T, return gated_bwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up), s, x, w_gate, w_up,
+    TSD_BY_DTYPE(dtype, T, return gated_bwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, b_gate, b_up), s, x, w_gate, w_up,
                                                b_gate, b_up, dh, lddh, dx, dw_gate, dw_up, db_gate, db_up, (char*)scratch,
                                                (hipStream_t)stream));
     return TSD_OK;
