@@ -22,6 +22,7 @@ namespace tsd {
 namespace blk {
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LAG = 6.f;
 
 struct AttDims {
     int graphs, rows_q, rows_k, heads, kv_heads, group, dim;
@@ -105,33 +106,64 @@ template <class T> struct Rows {
         const int q = r / group;
         return p + (int64_t)q * row + (r - q * group) * head;
     }
-    // bit i: row r0 + i (i < ROWS <= 64) is there and open; the same in every lane
+    // bit i: row r0 + i (i < 64) is there
+    __device__ __forceinline__ uint64_t there(int r0) const { return n - r0 >= 64 ? ~0ull : n > r0 ? (1ull << (n - r0)) - 1 : 0; }
+    // ... and open (i < ROWS); the same in every lane
     template <int ROWS> __device__ __forceinline__ uint64_t open(int r0) const {
-        if (mask == nullptr) return n - r0 >= 64 ? ~0ull : n > r0 ? (1ull << (n - r0)) - 1 : 0;
+        if (mask == nullptr) return there(r0);
         const int lane = threadIdx.x & 63;
         return __ballot(lane < ROWS && has(r0 + lane));
     }
 };
+// Which keys are open, a word a tile, MASK_TILES tiles at a time in LDS: looked up tile by tile, the mask's bytes would be
+// waited for in front of every tile's loads.
+constexpr int MASK_TILES = 256, MASK_BYTES = MASK_TILES * 8;
+template <int WAVES, int KT, class T>
+__device__ __forceinline__ void mask_words(const Rows<T>& s, int tb, int te, uint64_t* words) {
+    if (s.mask == nullptr) return;
+    __syncthreads();
+#pragma unroll 4
+    for (int t = tb + (int)(threadIdx.x >> 6); t < te; t += WAVES) {
+        const uint64_t w = s.template open<KT>(t * KT);
+        if ((threadIdx.x & 63) == 0) words[t - tb] = w;
+    }
+    __syncthreads();
+}
+template <int KT, class T> __device__ __forceinline__ uint64_t mask_word(const Rows<T>& s, int t, int tb, const uint64_t* words) {
+    if (s.mask == nullptr) return s.there(t * KT);
+    const uint64_t w = words[t - tb];
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)w) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(w >> 32)) << 32;
+}
 
-// A tile of ROWS rows on its way to LDS; rows that are not open become zeros.  DMA: straight there; registers otherwise.
-template <class T, int ROWS, int DP, int NT, bool DMA> struct RowStage {
+// A tile of ROWS rows on its way to LDS; rows that are not open become zeros.  FAST: 16-byte loads with bounds in the buffer,
+// straight to LDS (DMA) for the 16-bit types, by way of registers for f32; otherwise guarded loads.
+template <class T, bool FAST> constexpr bool att_dma() { return FAST && sizeof(T) == 2; }
+template <class T, int ROWS, int DP, int NT, bool FAST> struct RowStage {
     using Lds = Tile<T, ROWS, DP / 8>;
+    static constexpr bool DMA = att_dma<T, FAST>();
     static constexpr int C = DP / 8, UNITS = ROWS * C, U = (UNITS + NT - 1) / NT;
-    static_assert(!DMA || UNITS % NT == 0 || (NT % UNITS == 0 && UNITS % 64 == 0), "whole loads");
+    static_assert(UNITS % NT == 0 || (NT % UNITS == 0 && UNITS % 64 == 0), "whole loads");
     Raw<T> raw[DMA ? 1 : U];
     __device__ __forceinline__ void load(const Rows<T>& s, int r0, uint64_t open, uint32_t lds) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            int u = threadIdx.x + i * NT;
-            if constexpr (DMA) {
-                u %= UNITS;  // (a small tile is loaded by several waves alike: every wave counts the same loads)
-                const int r = u / C, c = (u % C) ^ Lds::swizzle(r);
-                const T* base = s.group == 1 ? s.p + (int64_t)r0 * s.row : s.p + (int64_t)(r0 / s.group) * s.row;
-                uint32_t off = DMA_NOWHERE;
-                if ((open >> r & 1) && c * 8 < s.dim) off = (uint32_t)((s.at(r0 + r) - base + c * 8) * (int)sizeof(T));
-                dma_load(dma_buffer(base), off, lds + (threadIdx.x / 64 * 64 + i * NT) % UNITS * 16);
-            } else if (UNITS % NT == 0 || u < UNITS) {
-                const int r = u / C, c = u % C, n = (open >> r & 1) ? s.dim - c * 8 : 0;
+            const int u = (threadIdx.x + i * NT) % UNITS;  // (a small tile is loaded by several waves alike)
+            const int r = u / C, c = DMA ? (u % C) ^ Lds::swizzle(r) : u % C;
+            const bool has = open >> r & 1;
+            if constexpr (FAST) {
+                const T* base = s.p + (s.group == 1 ? r0 : r0 / s.group) * s.row;
+                uint32_t off = (uint32_t)((s.group == 1 ? r * (int)s.row : (int)(s.at(r0 + r) - base)) + c * 8) * (uint32_t)sizeof(T);
+                off = has && c * 8 < s.dim ? off : DMA_NOWHERE;
+                const i32x4 buf = dma_buffer(base);
+                if constexpr (DMA) {
+                    dma_load(buf, off, lds + (threadIdx.x / 64 * 64 + i * NT) % UNITS * 16);
+                } else {
+                    raw[i].a = buffer_load(buf, off);
+                    raw[i].b = buffer_load(buf, off + 16);
+                }
+            } else {
+                const int n = has ? s.dim - c * 8 : 0;
                 load_raw(raw[i], n > 0 ? s.at(r0 + r) + c * 8 : s.p, n < 0 ? 0 : n > 8 ? 8 : n, s.vw);
             }
         }
@@ -186,13 +218,21 @@ template <class T> __device__ __forceinline__ Chunk<T> joined(const f32x4& a, co
     return to_chunk(x, T());
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// over the four lanes l % 16 + 0, 16, 32, 48
+template <class F> __device__ __forceinline__ float over_groups(float v, F f) {
+    uint32_t a = __builtin_bit_cast(uint32_t, v);
+    auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    uint32_t x = r[0], y = r[1];
+    a = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)));
+    r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    x = r[0], y = r[1];
+    return f(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
 __device__ __forceinline__ float over_groups_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float over_groups_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    return over_groups(v, [](float a, float b) { return a + b; });
 }
 template <class T>
 __device__ __forceinline__ Rows<T> rows_of(const T* p, int64_t row, int64_t head, int start, int n, int first_head, int group,
@@ -207,8 +247,9 @@ __device__ __forceinline__ void split_range(int n, int tile, int splits, int z, 
     *e = (z + 1) * per < tiles ? (z + 1) * per : tiles;
 }
 
-// The tiles b .. e - 1 of one pair of row sets, one after the other in LDS: stage(i, open, buffer) starts tile i's loads,
-// step(i, open, buffer) is its work.  DMA: three buffers, two tiles under way; registers: two buffers, one tile under way.
+// The tiles b .. e - 1 of one pair of row sets, one after the other in LDS: load(i, open, buffer) starts tile i's loads,
+// step(i, open, buffer) is its work.  DMA: three buffers, two tiles under way; registers: one buffer (the planes of f32 take
+// three times the room, and workgroups on a CU are worth more than the barrier saved), one tile under way.
 // LOADS: the loads of a wave a tile.
 template <int LOADS, bool DMA, class Open, class Load, class Store, class Step>
 __device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, Store store, Step step) {
@@ -232,30 +273,28 @@ __device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, S
     } else {
         uint64_t m0 = open(b);
         load(b, m0, 0);
-        store(0);
-        int buf = 0;
         for (int i = b; i < e; ++i) {
+            if (i > b) __syncthreads();
+            store(0);
             __syncthreads();
             const uint64_t m1 = i + 1 < e ? open(i + 1) : 0;
-            if (i + 1 < e) load(i + 1, m1, buf ^ 1);
-            step(i, m0, buf);
-            if (i + 1 < e) store(buf ^ 1);
+            if (i + 1 < e) load(i + 1, m1, 0);
+            step(i, m0, 0);
             m0 = m1;
-            buf ^= 1;
         }
     }
 }
-template <bool DMA> constexpr int att_buffers() { return DMA ? 3 : 2; }
+template <class T, bool FAST> constexpr int att_buffers() { return att_dma<T, FAST>() ? 3 : 1; }
 
 // ---------------------------------------------------------------------------------------------
 // forward: WAVES waves of RS x 16 rows each share the key tiles
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int RS, int KT, bool DMA>
+template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, T* __restrict__ out,
                                                              float* __restrict__ lse, float* __restrict__ part) {
     constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
-    using Stage = RowStage<T, KT, DP, NT, DMA>;
+    using Stage = RowStage<T, KT, DP, NT, FAST>;
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
@@ -281,10 +320,14 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
     }
     Stage ks, vs;
     const uint32_t at_lds = lds_offset(lds);
-    int tb, te;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &tb, &te);
-    over_tiles<2 * Stage::U, DMA>(
-        tb, te, [&](int i) { return kr.template open<KT>(i * KT); },
+    int first, last;
+    split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
+    uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
+    for (int tb = first; tb < last; tb += MASK_TILES) {
+    const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
+    mask_words<WAVES, KT>(kr, tb, te, words);
+    over_tiles<2 * Stage::U, Stage::DMA>(
+        tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
         [&](int i, uint64_t open, int buf) {
             ks.load(kr, i * KT, open, at_lds + buf * BUF);
             vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
@@ -294,6 +337,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
             vs.store(lds + buf * BUF + KTile::BYTES);
         },
         [&](int, uint64_t open, int buf) {
+            if (open == 0) return;  // nothing to attend to
             const char* kl = lds + buf * BUF;
             const char* vl = kl + KTile::BYTES;
             f32x4 s[RS][KT / 16];
@@ -335,10 +379,17 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
 #pragma unroll
                         for (int e = 0; e < 4; ++e) hi = fmaxf(hi, -s[x][t][e]);
                 }
-                const float top = fmaxf(m[x], over_groups_max(hi * fabsf(sc)));
-                const float safe = top == -INFINITY ? 0.f : top, a = exp2_fast(m[x] - safe);
-                m[x] = top;
-                l[x] *= a;
+                hi *= fabsf(sc);
+                // The weights are taken from a maximum that may lag behind by a factor of 2^LAG, which neither they nor their
+                // sum notice: most tiles then need no look at the other lanes and no scaling of what is summed up.
+                if (__any(hi > m[x] + LAG)) {
+                    const float top = fmaxf(m[x], over_groups_max(hi)), a = exp2_fast(m[x] - (top == -INFINITY ? 0.f : top));
+                    m[x] = top;
+                    l[x] *= a;
+#pragma unroll
+                    for (int t = 0; t < DP / 16; ++t) o[x][t] *= a;
+                }
+                const float safe = m[x] == -INFINITY ? 0.f : m[x];
 #pragma unroll
                 for (int t = 0; t < KT / 16; ++t)
 #pragma unroll
@@ -346,8 +397,6 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
                         s[x][t][e] = exp2_fast(__builtin_fmaf(s[x][t][e], sc, -safe));
                         l[x] += s[x][t][e];
                     }
-#pragma unroll
-                for (int t = 0; t < DP / 16; ++t) o[x][t] *= a;
             }
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b) {
@@ -362,6 +411,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
                 }
             }
         });
+    }
 #pragma unroll
     for (int x = 0; x < RS; ++x) {
         const float ls = over_groups_sum(l[x]);
@@ -426,14 +476,14 @@ __global__ __launch_bounds__(256) void att_sum_kernel(int64_t n, int splits, con
 // ---------------------------------------------------------------------------------------------
 // dQ: the forward's tiles again; delta on the way
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int RS, int KT, bool DMA>
+template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                             const T* __restrict__ v, const T* __restrict__ out,
                                                             const T* __restrict__ dout, const float* __restrict__ lse,
                                                             float* __restrict__ delta, T* __restrict__ dq,
                                                             float* __restrict__ part) {
     constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
-    using Stage = RowStage<T, KT, DP, NT, DMA>;
+    using Stage = RowStage<T, KT, DP, NT, FAST>;
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
@@ -476,10 +526,14 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
     }
     Stage ks, vs;
     const uint32_t at_lds = lds_offset(lds);
-    int tb, te;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &tb, &te);
-    over_tiles<2 * Stage::U, DMA>(
-        tb, te, [&](int i) { return kr.template open<KT>(i * KT); },
+    int first, last;
+    split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
+    uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
+    for (int tb = first; tb < last; tb += MASK_TILES) {
+    const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
+    mask_words<WAVES, KT>(kr, tb, te, words);
+    over_tiles<2 * Stage::U, Stage::DMA>(
+        tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
         [&](int i, uint64_t open, int buf) {
             ks.load(kr, i * KT, open, at_lds + buf * BUF);
             vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
@@ -489,6 +543,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
             vs.store(lds + buf * BUF + KTile::BYTES);
         },
         [&](int, uint64_t open, int buf) {
+            if (open == 0) return;  // nothing to attend to
             const char* kl = lds + buf * BUF;
             const char* vl = kl + KTile::BYTES;
 #pragma unroll
@@ -530,6 +585,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                 }
             }
         });
+    }
 #pragma unroll
     for (int x = 0; x < RS; ++x) {
         const int row = row0 + x * 16;
@@ -551,13 +607,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
 // ---------------------------------------------------------------------------------------------
 // dK, dV: WAVES waves of KS x 16 keys each; all rows (of all heads that read the keys) go by in tiles of RT
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int KS, int RT, bool DMA>
+template <class T, int DP, int WAVES, int KS, int RT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const T* __restrict__ dout,
                                                              const float* __restrict__ lse, const float* __restrict__ delta,
                                                              T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
     constexpr int NT = WAVES * 64, TK = WAVES * KS * 16;
-    using Stage = RowStage<T, RT, DP, NT, DMA>;
+    using Stage = RowStage<T, RT, DP, NT, FAST>;
     using RTile = typename Stage::Lds;
     constexpr int STAT = 2 * RTile::BYTES, BUF = STAT + 2 * 64 * 4;  // Q, dO, then 64 values of L and of delta each
     constexpr int STATS = WAVES > 1 ? 1 : 2;                         // stat loads of a wave a tile
@@ -592,13 +648,17 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
     const uint32_t at_lds = lds_offset(lds);
     int tb, te;
     split_range(nrows, RT, d.splits, blockIdx.z, &tb, &te);
-    over_tiles<2 * Stage::U + STATS, DMA>(
-        tb, te, [&](int i) { return qr.template open<RT>(i * RT); },
+    uint64_t any = 0;
+#pragma unroll
+    for (int i = 0; i < TK; i += 64) any |= kr.template open<(TK < 64 ? TK : 64)>(k0 + i);
+    if (any == 0) te = tb;  // nobody attends to these keys
+    over_tiles<2 * Stage::U + STATS, Stage::DMA>(
+        tb, te, [&](int i) { return qr.there(i * RT); },
         [&](int i, uint64_t open, int buf) {
             qs.load(qr, i * RT, open, at_lds + buf * BUF);
             gs.load(gr, i * RT, open, at_lds + buf * BUF + RTile::BYTES);
             // a missing row: its Q, dO, L and delta are zeros, and so is what it adds
-            if constexpr (DMA) {
+            if constexpr (Stage::DMA) {
                 const int64_t first = stat_at(i * RT);
                 const uint32_t off = (open >> lane & 1) && lane < RT ? (uint32_t)((stat_at(i * RT + lane) - first) * 4) : DMA_NOWHERE;
 #pragma unroll
@@ -615,7 +675,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
         [&](int buf) {
             qs.store(lds + buf * BUF);
             gs.store(lds + buf * BUF + RTile::BYTES);
-            if (!DMA && threadIdx.x < 2 * RT)
+            if (!Stage::DMA && threadIdx.x < 2 * RT)
                 reinterpret_cast<float*>(lds + buf * BUF + STAT)[threadIdx.x / RT * 64 + threadIdx.x % RT] = stat_reg;
         },
         [&](int, uint64_t, int buf) {
@@ -696,6 +756,9 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
 // host side
 // ---------------------------------------------------------------------------------------------
 // How a side (queries of all heads of a group, or keys) is cut into tiles
+#ifndef SMALL_
+#define SMALL_ 32
+#endif
 enum { SIDE_16, SIDE_64, SIDE_128 };
 static const int SIDE_ROWS[3] = {16, 64, 128};
 // One wave of 16 rows where the graphs are small (its tile is filled at least as well as one of 64 rows), 32 rows a wave where
@@ -703,8 +766,8 @@ static const int SIDE_ROWS[3] = {16, 64, 128};
 // have the middle instance alone; f32 has no 128 (its three planes of twice the rows do not fit the registers).
 static int att_side(int64_t rows, int graphs, bool f32, bool aligned) {
     const int64_t each = rows / (graphs < 1 ? 1 : graphs);
-    if (!f32 && !aligned) return SIDE_64;
-    return each <= 32 ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
+    if (!aligned) return SIDE_64;
+    return each <= SMALL_ ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
 }
 static int att_slots(int64_t rows, int graphs, int tile) { return (int)((rows + (int64_t)(graphs + 2) * (tile - 1)) / tile); }
 // Shares of the other side's tiles: enough workgroups for the 256 CUs, and four tiles of 64 a share at least.
@@ -798,16 +861,14 @@ static AttDims att_dims(const tsd_attention& a) {
     return d;
 }
 
-// rows of a tile of the other side: what keeps three workgroups (f32 of 128 values: one) on a CU
-template <class T, int DP, int WAVES> constexpr int att_tile() {
-    return WAVES == 1 || DP == 128 || (sizeof(T) == 4 && DP > 32) ? 32 : 64;
-}
-template <class T, int DP, int WAVES, int RS, bool DMA>
+// rows of a tile of the other side: what keeps three workgroups on a CU
+template <class T, int DP, int WAVES> constexpr int att_tile() { return WAVES == 1 || DP == 128 || sizeof(T) == 4 ? 32 : 64; }
+template <class T, int DP, int WAVES, int RS, bool FAST>
 static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse, float* scratch, hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
-    constexpr int lds = att_buffers<DMA>() * 2 * Tile<T, KT, DP / 8>::BYTES;
+    constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
-    auto k = att_fwd_kernel<T, DP, WAVES, RS, KT, DMA>;
+    auto k = att_fwd_kernel<T, DP, WAVES, RS, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
@@ -816,13 +877,13 @@ static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse,
     TSD_LAUNCH_CHECK("attention_fwd");
     return TSD_OK;
 }
-template <class T, int DP, int WAVES, int RS, bool DMA>
+template <class T, int DP, int WAVES, int RS, bool FAST>
 static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* dout, const float* lse, float* delta, T* dq,
                          float* part, hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
-    constexpr int lds = att_buffers<DMA>() * 2 * Tile<T, KT, DP / 8>::BYTES;
+    constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
-    auto k = att_dq_kernel<T, DP, WAVES, RS, KT, DMA>;
+    auto k = att_dq_kernel<T, DP, WAVES, RS, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
@@ -831,13 +892,13 @@ static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const 
     TSD_LAUNCH_CHECK("attention_dq");
     return TSD_OK;
 }
-template <class T, int DP, int WAVES, int KS, bool DMA>
+template <class T, int DP, int WAVES, int KS, bool FAST>
 static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, const float* lse, const float* delta, T* dk, T* dv,
                           float* part, hipStream_t st) {
     constexpr int RT = 32;
-    constexpr int lds = att_buffers<DMA>() * (2 * Tile<T, RT, DP / 8>::BYTES + 512);
+    constexpr int lds = att_buffers<T, FAST>() * (2 * Tile<T, RT, DP / 8>::BYTES + 512);
     static DeviceOnce once;
-    auto k = att_dkv_kernel<T, DP, WAVES, KS, RT, DMA>;
+    auto k = att_dkv_kernel<T, DP, WAVES, KS, RT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     d.slots = att_slots(d.rows_k, d.graphs, WAVES * KS * 16);
@@ -846,17 +907,12 @@ static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, cons
     TSD_LAUNCH_CHECK("attention_dkv");
     return TSD_OK;
 }
-// launch<T, DP, waves, subtiles of 16 a wave, DMA> of a side
+// launch<T, DP, waves, subtiles of 16 a wave, FAST> of a side
 #define ATT_BY_SIDE(rc, side, aligned, launch, ...)                                      \
-    if constexpr (sizeof(T) == 4) {                                                      \
-        if (side == SIDE_16) rc = launch<T, DP, 1, 1, false>(__VA_ARGS__);               \
-        else rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                               \
-    } else {                                                                             \
-        if (!(aligned)) rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                    \
-        else if (side == SIDE_16) rc = launch<T, DP, 1, 1, true>(__VA_ARGS__);           \
-        else if (side == SIDE_64) rc = launch<T, DP, 4, 1, true>(__VA_ARGS__);           \
-        else rc = launch<T, DP, 4, 2, true>(__VA_ARGS__);                                \
-    }
+    if (!(aligned)) rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                        \
+    else if (side == SIDE_16) rc = launch<T, DP, 1, 1, true>(__VA_ARGS__);               \
+    else if (sizeof(T) == 4 || side == SIDE_64) rc = launch<T, DP, 4, 1, true>(__VA_ARGS__); \
+    else if constexpr (sizeof(T) == 2) rc = launch<T, DP, 4, 2, true>(__VA_ARGS__);
 
 template <class T, int DP>
 static int att_fwd(AttDims d, const tsd_attention& a, void* out, float* lse, float* scratch, hipStream_t st) {
