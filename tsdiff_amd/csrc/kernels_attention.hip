@@ -28,7 +28,9 @@ struct AttDims {
     int graphs, rows_q, rows_k, heads, kv_heads, group, dim;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
     float scale, scale2;  // scale2 = scale * log2 e
-    int splits, slots;
+    int splits;
+    int heads_a_wg;       // key heads that a workgroup goes over, one after the other
+    float graph_of_slot;  // where equal graphs would have a slot's graph
     int qvw, kvw, vvw, dovw;  // values a load of each may take (load_raw)
     bool ovec;
     const int32_t *q_ptr, *k_ptr;
@@ -50,8 +52,9 @@ __device__ __forceinline__ Span find_span(const AttDims& d, bool by_key, int T, 
     const int32_t* ptr = by_key ? d.k_ptr : d.q_ptr;
     const int32_t* other = by_key ? d.q_ptr : d.k_ptr;
     const int n = by_key ? d.rows_k : d.rows_q, on = by_key ? d.rows_q : d.rows_k, lane = threadIdx.x & 63, all = d.graphs + 2;
-    auto slot = [&](int b, int v) { return ((int64_t)b * times + (int64_t)v * (T - 1)) / T; };
-    int lo = (int)((int64_t)s * all / d.slots) - 32;
+    // (32 bits: at most 2^30 rows and 2^22 graphs)
+    auto slot = [&](int b, int v) { return (int)(((uint32_t)b * (uint32_t)times + (uint32_t)v * (uint32_t)(T - 1)) / (uint32_t)T); };
+    int lo = (int)((float)s * d.graph_of_slot) - 32;
     lo = lo > all - 64 ? all - 64 : lo;
     lo = lo < 0 ? 0 : lo;
     int b = bound_at(ptr, d.graphs, n, lo + lane);
@@ -83,7 +86,7 @@ __device__ __forceinline__ Span find_span(const AttDims& d, bool by_key, int T, 
         }
     }
     Span sp;
-    sp.tile = s - (int)slot(start, v);
+    sp.tile = s - slot(start, v);
     end = end < start ? start : end;
     oe = oe < os ? os : oe;
     sp.qs = by_key ? os : start;
@@ -92,6 +95,9 @@ __device__ __forceinline__ Span find_span(const AttDims& d, bool by_key, int T, 
     sp.ke = by_key ? end : oe;
     return sp;
 }
+
+// row = query * group + head of the group
+__device__ __forceinline__ int query_of(int row, int group) { return group == 1 ? row : row / group; }
 
 // Values (row, d) of a graph's rows or keys
 template <class T> struct Rows {
@@ -152,7 +158,7 @@ template <class T, int ROWS, int DP, int NT, bool FAST> struct RowStage {
             const int r = u / C, c = DMA ? (u % C) ^ Lds::swizzle(r) : u % C;
             const bool has = open >> r & 1;
             if constexpr (FAST) {
-                const T* base = s.p + (s.group == 1 ? r0 : r0 / s.group) * s.row;
+                const T* base = s.p + (int64_t)query_of(r0, s.group) * s.row;
                 uint32_t off = (uint32_t)((s.group == 1 ? r * (int)s.row : (int)(s.at(r0 + r) - base)) + c * 8) * (uint32_t)sizeof(T);
                 off = has && c * 8 < s.dim ? off : DMA_NOWHERE;
                 const i32x4 buf = dma_buffer(base);
@@ -298,10 +304,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
-    const int hk = blockIdx.x % d.kv_heads;
-    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / d.kv_heads);
+    const int hgroups = (d.kv_heads + d.heads_a_wg - 1) / d.heads_a_wg;
+    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / hgroups);
     const int r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
     if (r0 >= nrows) return;
+    const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
+    for (int hk = h0; hk < h1; ++hk) {
+    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int row0 = r0 + wave * RS * 16 + c;
     const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, (const uint8_t*)nullptr, d.qvw);
@@ -417,8 +426,8 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
         const float ls = over_groups_sum(l[x]);
         const int row = row0 + x * 16;
         if (row >= nrows) continue;
-        const int qi = sp.qs + row / d.group, h = hk * d.group + row % d.group;
-        const int64_t at = (int64_t)qi * d.heads + h;
+        const int qi = query_of(row, d.group);
+        const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + row - qi * d.group;
         if (d.splits > 1) {  // unnormalised sums and their statistics: att_join_kernel ends the work
             const int64_t all = (int64_t)d.rows_q * d.heads, i = blockIdx.z * all + at;
             float* po = part + i * d.dim;
@@ -431,11 +440,12 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
             }
             continue;
         }
-        const float inv = ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;
+        const float inv = ls > 0.f ? __builtin_amdgcn_rcpf(ls) : ls == 0.f ? 0.f : ls;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t)
             store4(out + at * d.dim + t * 16 + g * 4, o[x][t] * inv, d.dim - t * 16 - g * 4, d.ovec);
-        if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? -INFINITY : m[x] + log2f(ls);
+        if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? -INFINITY : m[x] + __builtin_amdgcn_logf(ls);
+    }
     }
 }
 
@@ -448,16 +458,18 @@ __global__ __launch_bounds__(256) void att_join_kernel(int64_t all, int dim, int
     const int e = (int)(i % dim);
     const float* stat = part + splits * all * dim;
     float m = -INFINITY;
+#pragma unroll 8
     for (int z = 0; z < splits; ++z) m = fmaxf(m, stat[2 * (z * all + at)]);
     const float safe = m == -INFINITY ? 0.f : m;
     float l = 0.f, o = 0.f;
+#pragma unroll 8
     for (int z = 0; z < splits; ++z) {
         const float a = exp2_fast(stat[2 * (z * all + at)] - safe);
         l += a * stat[2 * (z * all + at) + 1];
         o += a * part[(z * all + at) * dim + e];
     }
     out[i] = (T)(l == 0.f ? 0.f : o / l);
-    if (lse != nullptr && e == 0) lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+    if (lse != nullptr && e == 0) lse[at] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // out[i] = sum_z part[z][i]
@@ -469,6 +481,7 @@ __global__ __launch_bounds__(256) void att_sum_kernel(int64_t n, int splits, con
     const float* p = blockIdx.y ? part2 : part;
     T* o = blockIdx.y ? a2 : a;
     float s = 0.f;
+#pragma unroll 8
     for (int z = 0; z < splits; ++z) s += p[z * n + i];
     o[i] = (T)s;
 }
@@ -487,10 +500,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
     extern __shared__ __align__(16) char lds[];
-    const int hk = blockIdx.x % d.kv_heads;
-    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / d.kv_heads);
+    const int hgroups = (d.kv_heads + d.heads_a_wg - 1) / d.heads_a_wg;
+    const Span sp = find_span(d, false, TR, d.group, blockIdx.x / hgroups);
     const int r0 = sp.tile * TR, nrows = (sp.qe - sp.qs) * d.group;
     if (r0 >= nrows) return;
+    const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
+    for (int hk = h0; hk < h1; ++hk) {
+    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int row0 = r0 + wave * RS * 16 + c;
     const uint8_t* no = nullptr;
@@ -517,7 +533,8 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
             s += raw_dot(a, o);
         }
         del[x] = over_groups_sum(s);
-        const int64_t at = (int64_t)(sp.qs + (mine ? row / d.group : 0)) * d.heads + hk * d.group + (mine ? row % d.group : 0);
+        const int qi = mine ? query_of(row, d.group) : 0;
+        const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + (mine ? row - qi * d.group : 0);
         L[x] = mine ? lse[at] : INFINITY;
         safe[x] = L[x] == -INFINITY ? INFINITY : L[x];  // no open key: every weight is 0
         if (mine && g == 0 && blockIdx.z == 0) delta[at] = del[x];
@@ -590,7 +607,8 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
     for (int x = 0; x < RS; ++x) {
         const int row = row0 + x * 16;
         if (row >= nrows) continue;
-        const int64_t at = (int64_t)(sp.qs + row / d.group) * d.heads + hk * d.group + row % d.group;
+        const int qi = query_of(row, d.group);
+        const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + row - qi * d.group;
         // a row without an open key has dQ = 0 whatever dO and O hold
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
@@ -601,6 +619,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
             else
                 store4(dq + at * d.dim + t * 16 + g * 4, r, n, d.ovec);
         }
+    }
     }
 }
 
@@ -618,10 +637,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
     constexpr int STAT = 2 * RTile::BYTES, BUF = STAT + 2 * 64 * 4;  // Q, dO, then 64 values of L and of delta each
     constexpr int STATS = WAVES > 1 ? 1 : 2;                         // stat loads of a wave a tile
     extern __shared__ __align__(16) char lds[];
-    const int hk = blockIdx.x % d.kv_heads;
-    const Span sp = find_span(d, true, TK, 1, blockIdx.x / d.kv_heads);
+    const int hgroups = (d.kv_heads + d.heads_a_wg - 1) / d.heads_a_wg;
+    const Span sp = find_span(d, true, TK, 1, blockIdx.x / hgroups);
     const int k0 = sp.tile * TK, nkeys = sp.ke - sp.ks, nrows = (sp.qe - sp.qs) * d.group;
     if (k0 >= nkeys) return;
+    const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
+    for (int hk = h0; hk < h1; ++hk) {
+    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int key0 = k0 + wave * KS * 16 + c;
     const uint8_t* no = nullptr;
@@ -631,7 +653,10 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
     const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.vvw);
     // row r's statistics lie at (qs + r / group) heads + hk group + r % group
     const int64_t stat0 = (int64_t)sp.qs * d.heads + hk * d.group;
-    auto stat_at = [&](int r) { return (int64_t)(r / d.group) * d.heads + r % d.group; };
+    auto stat_at = [&](int r) {
+        const int qi = query_of(r, d.group);
+        return (int64_t)qi * d.heads + r - qi * d.group;
+    };
     Chunk<T> kf[KS][DP / 32], vf[KS][DP / 32];
     bool open_key[KS];
     f32x4 ak[KS][DP / 16], av[KS][DP / 16];
@@ -750,15 +775,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
             }
         }
     }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
 // How a side (queries of all heads of a group, or keys) is cut into tiles
-#ifndef SMALL_
-#define SMALL_ 32
-#endif
 enum { SIDE_16, SIDE_64, SIDE_128 };
 static const int SIDE_ROWS[3] = {16, 64, 128};
 // One wave of 16 rows where the graphs are small (its tile is filled at least as well as one of 64 rows), 32 rows a wave where
@@ -767,12 +790,20 @@ static const int SIDE_ROWS[3] = {16, 64, 128};
 static int att_side(int64_t rows, int graphs, bool f32, bool aligned) {
     const int64_t each = rows / (graphs < 1 ? 1 : graphs);
     if (!aligned) return SIDE_64;
-    return each <= SMALL_ ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
+    return each <= 32 ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
 }
-static int att_slots(int64_t rows, int graphs, int tile) { return (int)((rows + (int64_t)(graphs + 2) * (tile - 1)) / tile); }
-// Shares of the other side's tiles: enough workgroups for the 256 CUs, and four tiles of 64 a share at least.
-static int att_splits(int64_t workgroups, int64_t other, int graphs) {
-    const int64_t want = 1024 / (workgroups < 1 ? 1 : workgroups), most = other / (graphs < 1 ? 1 : graphs) / 256;
+// Workgroups of a launch.  Where there are many, each goes over several key heads: looking the graph up, and the workgroups
+// that find no tile, are then paid for less often.
+static int att_grid(AttDims& d, int64_t rows, int tile) {
+    const int64_t slots = (rows + (int64_t)(d.graphs + 2) * (tile - 1)) / tile;
+    d.graph_of_slot = (float)(d.graphs + 2) / (float)(slots > 0 ? slots : 1);
+    d.heads_a_wg = 1;
+    while (d.heads_a_wg < d.kv_heads && slots * d.splits * (d.kv_heads / (2 * d.heads_a_wg)) >= 2048) d.heads_a_wg *= 2;
+    return (int)(slots * ((d.kv_heads + d.heads_a_wg - 1) / d.heads_a_wg));
+}
+// Shares of the other side's tiles: two waves for each of the 1024 SIMDs, and 256 rows a share at least.
+static int att_splits(int64_t waves, int64_t other, int graphs) {
+    const int64_t want = 2048 / (waves < 1 ? 1 : waves), most = other / (graphs < 1 ? 1 : graphs) / 256;
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
@@ -803,11 +834,14 @@ static AttPlan att_plan(const tsd_attention& a, bool aligned) {
     const int group = a.heads / a.kv_heads;
     const bool f32 = a.dtype == TSD_F32;
     const int64_t rows = (int64_t)a.num_queries * group, keys = a.num_keys;
-    auto tiles = [&](int64_t n) { return (n / SIDE_ROWS[att_side(n, a.num_graphs, f32, true)] + a.num_graphs) * a.kv_heads; };
+    auto waves = [&](int64_t n) {
+        const int side = att_side(n, a.num_graphs, f32, true);
+        return (n / SIDE_ROWS[side] + a.num_graphs) * a.kv_heads * (side == SIDE_16 ? 1 : 4);
+    };
     p.side_q = att_side(rows, a.num_graphs, f32, aligned);
     p.side_k = att_side(keys, a.num_graphs, f32, aligned);
-    p.splits_q = att_splits(tiles(rows), keys, a.num_graphs);
-    p.splits_k = att_splits(tiles(keys), rows, a.num_graphs);
+    p.splits_q = att_splits(waves(rows), keys, a.num_graphs);
+    p.splits_k = att_splits(waves(keys), rows, a.num_graphs);
     const size_t nq = (size_t)a.num_queries * a.heads, nk = (size_t)keys * a.kv_heads;
     p.fwd = p.splits_q > 1 ? p.splits_q * nq * (a.dim + 2) : 0;
     const size_t q = p.splits_q > 1 ? p.splits_q * nq * a.dim : 0, k = p.splits_k > 1 ? 2 * p.splits_k * nk * a.dim : 0;
@@ -871,8 +905,7 @@ static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse,
     auto k = att_fwd_kernel<T, DP, WAVES, RS, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
-    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
                        (const T*)a.v, out, lse, scratch);
     TSD_LAUNCH_CHECK("attention_fwd");
     return TSD_OK;
@@ -886,8 +919,7 @@ static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const 
     auto k = att_dq_kernel<T, DP, WAVES, RS, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    d.slots = att_slots((int64_t)d.rows_q * d.group, d.graphs, WAVES * RS * 16);
-    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
                        (const T*)a.v, out, dout, lse, delta, dq, part);
     TSD_LAUNCH_CHECK("attention_dq");
     return TSD_OK;
@@ -901,8 +933,7 @@ static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, cons
     auto k = att_dkv_kernel<T, DP, WAVES, KS, RT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    d.slots = att_slots(d.rows_k, d.graphs, WAVES * KS * 16);
-    hipLaunchKernelGGL(k, dim3(d.slots * d.kv_heads, 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
+    hipLaunchKernelGGL(k, dim3(att_grid(d, d.rows_k, WAVES * KS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
                        (const T*)a.v, dout, lse, delta, dk, dv, part);
     TSD_LAUNCH_CHECK("attention_dkv");
     return TSD_OK;
