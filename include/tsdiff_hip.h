@@ -629,10 +629,13 @@ int tsd_layer_norm_bwd(int32_t dtype, int32_t rows, int32_t dim, const void* x, 
                        void* dbias, float* scratch, size_t scratch_floats, void* stream);
 /* h[rows,out] = act(x w_gate^T + b_gate) * (x w_up^T + b_up); weights [out, in] dense, biases [out] or NULL; `act` as in
  * tsd_act_fwd (0 .. 3).  The backward computes both projections again; any of its outputs may be NULL (each dense, the
- * layout of what it is the gradient of); scratch 16-byte aligned, tsd_gated_linear_scratch_floats floats. */
+ * layout of what it is the gradient of).  scratch: 16-byte aligned, as many floats as the query function says for the call
+ * (it looks at the addresses and strides of x and the weights; 0, then scratch may be NULL, for most forward calls). */
+size_t tsd_gated_linear_scratch_floats(int32_t dtype, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
+                                       const void* w_gate, const void* w_up, int32_t backward);
 int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
-                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, void* stream);
-size_t tsd_gated_linear_scratch_floats(int32_t dtype, int32_t rows, int32_t in, int32_t out);
+                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, float* scratch,
+                         size_t scratch_floats, void* stream);
 int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
                          const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, const void* dh,
                          int64_t lddh, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, float* scratch,

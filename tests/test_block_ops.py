@@ -62,15 +62,18 @@ def test_c_entries_refuse_before_any_launch():
     assert bwd(0, 4, 8, p, 8, p, p, 8, p, p, p, p, p, p, 1, None) == bad    # scratch
     assert bwd(0, 4, 8, p, 8, p, p, 8, p, p, p, p, p, None, 0, None) == bad
     g = lib.tsd_gated_linear_fwd
-    assert g(5, 0, 4, 8, 8, p, 8, p, p, None, None, p, None) == bad
-    assert g(0, 4, 4, 8, 8, p, 8, p, p, None, None, p, None) == bad         # activation
-    assert g(0, 0, 4, 0, 8, p, 8, p, p, None, None, p, None) == bad
-    assert g(0, 0, 4, 8, 8, p, 7, p, p, None, None, p, None) == bad
-    assert g(0, 0, 4, 8, 8, p, 8, p, None, None, None, p, None) == bad
-    assert g(0, 0, 4, 8, 8, p, 8, p, p, None, None, None, None) == bad
-    assert g(0, 0, 4, 1 << 21, 8, p, 1 << 21, p, p, None, None, p, None) == no
+    assert g(5, 0, 4, 8, 8, p, 8, p, p, None, None, p, None, 0, None) == bad
+    assert g(0, 4, 4, 8, 8, p, 8, p, p, None, None, p, None, 0, None) == bad         # activation
+    assert g(0, 0, 4, 0, 8, p, 8, p, p, None, None, p, None, 0, None) == bad
+    assert g(0, 0, 4, 8, 8, p, 7, p, p, None, None, p, None, 0, None) == bad
+    assert g(0, 0, 4, 8, 8, p, 8, p, None, None, None, p, None, 0, None) == bad
+    assert g(0, 0, 4, 8, 8, p, 8, p, p, None, None, None, None, 0, None) == bad
+    assert g(0, 0, 4, 1 << 21, 8, p, 1 << 21, p, p, None, None, p, None, 0, None) == no
+    n = lib.tsd_gated_linear_scratch_floats(1, 4096, 33, 64, p, 33, p, p, 0)  # rows that no 16-byte load fits: copies
+    assert n > 0 and g(1, 0, 4096, 33, 64, p, 33, p, p, None, None, p, p, n - 1, None) == bad
+    assert lib.tsd_gated_linear_scratch_floats(1, 4096, 32, 64, p, 32, p, p, 0) == 0
     gb = lib.tsd_gated_linear_bwd
-    n = lib.tsd_gated_linear_scratch_floats(0, 4, 8, 8)
+    n = lib.tsd_gated_linear_scratch_floats(0, 4, 8, 8, p, 8, p, p, 1)
     assert n > 0
     assert gb(0, 0, 4, 8, 8, p, 8, p, p, None, None, p, 8, p, p, p, None, None, p, n - 1, None) == bad
     assert gb(0, 0, 4, 8, 8, p, 8, p, p, None, None, p, 8, p, p, p, None, None, p + 4, n, None) == bad  # alignment

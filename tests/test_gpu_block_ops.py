@@ -108,7 +108,7 @@ def gated_check(got, grads, want):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,fin,out", [(1, 1, 1), (1, 16, 8), (17, 256, 512), (5, 24, 40), (130, 33, 70), (64, 64, 64),
-                                          (257, 100, 129), (300, 204, 530), (1000, 8, 16), (40, 1000, 12)])
+                                          (257, 100, 129), (300, 204, 530), (520, 965, 129), (1000, 8, 16), (40, 1000, 12)])
 def test_gated_linear(rows, fin, out, dtype):
     from tsdiff_amd.block_ops import gated_linear
     x, wg, wu, bg, bu, dh, want = gated_case(rows, fin, out, dtype, "swish", True)
@@ -380,9 +380,9 @@ def test_second_derivatives_and_wrong_types_are_refused():
 
 
 def test_offsets_past_32_bits():
-    """rows 2^22 values apart: the last ones lie past 2^31 values"""
+    """rows 2^21 values apart: the last ones lie past 2^31 values"""
     from tsdiff_amd import block_ops as B
-    n, gap = 520, 1 << 22
+    n, gap = 1040, 1 << 21
     far = torch.empty(n * gap, dtype=torch.bfloat16, device=DEV)
     x = normal(1, n, 64, dtype=torch.bfloat16).to(DEV)
     xf = far.view(n, gap)[:, :64]

@@ -217,8 +217,9 @@ SIGNATURES = {
     "tsd_layer_norm_bwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, _P, _P,
                                      _P, C.c_size_t, _P]),
     "tsd_gated_linear_fwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P,
-                                       _P, _P]),
-    "tsd_gated_linear_scratch_floats": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+                                       _P, _P, C.c_size_t, _P]),
+    "tsd_gated_linear_scratch_floats": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P,
+                                                     C.c_int32]),
     "tsd_gated_linear_bwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P,
                                        _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "tsd_graph_attention_scratch_floats": (C.c_size_t, [C.POINTER(Attention), C.c_int32]),

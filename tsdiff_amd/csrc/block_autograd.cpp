@@ -146,9 +146,12 @@ Tensor gated_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
     c10::DeviceGuard guard(x.device());
     const int32_t rows = count("gated_linear", x.size(0)), in = count("gated_linear", x.size(1)),
                   out = count("gated_linear", wg.size(0));
-    Tensor h = at::empty({rows, out}, x.options());
-    check(tsd_gated_linear_fwd(dtype_of(x.scalar_type()), (int32_t)act, rows, in, out, ptr(x), ld(x), ptr(wg), ptr(wu), ptr(bg),
-                               ptr(bu), ptr(h), stream_of(x)));
+    const int dtype = dtype_of(x.scalar_type());
+    Tensor h = at::empty({rows, out}, x.options()), scratch;
+    const size_t n = tsd_gated_linear_scratch_floats(dtype, rows, in, out, ptr(x), ld(x), ptr(wg), ptr(wu), 0);
+    if (n > 0) scratch = at::empty({(int64_t)n}, x.options().dtype(at::kFloat));
+    check(tsd_gated_linear_fwd(dtype, (int32_t)act, rows, in, out, ptr(x), ld(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), ptr(h),
+                               (float*)ptr(scratch), n, stream_of(x)));
     return h;
 }
 
@@ -172,7 +175,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const Tensor* like[5] = {&x, &wg, &wu, &bg, &bu};
         for (int k = 0; k < 5; ++k)
             if (needs(ctx, s, k)) g[k] = at::empty(like[k]->sizes(), x.options());
-        const size_t n = tsd_gated_linear_scratch_floats(dtype, rows, in, out);
+        const size_t n = tsd_gated_linear_scratch_floats(dtype, rows, in, out, ptr(x), ld(x), ptr(wg), ptr(wu), 1);
         Tensor scratch;
         if (n > 0) scratch = at::empty({(int64_t)n}, x.options().dtype(at::kFloat));
         check(tsd_gated_linear_bwd(dtype, (int32_t)ctx->saved_data["act"].toInt(), rows, in, out, ptr(x), ld(x), ptr(wg), ptr(wu),

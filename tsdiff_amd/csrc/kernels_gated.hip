@@ -35,7 +35,8 @@ template <int KIND> __device__ __forceinline__ float act_slope(int kind, float g
 
 struct GatedDims {
     int rows, in, out, outp;  // outp: out rounded up to 8, the width of each half of D
-    int64_t ldx, lddh;
+    int inw;                  // values a row of x and the weights as the products read them: in, or in rounded up to 8 (packed)
+    int64_t ldx, lddh, ldw;
     int kind;
     bool bvec;  // both biases: four values a load
     int xvw, wvw, dhvw, hvw, dxvw;  // values a load or store of x, the weights, dh, h, dx may take
@@ -112,8 +113,8 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
     const int m0 = at.lo * BM, f0 = at.sh * FT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave & 1, wm = wave >> 1;
     const int nbase = wn * (FT / 2), mrow = wm * (BM / 2);
-    const RowOperand<T> ns = {wg, wu, d.in, d.out, d.in, f0, FT, f0, d.wvw};
-    const RowOperand<T> ms = {x, x, d.ldx, d.rows, d.in, m0, BM, 0, d.xvw};
+    const RowOperand<T> ns = {wg, wu, d.ldw, d.out, d.inw, f0, FT, f0, d.wvw};
+    const RowOperand<T> ms = {x, x, d.ldx, d.rows, d.inw, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     f32x4 vbg[TN], vbu[TN];
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
     }
     Raw<T> dhr[BWD ? Out::U : 1];
     if constexpr (BWD) Out::fetch(dhr, dh + (int64_t)m0 * d.lddh + f0, d.lddh, d.rows - m0, d.out - f0, d.dhvw);
-    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.in, mrow,
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.inw, mrow,
                                [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     char* second = lds + Out::BYTES;
     float* red = reinterpret_cast<float*>(lds + 2 * Out::BYTES);  // [2 (wm)][2][FT] column sums
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktil
     const int m0 = at.lo * BM, k0 = at.sh * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
-    const ColOperand<T> ns = {wg, wu, d.in, d.in, d.out, k0, d.outp, d.wvw};
+    const ColOperand<T> ns = {wg, wu, d.ldw, d.inw, d.out, k0, d.outp, d.wvw};
     const RowOperand<T> ms = {D, D, 2 * d.outp, d.rows, 2 * d.outp, m0, BM, 0, 8};
     f32x4 acc[BN / 32][BM / 32];
     const int fb = blockIdx.y * share, fe = fb + share < 2 * d.outp ? fb + share : 2 * d.outp;
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
     const int64_t rb = (int64_t)blockIdx.y * rows_a_split;
     const int n = (int)(d.rows - rb < rows_a_split ? d.rows - rb : rows_a_split);
-    const ColOperand<T> ns = {x + rb * d.ldx, x, d.ldx, d.in, n, k0, 1 << 30, d.xvw};
+    const ColOperand<T> ns = {x + rb * d.ldx, x, d.ldx, d.inw, n, k0, 1 << 30, d.xvw};
     const ColOperand<T> ms = {D + rb * 2 * d.outp, D, 2 * d.outp, 2 * d.outp, n, f0, 1 << 30, 8};
     f32x4 acc[BN / 32][BM / 32];
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
@@ -261,6 +262,22 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
             const int f = f0 + mrow + i * 16 + r, k = k0 + nbase + j * 16 + c4;
             if (f < 2 * d.outp) store4(o + (int64_t)f * d.in + k, acc[j][i], d.in - k, d.in % 4 == 0);
         }
+}
+
+// x and the weights with rows of `inw` values, zeros behind the first `in`: a thread a chunk of 8
+template <class T>
+__global__ __launch_bounds__(256) void gated_pack_kernel(GatedDims d, const T* __restrict__ x, const T* __restrict__ wg,
+                                                         const T* __restrict__ wu, T* __restrict__ xp, T* __restrict__ wp) {
+    const int chunks = d.inw / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / chunks;
+    const int c = (int)(i % chunks) * 8, n = d.in - c;
+    if (row >= d.rows + 2 * (int64_t)d.out) return;
+    Raw<T> raw;
+    if (row < d.rows) load_raw(raw, x + row * d.ldx + c, n > 8 ? 8 : n, d.xvw);
+    else if (row < d.rows + (int64_t)d.out) load_raw(raw, wg + (row - d.rows) * d.in + c, n > 8 ? 8 : n, d.wvw);
+    else load_raw(raw, wu + (row - d.rows - d.out) * d.in + c, n > 8 ? 8 : n, d.wvw);
+    T* to = row < d.rows ? xp + row * d.inw + c : wp + (row - d.rows) * d.inw + c;
+    __builtin_memcpy(__builtin_assume_aligned(to, 16), &raw, sizeof(raw));
 }
 
 // the parts of dx (workgroups below xblocks), of dW (wblocks more) and of the column sums, added in order
@@ -313,11 +330,12 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblo
     }
 }
 
-// Tiles of an output of m x n: 128 x 128 where they fill the 256 CUs, else 64 x 64, else 32 x 64.
-enum { TILE_128, TILE_64, TILE_32 };
-static const int TILE_M[3] = {128, 64, 32}, TILE_N[3] = {128, 64, 64};
+// Tiles of an output of m x n: 128 x 128 where they fill the 256 CUs, else 64 x 64, else 32 x 64; guarded loads: 32 x 64.
+enum { TILE_128, TILE_64, TILE_32, TILE_GUARDED };
+static const int TILE_M[4] = {128, 64, 32, 32}, TILE_N[4] = {128, 64, 64, 64};
 static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
-static int gated_tile(int64_t m, int64_t n, int64_t times) {
+static int gated_tile(int64_t m, int64_t n, int64_t times, bool guarded) {
+    if (guarded) return TILE_GUARDED;
     for (int t = TILE_128; t < TILE_32; ++t)
         if (times * div_up(m, TILE_M[t]) * div_up(n, TILE_N[t]) >= 256) return t;
     return TILE_32;
@@ -326,24 +344,30 @@ static int gated_tile(int64_t m, int64_t n, int64_t times) {
     switch (tile) {                                                                    \
         case TILE_128: { constexpr int BM = 128, BN = 128; __VA_ARGS__; } break;       \
         case TILE_64: { constexpr int BM = 64, BN = 64; __VA_ARGS__; } break;          \
-        default: { constexpr int BM = 32, BN = 64; __VA_ARGS__; } break;               \
+        case TILE_32: { constexpr int BM = 32, BN = 64; __VA_ARGS__; } break;          \
+        default: break;                                                                \
     }
 
 struct GatedScratch {  // bytes from the start
-    size_t D, bpart, wpart, xpart, total;
+    size_t pack, D, bpart, wpart, xpart, total;
     int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
     int wtile, splits, rows_a_split;   // of dW
     int xtile, xsplits, share;         // of dx
 };
-static GatedScratch gated_scratch(int dtype, int rows, int in, int out) {
+// Rows that no 16-byte load fits are copied to rows that it does where the products are long enough to pay for the launch;
+// below, their tiles come in by narrower, guarded loads (2 rows of 19 -> 177 f32 values, forward: 6 us against 9; 2066 of
+// 965 -> 1292 f16, forward and backward: 570 us against 110).
+static bool gated_packed(int rows, int in, int out) { return (int64_t)rows * in * out >= (1 << 22); }
+static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fast, bool bwd) {
     GatedScratch s = {};
-    const size_t outp = ((size_t)out + 7) / 8 * 8, es = dtype == TSD_F32 ? 4 : 2;
+    const size_t outp = ((size_t)out + 7) / 8 * 8, inp = ((size_t)in + 7) / 8 * 8, es = dtype == TSD_F32 ? 4 : 2;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    s.tile = gated_tile(rows, 2 * outp, 1);
+    const bool guarded = !fast && !gated_packed(rows, in, out);
+    s.tile = gated_tile(rows, 2 * outp, 1, guarded);
     s.mtiles = div_up(rows, TILE_M[s.tile]);
     // dW: the rows in shares of at least 256, about two workgroups a CU
     const int most = div_up(rows, 256);
-    s.wtile = gated_tile(2 * outp, in, most);
+    s.wtile = gated_tile(2 * outp, in, most, guarded);
     if (s.wtile == TILE_32) s.wtile = TILE_64;
     const int tiles = div_up(2 * outp, TILE_M[s.wtile]) * div_up(in, TILE_N[s.wtile]);
     int n = div_up(512, tiles);
@@ -353,17 +377,22 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out) {
     s.splits = div_up(rows, s.rows_a_split);
     // dx: the largest tiles that fill the chip with shares of at least eight steps of the contraction
     const int steps = div_up(2 * outp, GEMM_K);
-    for (s.xtile = TILE_128;; ++s.xtile) {
+    for (s.xtile = guarded ? TILE_GUARDED : TILE_128;; ++s.xtile) {
         const int t = div_up(rows, TILE_M[s.xtile]) * div_up(in, TILE_N[s.xtile]);
         int x = div_up(512, t > 0 ? t : 1);
         x = x < steps / 8 ? x : steps / 8;
         x = x < 1 ? 1 : x;
         s.share = div_up(steps, x) * GEMM_K;
         s.xsplits = div_up(2 * outp, s.share);
-        if (s.xtile == TILE_32 || (int64_t)t * s.xsplits >= 256) break;
+        if (s.xtile >= TILE_32 || (int64_t)t * s.xsplits >= 256) break;
     }
-    s.D = 0;
-    s.bpart = up((size_t)rows * 2 * outp * es);
+    s.pack = 0;
+    s.D = up(!fast && gated_packed(rows, in, out) ? ((size_t)rows + 2 * (size_t)out) * inp * es : 0);
+    if (!bwd) {
+        s.total = s.D;
+        return s;
+    }
+    s.bpart = s.D + up((size_t)rows * 2 * outp * es);
     s.wpart = s.bpart + up((size_t)s.mtiles * 2 * outp * 4);
     s.xpart = s.wpart + up((size_t)s.splits * 2 * outp * in * 4);
     s.total = s.xpart + (s.xsplits > 1 ? up((size_t)s.xsplits * rows * in * 4) : 0);
@@ -393,6 +422,8 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
     d.out = out;
     d.outp = (out + 7) / 8 * 8;
     d.ldx = ldx;
+    d.inw = in;
+    d.ldw = in;
     d.kind = act;
     d.xvw = load_width(sizeof(T), in, ldx, x);
     const int a = load_width(sizeof(T), in, in, wg), b = load_width(sizeof(T), in, in, wu);
@@ -402,6 +433,24 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
 }
 // 16-byte loads everywhere, and a tile's rows within the 2 GiB that a buffer's offsets reach
 static bool gated_fast(const GatedDims& d) { return d.xvw == 8 && d.wvw == 8 && d.ldx <= (1 << 21); }
+
+// packed: x, wg and wu become the copies in scratch
+template <class T>
+static int gated_pack(GatedDims& d, const void*& x, const void*& wg, const void*& wu, char* scratch, hipStream_t st) {
+    if (gated_fast(d) || !gated_packed(d.rows, d.in, d.out)) return TSD_OK;
+    d.inw = (d.in + 7) / 8 * 8;
+    T *xp = reinterpret_cast<T*>(scratch), *wp = xp + (int64_t)d.rows * d.inw;
+    const int64_t chunks = ((int64_t)d.rows + 2 * (int64_t)d.out) * (d.inw / 8);
+    hipLaunchKernelGGL(gated_pack_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, d, (const T*)x,
+                       (const T*)wg, (const T*)wu, xp, wp);
+    TSD_LAUNCH_CHECK("gated_pack");
+    x = xp;
+    wg = wp;
+    wu = wp + (int64_t)d.out * d.inw;
+    d.ldx = d.ldw = d.inw;
+    d.xvw = d.wvw = 8;
+    return TSD_OK;
+}
 
 template <class T, int BM, int BN, bool FAST, bool BWD>
 static int gated_first(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
@@ -444,16 +493,16 @@ static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* 
     return TSD_OK;
 }
 template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
-    GATED_BY_TILE(tile, BM, BN, {
-        if (gated_fast(d)) return gated_first<T, BM, BN, true, BWD>(d, a...);
-        return gated_first<T, BM, BN, false, BWD>(d, a...);
-    });
+    GATED_BY_TILE(tile, BM, BN, { return gated_first<T, BM, BN, true, BWD>(d, a...); });
+    return gated_first<T, 32, 64, false, BWD>(d, a...);
 }
 
 template <class T>
-static int gated_bwd(GatedDims d, const GatedScratch& s, const void* x, const void* wg, const void* wu, const void* bg,
-                     const void* bu, const void* dh, int64_t lddh, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
-                     char* scratch, hipStream_t st) {
+static int gated_bwd(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                     const void* dh, int64_t lddh, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
+                     const GatedScratch& s, char* scratch, hipStream_t st) {
+    const int prc = d.rows > 0 ? gated_pack<T>(d, x, wg, wu, scratch + s.pack, st) : TSD_OK;
+    if (prc != TSD_OK) return prc;
     T* D = reinterpret_cast<T*>(scratch + s.D);
     float* bpart = reinterpret_cast<float*>(scratch + s.bpart);
     float* wpart = reinterpret_cast<float*>(scratch + s.wpart);
@@ -466,14 +515,12 @@ static int gated_bwd(GatedDims d, const GatedScratch& s, const void* x, const vo
         d.dxvw = load_width(sizeof(T), d.in, d.in, dx);
         rc = gated_first_by<T, true>(s.tile, d, x, wg, wu, bg, bu, dh, (void*)nullptr, (void*)D, sums ? bpart : (float*)nullptr, st);
         if (rc == TSD_OK && dx != nullptr) {
-            GATED_BY_TILE(s.xtile, BM, BN, {
-                rc = gated_fast(d) ? gated_dx<T, BM, BN, true>(d, s, D, wg, wu, dx, xpart, st) : gated_dx<T, BM, BN, false>(d, s, D, wg, wu, dx, xpart, st);
-            });
+            GATED_BY_TILE(s.xtile, BM, BN, { rc = gated_dx<T, BM, BN, true>(d, s, D, wg, wu, dx, xpart, st); });
+            if (s.xtile == TILE_GUARDED) rc = gated_dx<T, 32, 64, false>(d, s, D, wg, wu, dx, xpart, st);
         }
         if (rc == TSD_OK && weights) {
-            GATED_BY_TILE(s.wtile, BM, BN, {
-                rc = gated_fast(d) ? gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st) : gated_dw<T, BM, BN, false>(d, s, D, x, wpart, st);
-            });
+            GATED_BY_TILE(s.wtile, BM, BN, { rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st); });
+            if (s.wtile == TILE_GUARDED) rc = gated_dw<T, 32, 64, false>(d, s, D, x, wpart, st);
         }
     }
     const bool parts = d.rows > 0 && dx != nullptr && s.xsplits > 1;
@@ -495,24 +542,34 @@ using namespace tsd::blk;
 
 extern "C" {
 
+size_t tsd_gated_linear_scratch_floats(int32_t dtype, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
+                                       const void* w_gate, const void* w_up, int32_t backward) {
+    if (rows < 1 || in < 1 || out < 1) return 0;
+    TSD_BY_DTYPE(dtype, T, {
+        const GatedDims d = gated_dims<T>(rows, in, out, 0, x, ldx, w_gate, w_up, nullptr, nullptr);
+        return gated_scratch(dtype, rows, in, out, gated_fast(d), backward != 0).total / 4;
+    });
+    return 0;
+}
+
 int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
-                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, void* stream) {
-    const int rc = gated_check("tsd_gated_linear_fwd", dtype, act, rows, in, out, ldx, x, w_gate, w_up);
+                         const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, float* scratch,
+                         size_t scratch_floats, void* stream) {
+    int rc = gated_check("tsd_gated_linear_fwd", dtype, act, rows, in, out, ldx, x, w_gate, w_up);
     if (rc != TSD_OK) return rc;
     if (rows == 0) return TSD_OK;
     TSD_REQUIRE(h != nullptr, "tsd_gated_linear_fwd: null pointer");
     TSD_BY_DTYPE(dtype, T, {
         GatedDims d = gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, b_gate, b_up);
+        const GatedScratch s = gated_scratch(dtype, rows, in, out, gated_fast(d), false);
+        TSD_REQUIRE(s.total == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats * 4 >= s.total),
+                    "tsd_gated_linear_fwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, s.total / 4);
         d.hvw = load_width(sizeof(T), out, out, h);
-        return gated_first_by<T, false>(gated_tile(rows, 2 * (int64_t)d.outp, 1), d, x, w_gate, w_up, b_gate, b_up,
-                                        (const void*)nullptr, h, (void*)nullptr, (float*)nullptr, (hipStream_t)stream);
+        if ((rc = gated_pack<T>(d, x, w_gate, w_up, (char*)scratch, (hipStream_t)stream)) != TSD_OK) return rc;
+        return gated_first_by<T, false>(s.tile, d, x, w_gate, w_up, b_gate, b_up, (const void*)nullptr, h, (void*)nullptr,
+                                        (float*)nullptr, (hipStream_t)stream);
     });
     return TSD_OK;
-}
-
-size_t tsd_gated_linear_scratch_floats(int32_t dtype, int32_t rows, int32_t in, int32_t out) {
-    if (rows < 1 || in < 1 || out < 1) return 0;
-    return gated_scratch(dtype, rows, in, out).total / 4;
 }
 
 int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, int32_t out, const void* x, int64_t ldx,
@@ -521,13 +578,15 @@ int tsd_gated_linear_bwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
                          size_t scratch_floats, void* stream) {
     const int rc = gated_check("tsd_gated_linear_bwd", dtype, act, rows, in, out, ldx, x, w_gate, w_up);
     if (rc != TSD_OK) return rc;
-    const GatedScratch s = gated_scratch(dtype, rows, in, out);
     TSD_REQUIRE(rows == 0 || (dh != nullptr && lddh >= out), "tsd_gated_linear_bwd: null pointer or row stride");
-    TSD_REQUIRE(rows == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats * 4 >= s.total),
-                "tsd_gated_linear_bwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, s.total / 4);
-    TSD_BY_DTYPE(dtype, T, return gated_bwd<T>(gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, b_gate, b_up), s, x, w_gate, w_up,
-                                               b_gate, b_up, dh, lddh, dx, dw_gate, dw_up, db_gate, db_up, (char*)scratch,
-                                               (hipStream_t)stream));
+    TSD_BY_DTYPE(dtype, T, {
+        const GatedDims d = gated_dims<T>(rows, in, out, act, x, ldx, w_gate, w_up, b_gate, b_up);
+        const GatedScratch s = gated_scratch(dtype, rows, in, out, gated_fast(d), true);
+        TSD_REQUIRE(rows == 0 || (scratch != nullptr && aligned16(scratch) && scratch_floats * 4 >= s.total),
+                    "tsd_gated_linear_bwd: scratch of %zu floats, %zu needed (16-byte aligned)", scratch_floats, s.total / 4);
+        return gated_bwd<T>(d, x, w_gate, w_up, b_gate, b_up, dh, lddh, dx, dw_gate, dw_up, db_gate, db_up, s, (char*)scratch,
+                            (hipStream_t)stream);
+    });
     return TSD_OK;
 }
 
