@@ -655,12 +655,16 @@ typedef struct tsd_attention {
     const uint8_t* key_mask;         /* [num_keys] or NULL */
 } tsd_attention;
 size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backward);
-/* out [num_queries, heads, dim] dense; lse [num_queries, heads]: log2 of the sum of 2^(score log2 e), what the backward needs
- * (NULL: not kept); scratch (16-byte aligned) may be NULL where the query function says 0 floats. */
-int tsd_graph_attention_fwd(const tsd_attention* a, void* out, float* lse, float* scratch, size_t scratch_floats, void* stream);
-/* dq, dk, dv dense in the layouts of q, k, v; do_row / do_head: strides of dout */
-int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float* lse, const void* dout, int64_t do_row,
-                            int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream);
+/* out [num_queries, heads, dim] dense.  For the backward: lse [num_queries, heads], log2 of the sum of 2^(score log2 e), and for
+ * bf16 / f16 out_rest, what the rounding of `out` left (same type and shape: sum dO O, which the gradients of the scores are
+ * taken from, needs more digits than `out` has).  Either NULL: not kept.  scratch (16-byte aligned) may be NULL where the query
+ * function says 0 floats. */
+int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats,
+                            void* stream);
+/* dq, dk, dv dense in the layouts of q, k, v; do_row / do_head: strides of dout; out_rest may be NULL */
+int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const void* out_rest, const float* lse, const void* dout,
+                            int64_t do_row, int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats,
+                            void* stream);
 
 #ifdef __cplusplus
 }

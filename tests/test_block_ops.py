@@ -88,15 +88,15 @@ def test_c_entries_refuse_before_any_launch():
     af, ab = lib.tsd_graph_attention_fwd, lib.tsd_graph_attention_bwd
     for kw in (dict(dtype=7), dict(kv_heads=3), dict(kv_heads=0), dict(dim=0), dict(num_graphs=-1), dict(q=None), dict(v=None),
                dict(q_ptr=None), dict(k_ptr=None), dict(num_keys=-1)):
-        assert af(att(**kw), p, None, None, 0, None) == bad, kw
-    assert af(att(dim=129), p, None, None, 0, None) == no
-    assert af(att(num_queries=1 << 30), p, None, None, 0, None) == no
-    assert af(att(), None, None, None, 0, None) == bad
-    assert ab(att(), p, p, p, 32, 8, p, p, p, None, 0, None) == bad          # scratch
-    assert ab(att(), p, p, p, 32, 8, None, p, p, p, 1 << 20, None) == bad
+        assert af(att(**kw), p, None, None, None, 0, None) == bad, kw
+    assert af(att(dim=129), p, None, None, None, 0, None) == no
+    assert af(att(num_queries=1 << 30), p, None, None, None, 0, None) == no
+    assert af(att(), None, None, None, None, 0, None) == bad
+    assert ab(att(), p, None, p, p, 32, 8, p, p, p, None, 0, None) == bad          # scratch
+    assert ab(att(), p, None, p, p, 32, 8, None, p, p, p, 1 << 20, None) == bad
     long = dict(num_graphs=1, num_queries=1, num_keys=1 << 16)               # few rows, many keys: parts to be joined
     n = lib.tsd_graph_attention_scratch_floats(att(**long), 0)
-    assert n > 0 and af(att(**long), p, None, p, n - 1, None) == bad
+    assert n > 0 and af(att(**long), p, None, None, p, n - 1, None) == bad
 
 
 def close(got, want, tol=1e-6):

@@ -223,9 +223,9 @@ SIGNATURES = {
     "tsd_gated_linear_bwd": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P,
                                        _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "tsd_graph_attention_scratch_floats": (C.c_size_t, [C.POINTER(Attention), C.c_int32]),
-    "tsd_graph_attention_fwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_size_t, _P]),
-    "tsd_graph_attention_bwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, C.c_size_t,
-                                          _P]),
+    "tsd_graph_attention_fwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, _P, C.c_size_t, _P]),
+    "tsd_graph_attention_bwd": (C.c_int, [C.POINTER(Attention), _P, _P, _P, _P, C.c_int64, C.c_int64, _P, _P, _P, _P,
+                                          C.c_size_t, _P]),
     "tsd_sampler_plan_create": (C.c_int, [_CFG, C.POINTER(Batch), C.c_int32, C.c_float, C.c_float, _P, _P, _P,
                                           C.POINTER(_P)]),
     "tsd_sampler_plan_run": (C.c_int, [_P, C.c_int32, C.POINTER(RunArgs), C.c_int32, _P]),

@@ -235,22 +235,24 @@ tsd_attention attention_args(const Tensor& q, const Tensor& k, const Tensor& v, 
     return a;
 }
 Tensor attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Tensor& k_ptr,
-                     const Tensor& mask, double scale, Tensor* lse) {
+                     const Tensor& mask, double scale, Tensor* rest, Tensor* lse) {
     c10::DeviceGuard guard(q.device());
     const tsd_attention a = attention_args(q, k, v, q_ptr, k_ptr, mask, scale);
     Tensor out = at::empty(q.sizes(), q.options()), scratch;
     if (lse != nullptr) *lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    if (rest != nullptr && q.scalar_type() != at::kFloat) *rest = at::empty(q.sizes(), q.options());
     const size_t n = tsd_graph_attention_scratch_floats(&a, 0);
     if (n > 0) scratch = at::empty({(int64_t)n}, q.options().dtype(at::kFloat));
-    check(tsd_graph_attention_fwd(&a, ptr(out), lse != nullptr ? (float*)ptr(*lse) : nullptr, (float*)ptr(scratch), n, stream_of(q)));
+    check(tsd_graph_attention_fwd(&a, ptr(out), rest != nullptr ? ptr(*rest) : nullptr, lse != nullptr ? (float*)ptr(*lse) : nullptr,
+                                  (float*)ptr(scratch), n, stream_of(q)));
     return out;
 }
 
 struct GraphAttention : torch::autograd::Function<GraphAttention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr,
                           const Tensor& k_ptr, const Opt& mask, double scale) {
-        Tensor lse, out = attention_fwd(q, k, v, q_ptr, k_ptr, given(mask), scale, &lse);
-        ctx->save_for_backward({q, k, v, q_ptr, k_ptr, given(mask), out, lse});
+        Tensor lse, rest, out = attention_fwd(q, k, v, q_ptr, k_ptr, given(mask), scale, &rest, &lse);
+        ctx->save_for_backward({q, k, v, q_ptr, k_ptr, given(mask), out, lse, rest});
         ctx->saved_data["scale"] = scale;
         return out;
     }
@@ -265,7 +267,7 @@ struct GraphAttention : torch::autograd::Function<GraphAttention> {
         const size_t n = tsd_graph_attention_scratch_floats(&a, 1);
         Tensor scratch;
         if (n > 0) scratch = at::empty({(int64_t)n}, lse.options());
-        check(tsd_graph_attention_bwd(&a, ptr(out), (const float*)ptr(lse), ptr(dout), dout.stride(0), dout.stride(1), ptr(dq),
+        check(tsd_graph_attention_bwd(&a, ptr(out), ptr(s[8]), (const float*)ptr(lse), ptr(dout), dout.stride(0), dout.stride(1), ptr(dq),
                                       ptr(dk), ptr(dv), (float*)ptr(scratch), n, stream_of(q)));
         return once("graph_attention", {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
     }
@@ -303,7 +305,7 @@ Tensor graph_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(2));
     const Tensor qh = heads_of(q), kh = heads_of(k), vh = heads_of(v);
     return wants_grad({&qh, &kh, &vh}) ? GraphAttention::apply(qh, kh, vh, qp, kpi, maybe(mask), s)
-                                       : attention_fwd(qh, kh, vh, qp, kpi, mask, s, nullptr);
+                                       : attention_fwd(qh, kh, vh, qp, kpi, mask, s, nullptr, nullptr);
 }
 
 }  // namespace

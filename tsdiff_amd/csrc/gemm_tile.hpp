@@ -37,17 +37,19 @@ template <class T> struct RowOperand {
     }
     __device__ __forceinline__ bool second(int r, int) const { return r >= split; }
 };
-// Rows of the contraction, from `ksplit` on those of a second matrix (kmax rows each); columns first ..
+// Rows of the contraction, from `ksplit` on those of a second matrix (kmax rows each), from `wrap` on all of them once more
+// (wrap: a multiple of 16); columns first ..
 template <class T> struct ColOperand {
     static constexpr bool ACROSS = true;
     const T *p, *p2;
     int64_t ld;
-    int cols, kmax, first, ksplit;
+    int cols, kmax, first, ksplit, wrap;
     int vw;  // load_raw's
     template <int N> using TileOf = Tile<T, GEMM_K, N / 8>;
     __device__ __forceinline__ void load(Raw<T>& raw, int r, int c, int k) const {
-        const bool two = k + r >= ksplit;
-        const int kk = k + r - (two ? ksplit : 0), col = first + c * 8, n = kk < kmax ? cols - col : 0;
+        const int kr = k + r - (k + r >= wrap ? wrap : 0);
+        const bool two = kr >= ksplit;
+        const int kk = kr - (two ? ksplit : 0), col = first + c * 8, n = kk < kmax ? cols - col : 0;
         load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)kk * ld + col : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
     }
 };
@@ -83,9 +85,10 @@ template <class T, int N, class Op, bool PERMUTED> struct Places {
             const int wave_row = __builtin_amdgcn_readfirstlane(row[i]);
             if constexpr (!Op::ACROSS) {
                 f(i, dma_buffer(op.base(wave_row >= op.split, k)), k + chunk[i] * 8 < op.kmax ? off[i] : DMA_NOWHERE);
-            } else {  // ksplit is a multiple of 8, as few rows as a wave's load may hold: it lies on one side
-                const bool two = k + wave_row >= op.ksplit;
-                const int kk = k - (two ? op.ksplit : 0);
+            } else {  // ksplit and wrap are multiples of 8, as few rows as a wave's load may hold: it lies on one side
+                const int kw = k - (k + wave_row >= op.wrap ? op.wrap : 0);
+                const bool two = kw + wave_row >= op.ksplit;
+                const int kk = kw - (two ? op.ksplit : 0);
                 f(i, dma_buffer((two ? op.p2 : op.p) + (int64_t)kk * op.ld + op.first),
                   kk + row[i] < op.kmax ? off[i] : DMA_NOWHERE);
             }

@@ -223,6 +223,29 @@ template <class T> __device__ __forceinline__ Chunk<T> joined(const f32x4& a, co
     const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return to_chunk(x, T());
 }
+// The weights as a matrix operand: rounded to the tensors' type where a wave has many products to do (f32: its three
+// planes); for the small graphs of one wave with what the rounding leaves as a second operand, at no cost that shows.
+template <class T, bool REST> struct Weights {
+    Chunk<T> c, rest;
+    __device__ __forceinline__ Weights() = default;
+    __device__ __forceinline__ Weights(const f32x4& a, const f32x4& b) {
+        c = joined<T>(a, b);
+        if constexpr (REST) {
+            f32x4 x = a, y = b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] -= (float)c.p[0][e];
+                y[e] -= (float)c.p[0][4 + e];
+            }
+            rest = joined<T>(x, y);
+        }
+    }
+    __device__ __forceinline__ f32x4 times(const Chunk<T>& v, f32x4 acc) const {
+        if constexpr (REST) acc = mma(v, rest, acc);
+        return mma(v, c, acc);
+    }
+};
+template <class T, int WAVES> constexpr bool att_rest() { return sizeof(T) == 2 && WAVES == 1; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // over the four lanes l % 16 + 0, 16, 32, 48
 template <class F> __device__ __forceinline__ float over_groups(float v, F f) {
@@ -298,7 +321,8 @@ template <class T, bool FAST> constexpr int att_buffers() { return att_dma<T, FA
 template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, T* __restrict__ out,
-                                                             float* __restrict__ lse, float* __restrict__ part) {
+                                                             T* __restrict__ rest, float* __restrict__ lse,
+                                                             float* __restrict__ part) {
     constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
     using Stage = RowStage<T, KT, DP, NT, FAST>;
     using KTile = typename Stage::Lds;
@@ -409,14 +433,14 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
             }
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b) {
-                Chunk<T> p[RS];
+                Weights<T, att_rest<T, WAVES>()> p[RS];
 #pragma unroll
-                for (int x = 0; x < RS; ++x) p[x] = joined<T>(s[x][2 * b], s[x][2 * b + 1]);
+                for (int x = 0; x < RS; ++x) p[x] = {s[x][2 * b], s[x][2 * b + 1]};
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     const Chunk<T> vf = KTile::get_across(vl, b * 32, t);
 #pragma unroll
-                    for (int x = 0; x < RS; ++x) o[x][t] = mma(vf, p[x], o[x][t]);
+                    for (int x = 0; x < RS; ++x) o[x][t] = p[x].times(vf, o[x][t]);
                 }
             }
         });
@@ -442,8 +466,15 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
         }
         const float inv = ls > 0.f ? __builtin_amdgcn_rcpf(ls) : ls == 0.f ? 0.f : ls;
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t)
-            store4(out + at * d.dim + t * 16 + g * 4, o[x][t] * inv, d.dim - t * 16 - g * 4, d.ovec);
+        for (int t = 0; t < DP / 16; ++t) {
+            f32x4 v = o[x][t] * inv;
+            store4(out + at * d.dim + t * 16 + g * 4, v, d.dim - t * 16 - g * 4, d.ovec);
+            if (rest != nullptr) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] -= to_f((T)v[e]);
+                store4(rest + at * d.dim + t * 16 + g * 4, v, d.dim - t * 16 - g * 4, d.ovec);
+            }
+        }
         if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? -INFINITY : m[x] + __builtin_amdgcn_logf(ls);
     }
     }
@@ -452,7 +483,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
 // The parts of a row: out = sum_z 2^(m_z - m) O_z / sum_z 2^(m_z - m) l_z, 64 rows' values a workgroup
 template <class T>
 __global__ __launch_bounds__(256) void att_join_kernel(int64_t all, int dim, int splits, const float* __restrict__ part,
-                                                       T* __restrict__ out, float* __restrict__ lse) {
+                                                        T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, at = i / dim;
     if (at >= all) return;
     const int e = (int)(i % dim);
@@ -468,7 +499,9 @@ __global__ __launch_bounds__(256) void att_join_kernel(int64_t all, int dim, int
         l += a * stat[2 * (z * all + at) + 1];
         o += a * part[(z * all + at) * dim + e];
     }
-    out[i] = (T)(l == 0.f ? 0.f : o / l);
+    const float v = l == 0.f ? 0.f : o / l;
+    out[i] = (T)v;
+    if (rest != nullptr) rest[i] = (T)(v - to_f((T)v));
     if (lse != nullptr && e == 0) lse[at] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -492,7 +525,7 @@ __global__ __launch_bounds__(256) void att_sum_kernel(int64_t n, int splits, con
 template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                             const T* __restrict__ v, const T* __restrict__ out,
-                                                            const T* __restrict__ dout, const float* __restrict__ lse,
+                                                            const T* __restrict__ rest, const T* __restrict__ dout, const float* __restrict__ lse,
                                                             float* __restrict__ delta, T* __restrict__ dq,
                                                             float* __restrict__ part) {
     constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
@@ -531,6 +564,12 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
             row_raw(o, orow, row, mine, b);
             gf[x][b] = raw_chunk(a);
             s += raw_dot(a, o);
+            if (rest != nullptr) {
+                Rows<T> more = orow;
+                more.p = rest + (orow.p - out);
+                row_raw(o, more, row, mine, b);
+                s += raw_dot(a, o);
+            }
         }
         del[x] = over_groups_sum(s);
         const int qi = mine ? query_of(row, d.group) : 0;
@@ -582,7 +621,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                     }
                 }
                 const uint32_t bits = (uint32_t)(open >> (32 * p + 8 * g));
-                Chunk<T> f[RS];
+                Weights<T, att_rest<T, WAVES>()> f[RS];
 #pragma unroll
                 for (int x = 0; x < RS; ++x) {
 #pragma unroll
@@ -592,13 +631,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                             const float w = exp2_fast(__builtin_fmaf(s[x][u][e], d.scale2, -safe[x])) * (dp[x][u][e] - del[x]);
                             s[x][u][e] = bits >> (4 * u + e) & 1 ? w : 0.f;
                         }
-                    f[x] = joined<T>(s[x][0], s[x][1]);
+                    f[x] = {s[x][0], s[x][1]};
                 }
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     const Chunk<T> kc = KTile::get_across(kl, p * 32, t);
 #pragma unroll
-                    for (int x = 0; x < RS; ++x) acc[x][t] = mma(kc, f[x], acc[x][t]);
+                    for (int x = 0; x < RS; ++x) acc[x][t] = f[x].times(kc, acc[x][t]);
                 }
             }
         });
@@ -725,7 +764,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                         }
                     }
                 }
-                Chunk<T> pf[KS], df[KS];
+                Weights<T, att_rest<T, WAVES>()> pf[KS], df[KS];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const f32x4 L = *reinterpret_cast<const f32x4*>(stat + 32 * p + 8 * g + 4 * u);
@@ -741,17 +780,17 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                 }
 #pragma unroll
                 for (int x = 0; x < KS; ++x) {
-                    pf[x] = joined<T>(s[x][0], s[x][1]);
-                    df[x] = joined<T>(dp[x][0], dp[x][1]);
+                    pf[x] = {s[x][0], s[x][1]};
+                    df[x] = {dp[x][0], dp[x][1]};
                 }
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     const Chunk<T> gc = RTile::get_across(gl, p * 32, t);
 #pragma unroll
-                    for (int x = 0; x < KS; ++x) av[x][t] = mma(gc, pf[x], av[x][t]);
+                    for (int x = 0; x < KS; ++x) av[x][t] = pf[x].times(gc, av[x][t]);
                     const Chunk<T> qc = RTile::get_across(ql, p * 32, t);
 #pragma unroll
-                    for (int x = 0; x < KS; ++x) ak[x][t] = mma(qc, df[x], ak[x][t]);
+                    for (int x = 0; x < KS; ++x) ak[x][t] = df[x].times(qc, ak[x][t]);
                 }
             }
         });
@@ -898,7 +937,8 @@ static AttDims att_dims(const tsd_attention& a) {
 // rows of a tile of the other side: what keeps three workgroups on a CU
 template <class T, int DP, int WAVES> constexpr int att_tile() { return WAVES == 1 || DP == 128 || sizeof(T) == 4 ? 32 : 64; }
 template <class T, int DP, int WAVES, int RS, bool FAST>
-static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse, float* scratch, hipStream_t st) {
+static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, T* rest, float* lse, float* scratch,
+                          hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
     constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
@@ -906,13 +946,13 @@ static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, float* lse,
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
-                       (const T*)a.v, out, lse, scratch);
+                       (const T*)a.v, out, rest, lse, scratch);
     TSD_LAUNCH_CHECK("attention_fwd");
     return TSD_OK;
 }
 template <class T, int DP, int WAVES, int RS, bool FAST>
-static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* dout, const float* lse, float* delta, T* dq,
-                         float* part, hipStream_t st) {
+static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* rest, const T* dout, const float* lse, float* delta,
+                         T* dq, float* part, hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
     constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
@@ -920,7 +960,7 @@ static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const 
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
-                       (const T*)a.v, out, dout, lse, delta, dq, part);
+                       (const T*)a.v, out, rest, dout, lse, delta, dq, part);
     TSD_LAUNCH_CHECK("attention_dq");
     return TSD_OK;
 }
@@ -946,23 +986,23 @@ static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, cons
     else if constexpr (sizeof(T) == 2) rc = launch<T, DP, 4, 2, true>(__VA_ARGS__);
 
 template <class T, int DP>
-static int att_fwd(AttDims d, const tsd_attention& a, void* out, float* lse, float* scratch, hipStream_t st) {
+static int att_fwd(AttDims d, const tsd_attention& a, void* out, void* rest, float* lse, float* scratch, hipStream_t st) {
     const bool aligned = att_aligned(a, nullptr, 0, 0);
     const AttPlan p = att_plan(a, aligned);
     d.splits = p.splits_q;
-    d.ovec = d.dim % 4 == 0 && aligned16(out);
+    d.ovec = d.dim % 4 == 0 && aligned16(out) && aligned16(rest);
     int rc;
-    ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_fwd, d, a, (T*)out, lse, scratch, st);
+    ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_fwd, d, a, (T*)out, (T*)rest, lse, scratch, st);
     if (rc == TSD_OK && d.splits > 1) {
         const int64_t all = (int64_t)d.rows_q * d.heads;
         hipLaunchKernelGGL(att_join_kernel<T>, dim3((unsigned)((all * d.dim + 255) / 256)), dim3(256), 0, st, all, d.dim, d.splits,
-                           scratch, (T*)out, lse);
+                           scratch, (T*)out, (T*)rest, lse);
         TSD_LAUNCH_CHECK("attention_join");
     }
     return rc;
 }
 template <class T, int DP>
-static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const void* dout, int64_t do_row, int64_t do_head,
+static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const void* rest, const void* dout, int64_t do_row, int64_t do_head,
                    const float* lse, void* dq, void* dk, void* dv, float* scratch, hipStream_t st) {
     const bool aligned = att_aligned(a, dout, do_row, do_head);
     const AttPlan p = att_plan(a, aligned);
@@ -970,11 +1010,12 @@ static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const voi
     d.do_row = do_row;
     d.do_head = do_head;
     d.dovw = att_width(dout, do_row, do_head, d.dim, sizeof(T));
-    d.ovec = d.dim % 8 == 0 && aligned16(out) && aligned16(dq) && aligned16(dk) && aligned16(dv);
+    d.ovec = d.dim % 8 == 0 && aligned16(out) && aligned16(rest) && aligned16(dq) && aligned16(dk) && aligned16(dv);
     int rc = TSD_OK;
     if (d.rows_q > 0) {
         d.splits = p.splits_q;
-        ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_dq, d, a, (const T*)out, (const T*)dout, lse, delta, (T*)dq, part, st);
+        ATT_BY_SIDE(rc, p.side_q, aligned, att_launch_dq, d, a, (const T*)out, (const T*)rest, (const T*)dout, lse, delta, (T*)dq, part,
+                    st);
         if (rc == TSD_OK && d.splits > 1) {
             const int64_t n = (int64_t)d.rows_q * d.heads * d.dim;
             hipLaunchKernelGGL(att_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, n, d.splits, part, (T*)dq,
@@ -1009,7 +1050,7 @@ size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backwa
     return backward ? p.bwd : p.fwd;
 }
 
-int tsd_graph_attention_fwd(const tsd_attention* a, void* out, float* lse, float* scratch, size_t scratch_floats, void* stream) {
+int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats, void* stream) {
     const int rc = att_check("tsd_graph_attention_fwd", a);
     if (rc != TSD_OK) return rc;
     if (a->num_queries == 0) return TSD_OK;
@@ -1020,14 +1061,14 @@ int tsd_graph_attention_fwd(const tsd_attention* a, void* out, float* lse, float
     const AttDims d = att_dims(*a);
     hipStream_t st = (hipStream_t)stream;
     TSD_BY_DTYPE(a->dtype, T, {
-        if (d.dim <= 32) return att_fwd<T, 32>(d, *a, out, lse, scratch, st);
-        if (d.dim <= 64) return att_fwd<T, 64>(d, *a, out, lse, scratch, st);
-        return att_fwd<T, 128>(d, *a, out, lse, scratch, st);
+        if (d.dim <= 32) return att_fwd<T, 32>(d, *a, out, out_rest, lse, scratch, st);
+        if (d.dim <= 64) return att_fwd<T, 64>(d, *a, out, out_rest, lse, scratch, st);
+        return att_fwd<T, 128>(d, *a, out, out_rest, lse, scratch, st);
     });
     return TSD_OK;
 }
 
-int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float* lse, const void* dout, int64_t do_row,
+int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const void* out_rest, const float* lse, const void* dout, int64_t do_row,
                             int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream) {
     const int rc = att_check("tsd_graph_attention_bwd", a);
     if (rc != TSD_OK) return rc;
@@ -1040,9 +1081,9 @@ int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const float
     const AttDims d = att_dims(*a);
     hipStream_t st = (hipStream_t)stream;
     TSD_BY_DTYPE(a->dtype, T, {
-        if (d.dim <= 32) return att_bwd<T, 32>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
-        if (d.dim <= 64) return att_bwd<T, 64>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
-        return att_bwd<T, 128>(d, *a, out, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        if (d.dim <= 32) return att_bwd<T, 32>(d, *a, out, out_rest, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        if (d.dim <= 64) return att_bwd<T, 64>(d, *a, out, out_rest, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
+        return att_bwd<T, 128>(d, *a, out, out_rest, dout, do_row, do_head, lse, dq, dk, dv, scratch, st);
     });
     return TSD_OK;
 }

@@ -6,7 +6,9 @@
 // Forward: one launch; a workgroup multiplies a tile of rows with the same columns of both weights, so a lane holds g and u
 // of one place and the product leaves the kernel as h.  Backward: launch 1 computes g and u again (they are not kept: at 256
 // inputs reading them back in f32 costs more than the products) and writes D = [dg | du] in the tensors' type -- the one
-// rounding of an intermediate, since D is the next two products' matrix operand -- with each row tile's column sums in fp32;
+// rounding of an intermediate, since D is the next two products' matrix operand; a small D (at most 2^18 values of 16 bits) is
+// written with what the rounding left as a second half of twice the width, which the products go over too, since sums of few
+// terms show one rounding more than large ones, and time is no matter there -- with each row tile's column sums in fp32;
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
 #include <type_traits>
 
@@ -35,6 +37,7 @@ template <int KIND> __device__ __forceinline__ float act_slope(int kind, float g
 
 struct GatedDims {
     int rows, in, out, outp;  // outp: out rounded up to 8, the width of each half of D
+    int planes;               // of D: 1, or 2 with what the rounding left
     int inw;                  // values a row of x and the weights as the products read them: in, or in rounded up to 8 (packed)
     int64_t ldx, lddh, ldw;
     int kind;
@@ -95,8 +98,9 @@ template <class T, int BM, int BN, bool FAST> constexpr int gated_lds(int behind
     const int g = (BM + BN) * 64 * Elem<T>::P * (FAST && sizeof(T) == 2 ? GATED_STAGES : gated_bufs<T, BM>());
     return g > behind ? g : behind;
 }
+template <class T, int BM> constexpr bool gated_rest() { return sizeof(T) == 2 && BM == 32; }  // instances that can write it
 template <class T, int BM, int BN> constexpr int gated_behind(bool bwd) {
-    return (bwd ? 2 : 1) * OutTile<T, BM, BN / 2>::BYTES + (bwd ? 4 * (BN / 2) * 4 : 0);
+    return (bwd ? gated_rest<T, BM>() ? 4 : 2 : 1) * OutTile<T, BM, BN / 2>::BYTES + (bwd ? 4 * (BN / 2) * 4 : 0);
 }
 
 template <class T, int BM, int BN, bool FAST, bool BWD>
@@ -130,7 +134,8 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.inw, mrow,
                                [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     char* second = lds + Out::BYTES;
-    float* red = reinterpret_cast<float*>(lds + 2 * Out::BYTES);  // [2 (wm)][2][FT] column sums
+    constexpr bool REST = BWD && gated_rest<T, BM>();
+    float* red = reinterpret_cast<float*>(lds + (REST ? 4 : 2) * Out::BYTES);  // [2 (wm)][2][FT] column sums
     if constexpr (BWD) {
         Out::keep(dhr, lds);
         __syncthreads();
@@ -165,6 +170,16 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
                         }
                     store4(o, og, 4, true);
                     store4(Out::at(second, ml, fl), ou, 4, true);
+                    if constexpr (REST) {
+                        f32x4 rg, ru;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            rg[e] = og[e] - to_f((T)og[e]);
+                            ru[e] = ou[e] - to_f((T)ou[e]);
+                        }
+                        store4(Out::at(second + Out::BYTES, ml, fl), rg, 4, true);
+                        store4(Out::at(second + 2 * Out::BYTES, ml, fl), ru, 4, true);
+                    }
                     sg += og;
                     su += ou;
                 }
@@ -191,9 +206,14 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
     if constexpr (!BWD) {
         Out::write(lds, h + (int64_t)m0 * d.out + f0, d.out, d.rows - m0, d.out - f0, d.hvw);
     } else {
-        T* o = D + (int64_t)m0 * 2 * d.outp + f0;
-        Out::write(lds, o, 2 * d.outp, d.rows - m0, d.outp - f0, 8);
-        Out::write(second, o + d.outp, 2 * d.outp, d.rows - m0, d.outp - f0, 8);
+        const int64_t ldd = (int64_t)d.planes * 2 * d.outp;
+        T* o = D + m0 * ldd + f0;
+        Out::write(lds, o, ldd, d.rows - m0, d.outp - f0, 8);
+        Out::write(second, o + d.outp, ldd, d.rows - m0, d.outp - f0, 8);
+        if (REST && d.planes == 2) {
+            Out::write(second + Out::BYTES, o + 2 * d.outp, ldd, d.rows - m0, d.outp - f0, 8);
+            Out::write(second + 2 * Out::BYTES, o + 3 * d.outp, ldd, d.rows - m0, d.outp - f0, 8);
+        }
         if (part == nullptr) return;
         for (int t = threadIdx.x; t < 2 * FT; t += GEMM_WG) {
             const int f = f0 + t % FT;
@@ -214,10 +234,11 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktil
     const int m0 = at.lo * BM, k0 = at.sh * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
-    const ColOperand<T> ns = {wg, wu, d.ldw, d.inw, d.out, k0, d.outp, d.wvw};
-    const RowOperand<T> ms = {D, D, 2 * d.outp, d.rows, 2 * d.outp, m0, BM, 0, 8};
+    const int width = d.planes * 2 * d.outp;  // of D
+    const ColOperand<T> ns = {wg, wu, d.ldw, d.inw, d.out, k0, d.outp, 2 * d.outp, d.wvw};
+    const RowOperand<T> ms = {D, D, width, d.rows, width, m0, BM, 0, 8};
     f32x4 acc[BN / 32][BM / 32];
-    const int fb = blockIdx.y * share, fe = fb + share < 2 * d.outp ? fb + share : 2 * d.outp;
+    const int fb = blockIdx.y * share, fe = fb + share < width ? fb + share : width;
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     if (gridDim.y > 1) {
@@ -249,10 +270,14 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
     const int64_t rb = (int64_t)blockIdx.y * rows_a_split;
     const int n = (int)(d.rows - rb < rows_a_split ? d.rows - rb : rows_a_split);
-    const ColOperand<T> ns = {x + rb * d.ldx, x, d.ldx, d.inw, n, k0, 1 << 30, d.xvw};
-    const ColOperand<T> ms = {D + rb * 2 * d.outp, D, 2 * d.outp, 2 * d.outp, n, f0, 1 << 30, 8};
+    // the rows of both halves of D, one behind the other, and x's rows twice
+    const int width = d.planes * 2 * d.outp, half = d.planes == 2 ? (n + 7) / 8 * 8 : 1 << 30;
+    const T *xb = x + rb * d.ldx, *db = D + rb * width;
+    const ColOperand<T> ns = {xb, xb, d.ldx, d.inw, n, k0, half, 1 << 30, d.xvw};
+    const ColOperand<T> ms = {db, db + 2 * d.outp, width, 2 * d.outp, n, f0, half, 1 << 30, 8};
     f32x4 acc[BN / 32][BM / 32];
-    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, n, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.planes == 2 ? half + n : n, mrow, [&](int j) { return nbase + j * 16; },
+                                acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + (int64_t)blockIdx.y * 2 * d.outp * d.in;
 #pragma unroll
@@ -353,6 +378,7 @@ struct GatedScratch {  // bytes from the start
     int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
     int wtile, splits, rows_a_split;   // of dW
     int xtile, xsplits, share;         // of dx
+    int planes;                        // of D
 };
 // Rows that no 16-byte load fits are copied to rows that it does where the products are long enough to pay for the launch;
 // below, their tiles come in by narrower, guarded loads (2 rows of 19 -> 177 f32 values, forward: 6 us against 9; 2066 of
@@ -365,6 +391,8 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
     const bool guarded = !fast && !gated_packed(rows, in, out);
     s.tile = gated_tile(rows, 2 * outp, 1, guarded);
     s.mtiles = div_up(rows, TILE_M[s.tile]);
+    s.planes = es == 2 && s.tile >= TILE_32 && (int64_t)rows * 2 * outp <= (1 << 18) ? 2 : 1;
+    const size_t width = s.planes * 2 * outp;
     // dW: the rows in shares of at least 256, about two workgroups a CU
     const int most = div_up(rows, 256);
     s.wtile = gated_tile(2 * outp, in, most, guarded);
@@ -376,14 +404,14 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
     s.rows_a_split = div_up(div_up(rows > 0 ? rows : 1, n), GEMM_K) * GEMM_K;
     s.splits = div_up(rows, s.rows_a_split);
     // dx: the largest tiles that fill the chip with shares of at least eight steps of the contraction
-    const int steps = div_up(2 * outp, GEMM_K);
+    const int steps = div_up(width, GEMM_K);
     for (s.xtile = guarded ? TILE_GUARDED : TILE_128;; ++s.xtile) {
         const int t = div_up(rows, TILE_M[s.xtile]) * div_up(in, TILE_N[s.xtile]);
         int x = div_up(512, t > 0 ? t : 1);
         x = x < steps / 8 ? x : steps / 8;
         x = x < 1 ? 1 : x;
         s.share = div_up(steps, x) * GEMM_K;
-        s.xsplits = div_up(2 * outp, s.share);
+        s.xsplits = div_up(width, s.share);
         if (s.xtile >= TILE_32 || (int64_t)t * s.xsplits >= 256) break;
     }
     s.pack = 0;
@@ -392,7 +420,7 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
         s.total = s.D;
         return s;
     }
-    s.bpart = s.D + up((size_t)rows * 2 * outp * es);
+    s.bpart = s.D + up((size_t)rows * width * es);
     s.wpart = s.bpart + up((size_t)s.mtiles * 2 * outp * 4);
     s.xpart = s.wpart + up((size_t)s.splits * 2 * outp * in * 4);
     s.total = s.xpart + (s.xsplits > 1 ? up((size_t)s.xsplits * rows * in * 4) : 0);
@@ -422,6 +450,7 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
     d.out = out;
     d.outp = (out + 7) / 8 * 8;
     d.ldx = ldx;
+    d.planes = 1;
     d.inw = in;
     d.ldw = in;
     d.kind = act;
@@ -509,6 +538,7 @@ static int gated_bwd(GatedDims d, const void* x, const void* wg, const void* wu,
     float* xpart = reinterpret_cast<float*>(scratch + s.xpart);
     const bool sums = dbg != nullptr || dbu != nullptr, weights = dwg != nullptr || dwu != nullptr;
     int rc = TSD_OK;
+    d.planes = s.planes;
     if (d.rows > 0) {
         d.lddh = lddh;
         d.dhvw = load_width(sizeof(T), d.out, lddh, dh);
