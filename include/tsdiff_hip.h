@@ -655,9 +655,9 @@ typedef struct tsd_attention {
     const uint8_t* key_mask;         /* [num_keys] or NULL */
 } tsd_attention;
 size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backward);
-/* out [num_queries, heads, dim] dense.  For the backward: lse [num_queries, heads], log2 of the sum of 2^(score log2 e), and for
- * bf16 / f16 out_rest, what the rounding of `out` left (same type and shape: sum dO O, which the gradients of the scores are
- * taken from, needs more digits than `out` has).  Either NULL: not kept.  scratch (16-byte aligned) may be NULL where the query
+/* out [num_queries, heads, dim] dense.  For the backward: lse [num_queries, heads], log2 of the sum of 2^(score log2 e) (+inf
+ * where there is no open key), and for bf16 / f16 out_rest, what the rounding of `out` left (same type and shape: sum dO O,
+ * which the gradients of the scores are taken from, needs more digits than `out` has).  Either NULL: not kept.  scratch (16-byte aligned) may be NULL where the query
  * function says 0 floats. */
 int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats,
                             void* stream);

@@ -228,6 +228,11 @@ def test_attention_with_queries_of_their_own(qs, ks, heads, kv_heads, dim, dtype
     attention_run(*attention_case(qs, ks, heads, kv_heads, dim, dtype, len(qs) > 1))
 
 
+@pytest.mark.parametrize("dtype,dim,masked", [(torch.float32, 8, False), (torch.float16, 72, False), (torch.float16, 72, True)])
+def test_attention_over_more_keys_than_one_list_of_tiles_holds(dtype, dim, masked):
+    attention_run(*attention_case([4, 512], [30, 4200], 64, 64, dim, dtype, masked))
+
+
 @pytest.mark.parametrize("graphs", [1, 62, 63, 64, 65, 200, 4100])
 def test_attention_finds_the_graph_of_every_tile(graphs):
     sizes = [(7 * i) % 5 for i in range(graphs)]

@@ -225,8 +225,9 @@ template <class T, int ROWS_, int C_> struct Tile {
 
 // ---------------------------------------------------------------------------------------------
 // Loads from memory to LDS that pass no register (16-bit types): lane l of a wave writes 16 bytes at the wave's base +
-// 16 l (m0 holds the base: nothing else in these kernels uses it); an offset past the buffer's end (NOWHERE) writes zeros.  The compiler does not see them: dma_wait<N> waits until
-// at most the N youngest loads of the wave are under way, behind it stands a barrier.
+// 16 l (m0 holds the base: nothing else in these kernels uses it); an offset past the buffer's end (NOWHERE) writes zeros.
+// The compiler does not see them: dma_wait<N> waits until at most the N youngest loads of the wave are under way, behind it
+// stands a barrier.
 // ---------------------------------------------------------------------------------------------
 using i32x4 = int __attribute__((ext_vector_type(4)));
 constexpr uint32_t DMA_NOWHERE = 0x80000000u;

@@ -1,12 +1,14 @@
 // kernels_attention.hip -- attention inside the graphs of a ragged batch, forward and backward.
 //
 //   S = scale Q K^T over the open keys of the row's graph, P = softmax S, O = P V, L = log2 sum exp2(S log2 e)
+//   (L = +inf for a row without keys: every 2^(S - L) of it is 0)
 //   delta = sum_d dO O;  dP = dO V^T;  dS = P (dP - delta);  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
 //
 // One pass over the keys: the running maximum and sum of each row stay in registers and the scores never leave them.  The
 // scores are computed turned, S^T = K Q^T, so that a lane holds one row's scores (their statistics are a lane's own, two
-// shuffles join the four lanes of a row) AND the result registers are the operand of the next product as they stand: the
-// contraction's order is free, so the keys of V are laid out in LDS in the order in which S^T leaves the matrix pipes.
+// swaps join the four lanes of a row) AND the result registers are the operand of the next product as they stand: the rows
+// of a tile are taken in the order (sub_row) in which a lane's eight scores are eight consecutive keys.  Every tile lies in
+// LDS as it lies in memory, for both products: S reads it along its rows, P V and dS K by the LDS's transposing read.
 // The backward computes the scores again from L: one launch over row tiles for dQ (and delta), one over key tiles for dK and
 // dV; every gradient is summed by one workgroup in a fixed order, without atomics.
 //
@@ -52,7 +54,7 @@ __device__ __forceinline__ Span find_span(const AttDims& d, bool by_key, int T, 
     const int32_t* ptr = by_key ? d.k_ptr : d.q_ptr;
     const int32_t* other = by_key ? d.q_ptr : d.k_ptr;
     const int n = by_key ? d.rows_k : d.rows_q, on = by_key ? d.rows_q : d.rows_k, lane = threadIdx.x & 63, all = d.graphs + 2;
-    // (32 bits: at most 2^30 rows and 2^22 graphs)
+    // (32 bits: at most 2^29 rows and 2^22 graphs)
     auto slot = [&](int b, int v) { return (int)(((uint32_t)b * (uint32_t)times + (uint32_t)v * (uint32_t)(T - 1)) / (uint32_t)T); };
     int lo = (int)((float)s * d.graph_of_slot) - 32;
     lo = lo > all - 64 ? all - 64 : lo;
@@ -123,7 +125,7 @@ template <class T> struct Rows {
 };
 // Which keys are open, a word a tile, MASK_TILES tiles at a time in LDS: looked up tile by tile, the mask's bytes would be
 // waited for in front of every tile's loads.
-constexpr int MASK_TILES = 256, MASK_BYTES = MASK_TILES * 8;
+constexpr int MASK_TILES = 128, MASK_BYTES = MASK_TILES * 8;
 template <int WAVES, int KT, class T>
 __device__ __forceinline__ void mask_words(const Rows<T>& s, int tb, int te, uint64_t* words) {
     if (s.mask == nullptr) return;
@@ -185,6 +187,15 @@ template <class T, int ROWS, int DP, int NT, bool FAST> struct RowStage {
     }
 };
 
+template <class T, int N> __device__ __forceinline__ void in_registers(const Chunk<T> (&f)[N]) {
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int p = 0; p < Elem<T>::P; ++p) {
+            const u32x4 v = __builtin_bit_cast(u32x4, f[b].p[p]);
+            asm volatile("" : : "v"(v));
+        }
+}
 // one row's operand, kept in registers: chunk (lane / 16) of each 32 values
 template <class T> __device__ __forceinline__ void row_raw(Raw<T>& raw, const Rows<T>& s, int r, bool has, int b) {
     const int d0 = b * 32 + ((threadIdx.x & 63) >> 4) * 8, n = has ? s.dim - d0 : 0;
@@ -279,14 +290,16 @@ __device__ __forceinline__ void split_range(int n, int tile, int splits, int z, 
 // The tiles b .. e - 1 of one pair of row sets, one after the other in LDS: load(i, open, buffer) starts tile i's loads,
 // step(i, open, buffer) is its work.  DMA: three buffers, two tiles under way; registers: one buffer (the planes of f32 take
 // three times the room, and workgroups on a CU are worth more than the barrier saved), one tile under way.
-// LOADS: the loads of a wave a tile.
-template <int LOADS, bool DMA, class Open, class Load, class Store, class Step>
-__device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, Store store, Step step) {
+// LOADS: the loads of a wave a tile.  ready() uses what was loaded to registers in front of the loop: the compiler would
+// otherwise wait for it inside, and with it, every time, for the tiles under way.
+template <int LOADS, bool DMA, class Open, class Load, class Store, class Ready, class Step>
+__device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, Store store, Ready ready, Step step) {
     if (b >= e) return;
     if constexpr (DMA) {
         uint64_t m0 = open(b), m1 = b + 1 < e ? open(b + 1) : 0;
         load(b, m0, 0);
         if (b + 1 < e) load(b + 1, m1, 1);
+        ready();
         int buf = 0;
         for (int i = b; i < e; ++i) {
             const uint64_t m2 = i + 2 < e ? open(i + 2) : 0;
@@ -316,14 +329,14 @@ __device__ __forceinline__ void over_tiles(int b, int e, Open open, Load load, S
 template <class T, bool FAST> constexpr int att_buffers() { return att_dma<T, FAST>() ? 3 : 1; }
 
 // ---------------------------------------------------------------------------------------------
-// forward: WAVES waves of RS x 16 rows each share the key tiles
+// forward: WAVES waves of 16 rows each share the key tiles
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
+template <class T, int DP, int WAVES, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, T* __restrict__ out,
                                                              T* __restrict__ rest, float* __restrict__ lse,
                                                              float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
+    constexpr int NT = WAVES * 64, TR = WAVES * 16;
     using Stage = RowStage<T, KT, DP, NT, FAST>;
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
@@ -334,121 +347,109 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
     if (r0 >= nrows) return;
     const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
     for (int hk = h0; hk < h1; ++hk) {
-    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int row0 = r0 + wave * RS * 16 + c;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, (const uint8_t*)nullptr, d.qvw);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
-    Chunk<T> qf[RS][DP / 32];
-    f32x4 o[RS][DP / 16];
-    float m[RS], l[RS];
+        if (hk > h0) lds_barrier();  // the tiles of the last head have been read
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+        const int row = r0 + wave * 16 + c;
+        const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, (const uint8_t*)nullptr, d.qvw);
+        const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
+        const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
+        Chunk<T> qf[DP / 32];
+        f32x4 o[DP / 16];
+        row_chunks<T, DP>(qf, qr, row);
 #pragma unroll
-    for (int x = 0; x < RS; ++x) {
-        row_chunks<T, DP>(qf[x], qr, row0 + x * 16);
+        for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.f;
+        Stage ks, vs;
+        const uint32_t at_lds = lds_offset(lds);
+        int first, last;
+        split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
+        uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
+        for (int tb = first; tb < last; tb += MASK_TILES) {
+            const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
+            if (tb > first) lds_barrier();  // the last tiles have been read
+            mask_words<WAVES, KT>(kr, tb, te, words);
+            over_tiles<2 * Stage::U, Stage::DMA>(
+                tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
+                [&](int i, uint64_t open, int buf) {
+                    ks.load(kr, i * KT, open, at_lds + buf * BUF);
+                    vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
+                },
+                [&](int buf) {
+                    ks.store(lds + buf * BUF);
+                    vs.store(lds + buf * BUF + KTile::BYTES);
+                },
+                [&]() { in_registers<T>(qf); },
+                [&](int, uint64_t open, int buf) {
+                    if (open == 0) return;  // nothing to attend to
+                    const char* kl = lds + buf * BUF;
+                    const char* vl = kl + KTile::BYTES;
+                    f32x4 s[KT / 16];
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) o[x][t] = f32x4{0, 0, 0, 0};
-        m[x] = -INFINITY;
-        l[x] = 0.f;
-    }
-    Stage ks, vs;
-    const uint32_t at_lds = lds_offset(lds);
-    int first, last;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
-    uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
-    for (int tb = first; tb < last; tb += MASK_TILES) {
-    const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
-    mask_words<WAVES, KT>(kr, tb, te, words);
-    over_tiles<2 * Stage::U, Stage::DMA>(
-        tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
-        [&](int i, uint64_t open, int buf) {
-            ks.load(kr, i * KT, open, at_lds + buf * BUF);
-            vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
-        },
-        [&](int buf) {
-            ks.store(lds + buf * BUF);
-            vs.store(lds + buf * BUF + KTile::BYTES);
-        },
-        [&](int, uint64_t open, int buf) {
-            if (open == 0) return;  // nothing to attend to
-            const char* kl = lds + buf * BUF;
-            const char* vl = kl + KTile::BYTES;
-            f32x4 s[RS][KT / 16];
+                    for (int t = 0; t < KT / 16; ++t) {
+                        s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int t = 0; t < KT / 16; ++t) {
-#pragma unroll
-                for (int x = 0; x < RS; ++x) s[x][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < DP / 32; ++b) {
-                    const Chunk<T> kf = KTile::get(kl, sub_row(t), b * 4 + g);
-#pragma unroll
-                    for (int x = 0; x < RS; ++x) s[x][t] = mma(kf, qf[x][b], s[x][t]);
-                }
-            }
-            const bool whole = KT == 64 ? open == ~0ull : (uint32_t)open == 0xffffffffu;
-            if (!whole) {
-#pragma unroll
-                for (int t = 0; t < KT / 16; ++t) {
-                    const uint32_t bits = (uint32_t)(open >> (32 * (t >> 1) + 8 * g + 4 * (t & 1)));
-#pragma unroll
-                    for (int x = 0; x < RS; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[x][t][e] = bits >> e & 1 ? s[x][t][e] * d.scale2 : -INFINITY;
-                }
-            }
-            const float sc = whole ? d.scale2 : 1.f;  // the scores' unit: a whole tile's are still to be scaled
-#pragma unroll
-            for (int x = 0; x < RS; ++x) {
-                float hi = -INFINITY;
-                if (sc >= 0.f) {
-#pragma unroll
-                    for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, s[x][t][e]);
-                } else {
-#pragma unroll
-                    for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, -s[x][t][e]);
-                }
-                hi *= fabsf(sc);
-                // The weights are taken from a maximum that may lag behind by a factor of 2^LAG, which neither they nor their
-                // sum notice: most tiles then need no look at the other lanes and no scaling of what is summed up.
-                if (__any(hi > m[x] + LAG)) {
-                    const float top = fmaxf(m[x], over_groups_max(hi)), a = exp2_fast(m[x] - (top == -INFINITY ? 0.f : top));
-                    m[x] = top;
-                    l[x] *= a;
-#pragma unroll
-                    for (int t = 0; t < DP / 16; ++t) o[x][t] *= a;
-                }
-                const float safe = m[x] == -INFINITY ? 0.f : m[x];
-#pragma unroll
-                for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[x][t][e] = exp2_fast(__builtin_fmaf(s[x][t][e], sc, -safe));
-                        l[x] += s[x][t][e];
+                        for (int b = 0; b < DP / 32; ++b) {
+                            const Chunk<T> kf = KTile::get(kl, sub_row(t), b * 4 + g);
+                            s[t] = mma(kf, qf[b], s[t]);
+                        }
                     }
-            }
+                    if (KT == 64 ? open != ~0ull : (uint32_t)open != 0xffffffffu) {
+                        // a closed key's score is as low as it gets: a sign-extended bit picks it (the scale may be negative)
+                        const uint32_t closed = d.scale2 < 0.f ? 0x7f800000u : 0xff800000u;
 #pragma unroll
-            for (int b = 0; b < KT / 32; ++b) {
-                Weights<T, att_rest<T, WAVES>()> p[RS];
+                        for (int t = 0; t < KT / 16; ++t) {
+                            const int bits = (int)(uint32_t)(open >> (32 * (t >> 1) + 8 * g + 4 * (t & 1)));
 #pragma unroll
-                for (int x = 0; x < RS; ++x) p[x] = {s[x][2 * b], s[x][2 * b + 1]};
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe(bits, e, 1);
+                                const float v = s[t][e];
+                                s[t][e] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & m) | (closed & ~m));
+                            }
+                        }
+                    }
+                    const float sc = d.scale2;
+                    float hi = -INFINITY;
+                    if (sc >= 0.f) {
 #pragma unroll
-                for (int t = 0; t < DP / 16; ++t) {
-                    const Chunk<T> vf = KTile::get_across(vl, b * 32, t);
+                        for (int t = 0; t < KT / 16; ++t)
 #pragma unroll
-                    for (int x = 0; x < RS; ++x) o[x][t] = p[x].times(vf, o[x][t]);
-                }
-            }
-        });
-    }
+                            for (int e = 0; e < 4; ++e) hi = fmaxf(hi, s[t][e]);
+                    } else {
 #pragma unroll
-    for (int x = 0; x < RS; ++x) {
-        const float ls = over_groups_sum(l[x]);
-        const int row = row0 + x * 16;
+                        for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) hi = fmaxf(hi, -s[t][e]);
+                    }
+                    hi *= fabsf(sc);
+                    // The weights are taken from a maximum that may lag behind by a factor of 2^LAG, which neither they nor their
+                    // sum notice: most tiles then need no look at the other lanes and no scaling of what is summed up.
+                    if (__any(hi > m + LAG)) {
+                        const float top = fmaxf(m, over_groups_max(hi)), a = exp2_fast(m - (top == -INFINITY ? 0.f : top));
+                        m = top;
+                        l *= a;
+#pragma unroll
+                        for (int t = 0; t < DP / 16; ++t) o[t] *= a;
+                    }
+                    const float safe = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[t][e] = exp2_fast(__builtin_fmaf(s[t][e], sc, -safe));
+                            l += s[t][e];
+                        }
+#pragma unroll
+                    for (int b = 0; b < KT / 32; ++b) {
+                        const Weights<T, att_rest<T, WAVES>()> p = {s[2 * b], s[2 * b + 1]};
+#pragma unroll
+                        for (int t = 0; t < DP / 16; ++t) {
+                            const Chunk<T> vf = KTile::get_across(vl, b * 32, t);
+                            o[t] = p.times(vf, o[t]);
+                        }
+                    }
+                });
+        }
+        const float ls = over_groups_sum(l);
         if (row >= nrows) continue;
         const int qi = query_of(row, d.group);
         const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + row - qi * d.group;
@@ -456,10 +457,10 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
             const int64_t all = (int64_t)d.rows_q * d.heads, i = blockIdx.z * all + at;
             float* po = part + i * d.dim;
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) store4(po + t * 16 + g * 4, o[x][t], d.dim - t * 16 - g * 4, d.dim % 4 == 0);
+            for (int t = 0; t < DP / 16; ++t) store4(po + t * 16 + g * 4, o[t], d.dim - t * 16 - g * 4, d.dim % 4 == 0);
             if (g == 0) {
                 float* ps = part + d.splits * all * d.dim + 2 * i;
-                ps[0] = m[x];
+                ps[0] = m;
                 ps[1] = ls;
             }
             continue;
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
         const float inv = ls > 0.f ? __builtin_amdgcn_rcpf(ls) : ls == 0.f ? 0.f : ls;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
-            f32x4 v = o[x][t] * inv;
+            f32x4 v = o[t] * inv;
             store4(out + at * d.dim + t * 16 + g * 4, v, d.dim - t * 16 - g * 4, d.ovec);
             if (rest != nullptr) {
 #pragma unroll
@@ -475,8 +476,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
                 store4(rest + at * d.dim + t * 16 + g * 4, v, d.dim - t * 16 - g * 4, d.ovec);
             }
         }
-        if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? -INFINITY : m[x] + __builtin_amdgcn_logf(ls);
-    }
+        if (lse != nullptr && g == 0) lse[at] = ls == 0.f ? INFINITY : m + __builtin_amdgcn_logf(ls);
     }
 }
 
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(256) void att_join_kernel(int64_t all, int dim, int
     const float v = l == 0.f ? 0.f : o / l;
     out[i] = (T)v;
     if (rest != nullptr) rest[i] = (T)(v - to_f((T)v));
-    if (lse != nullptr && e == 0) lse[at] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+    if (lse != nullptr && e == 0) lse[at] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // out[i] = sum_z part[z][i]
@@ -522,13 +522,13 @@ __global__ __launch_bounds__(256) void att_sum_kernel(int64_t n, int splits, con
 // ---------------------------------------------------------------------------------------------
 // dQ: the forward's tiles again; delta on the way
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int RS, int KT, bool FAST>
+template <class T, int DP, int WAVES, int KT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                             const T* __restrict__ v, const T* __restrict__ out,
-                                                            const T* __restrict__ rest, const T* __restrict__ dout, const float* __restrict__ lse,
-                                                            float* __restrict__ delta, T* __restrict__ dq,
-                                                            float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TR = WAVES * RS * 16;
+                                                            const T* __restrict__ rest, const T* __restrict__ dout,
+                                                            const float* __restrict__ lse, float* __restrict__ delta,
+                                                            T* __restrict__ dq, float* __restrict__ part) {
+    constexpr int NT = WAVES * 64, TR = WAVES * 16;
     using Stage = RowStage<T, KT, DP, NT, FAST>;
     using KTile = typename Stage::Lds;
     constexpr int BUF = 2 * KTile::BYTES;
@@ -539,30 +539,27 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
     if (r0 >= nrows) return;
     const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
     for (int hk = h0; hk < h1; ++hk) {
-    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int row0 = r0 + wave * RS * 16 + c;
-    const uint8_t* no = nullptr;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
-    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
-    const Rows<T> orow = rows_of(out, (int64_t)d.heads * d.dim, d.dim, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.ovec ? 8 : 1);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
-    Chunk<T> qf[RS][DP / 32], gf[RS][DP / 32];
-    float del[RS], L[RS], safe[RS];
-    f32x4 acc[RS][DP / 16];
-#pragma unroll
-    for (int x = 0; x < RS; ++x) {
-        const int row = row0 + x * 16;
+        if (hk > h0) lds_barrier();  // the tiles of the last head have been read
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+        const int row = r0 + wave * 16 + c;
+        const uint8_t* no = nullptr;
+        const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
+        const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
+        const Rows<T> orow = rows_of(out, (int64_t)d.heads * d.dim, d.dim, sp.qs, nrows, hk * d.group, d.group, d.dim, no,
+                                     d.ovec ? 8 : 1);
+        const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.kvw);
+        const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, sp.ke - sp.ks, hk, 1, d.dim, d.mask, d.vvw);
+        Chunk<T> qf[DP / 32], gf[DP / 32];
+        f32x4 acc[DP / 16];
         const bool mine = row < nrows;
-        row_chunks<T, DP>(qf[x], qr, row);
+        row_chunks<T, DP>(qf, qr, row);
         float s = 0.f;
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) {
             Raw<T> a, o;
             row_raw(a, gr, row, mine, b);
             row_raw(o, orow, row, mine, b);
-            gf[x][b] = raw_chunk(a);
+            gf[b] = raw_chunk(a);
             s += raw_dot(a, o);
             if (rest != nullptr) {
                 Rows<T> more = orow;
@@ -571,87 +568,78 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                 s += raw_dot(a, o);
             }
         }
-        del[x] = over_groups_sum(s);
+        const float del = over_groups_sum(s);
         const int qi = mine ? query_of(row, d.group) : 0;
         const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + (mine ? row - qi * d.group : 0);
-        L[x] = mine ? lse[at] : INFINITY;
-        safe[x] = L[x] == -INFINITY ? INFINITY : L[x];  // no open key: every weight is 0
-        if (mine && g == 0 && blockIdx.z == 0) delta[at] = del[x];
+        const float L = mine ? lse[at] : INFINITY;
+        if (mine && g == 0 && blockIdx.z == 0) delta[at] = del;
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) acc[x][t] = f32x4{0, 0, 0, 0};
-    }
-    Stage ks, vs;
-    const uint32_t at_lds = lds_offset(lds);
-    int first, last;
-    split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
-    uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
-    for (int tb = first; tb < last; tb += MASK_TILES) {
-    const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
-    mask_words<WAVES, KT>(kr, tb, te, words);
-    over_tiles<2 * Stage::U, Stage::DMA>(
-        tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
-        [&](int i, uint64_t open, int buf) {
-            ks.load(kr, i * KT, open, at_lds + buf * BUF);
-            vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
-        },
-        [&](int buf) {
-            ks.store(lds + buf * BUF);
-            vs.store(lds + buf * BUF + KTile::BYTES);
-        },
-        [&](int, uint64_t open, int buf) {
-            if (open == 0) return;  // nothing to attend to
-            const char* kl = lds + buf * BUF;
-            const char* vl = kl + KTile::BYTES;
+        for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
+        Stage ks, vs;
+        const uint32_t at_lds = lds_offset(lds);
+        int first, last;
+        split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
+        uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
+        for (int tb = first; tb < last; tb += MASK_TILES) {
+            const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
+            if (tb > first) lds_barrier();  // the last tiles have been read
+            mask_words<WAVES, KT>(kr, tb, te, words);
+            over_tiles<2 * Stage::U, Stage::DMA>(
+                tb, te, [&](int i) { return mask_word<KT>(kr, i, tb, words); },
+                [&](int i, uint64_t open, int buf) {
+                    ks.load(kr, i * KT, open, at_lds + buf * BUF);
+                    vs.load(vr, i * KT, open, at_lds + buf * BUF + KTile::BYTES);
+                },
+                [&](int buf) {
+                    ks.store(lds + buf * BUF);
+                    vs.store(lds + buf * BUF + KTile::BYTES);
+                },
+                [&]() {
+                    in_registers<T>(qf);
+                    in_registers<T>(gf);
+                    asm volatile("" : : "v"(L));
+                },
+                [&](int, uint64_t open, int buf) {
+                    if (open == 0) return;  // nothing to attend to
+                    const char* kl = lds + buf * BUF;
+                    const char* vl = kl + KTile::BYTES;
 #pragma unroll
-            for (int p = 0; p < KT / 32; ++p) {
-                f32x4 s[RS][2], dp[RS][2];
+                    for (int p = 0; p < KT / 32; ++p) {
+                        f32x4 s[2], dp[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                        for (int u = 0; u < 2; ++u) {
+                            s[u] = dp[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int x = 0; x < RS; ++x) s[x][u] = dp[x][u] = f32x4{0, 0, 0, 0};
+                            for (int b = 0; b < DP / 32; ++b) {
+                                const Chunk<T> kf = KTile::get(kl, sub_row(2 * p + u), b * 4 + g);
+                                const Chunk<T> vf = KTile::get(vl, sub_row(2 * p + u), b * 4 + g);
+                                s[u] = mma(kf, qf[b], s[u]);
+                                dp[u] = mma(vf, gf[b], dp[u]);
+                            }
+                        }
+                        const int bits = (int)(uint32_t)(open >> (32 * p + 8 * g));
 #pragma unroll
-                    for (int b = 0; b < DP / 32; ++b) {
-                        const Chunk<T> kf = KTile::get(kl, sub_row(2 * p + u), b * 4 + g);
-                        const Chunk<T> vf = KTile::get(vl, sub_row(2 * p + u), b * 4 + g);
+                        for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int x = 0; x < RS; ++x) {
-                            s[x][u] = mma(kf, qf[x][b], s[x][u]);
-                            dp[x][u] = mma(vf, gf[x][b], dp[x][u]);
+                            for (int e = 0; e < 4; ++e) {
+                                const float w = exp2_fast(__builtin_fmaf(s[u][e], d.scale2, -L)) * (dp[u][e] - del);
+                                s[u][e] = __builtin_bit_cast(
+                                    float, __builtin_bit_cast(uint32_t, w) & (uint32_t)__builtin_amdgcn_sbfe(bits, 4 * u + e, 1));
+                            }
+                        const Weights<T, att_rest<T, WAVES>()> f = {s[0], s[1]};
+#pragma unroll
+                        for (int t = 0; t < DP / 16; ++t) {
+                            const Chunk<T> kc = KTile::get_across(kl, p * 32, t);
+                            acc[t] = f.times(kc, acc[t]);
                         }
                     }
-                }
-                const uint32_t bits = (uint32_t)(open >> (32 * p + 8 * g));
-                Weights<T, att_rest<T, WAVES>()> f[RS];
-#pragma unroll
-                for (int x = 0; x < RS; ++x) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float w = exp2_fast(__builtin_fmaf(s[x][u][e], d.scale2, -safe[x])) * (dp[x][u][e] - del[x]);
-                            s[x][u][e] = bits >> (4 * u + e) & 1 ? w : 0.f;
-                        }
-                    f[x] = {s[x][0], s[x][1]};
-                }
-#pragma unroll
-                for (int t = 0; t < DP / 16; ++t) {
-                    const Chunk<T> kc = KTile::get_across(kl, p * 32, t);
-#pragma unroll
-                    for (int x = 0; x < RS; ++x) acc[x][t] = f[x].times(kc, acc[x][t]);
-                }
-            }
-        });
-    }
-#pragma unroll
-    for (int x = 0; x < RS; ++x) {
-        const int row = row0 + x * 16;
-        if (row >= nrows) continue;
-        const int qi = query_of(row, d.group);
-        const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + row - qi * d.group;
+                });
+        }
+        if (!mine) continue;
         // a row without an open key has dQ = 0 whatever dO and O hold
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
-            const f32x4 r = L[x] == -INFINITY ? f32x4{0, 0, 0, 0} : acc[x][t] * d.scale;
+            const f32x4 r = L == INFINITY ? f32x4{0, 0, 0, 0} : acc[t] * d.scale;
             const int n = d.dim - t * 16 - g * 4;
             if (d.splits > 1)
                 store4(part + (blockIdx.z * (int64_t)d.rows_q * d.heads + at) * d.dim + t * 16 + g * 4, r, n, d.dim % 4 == 0);
@@ -659,18 +647,17 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                 store4(dq + at * d.dim + t * 16 + g * 4, r, n, d.ovec);
         }
     }
-    }
 }
 
 // ---------------------------------------------------------------------------------------------
-// dK, dV: WAVES waves of KS x 16 keys each; all rows (of all heads that read the keys) go by in tiles of RT
+// dK, dV: WAVES waves of 16 keys each; all rows (of all heads that read the keys) go by in tiles of RT
 // ---------------------------------------------------------------------------------------------
-template <class T, int DP, int WAVES, int KS, int RT, bool FAST>
+template <class T, int DP, int WAVES, int RT, bool FAST>
 __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const T* __restrict__ dout,
                                                              const float* __restrict__ lse, const float* __restrict__ delta,
                                                              T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
-    constexpr int NT = WAVES * 64, TK = WAVES * KS * 16;
+    constexpr int NT = WAVES * 64, TK = WAVES * 16;
     using Stage = RowStage<T, RT, DP, NT, FAST>;
     using RTile = typename Stage::Lds;
     constexpr int STAT = 2 * RTile::BYTES, BUF = STAT + 2 * 64 * 4;  // Q, dO, then 64 values of L and of delta each
@@ -682,129 +669,113 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
     if (k0 >= nkeys) return;
     const int h0 = blockIdx.x % hgroups * d.heads_a_wg, h1 = h0 + d.heads_a_wg < d.kv_heads ? h0 + d.heads_a_wg : d.kv_heads;
     for (int hk = h0; hk < h1; ++hk) {
-    if (hk > h0) lds_barrier();  // the tiles of the last head have been read
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int key0 = k0 + wave * KS * 16 + c;
-    const uint8_t* no = nullptr;
-    const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
-    const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
-    const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.kvw);
-    const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.vvw);
-    // row r's statistics lie at (qs + r / group) heads + hk group + r % group
-    const int64_t stat0 = (int64_t)sp.qs * d.heads + hk * d.group;
-    auto stat_at = [&](int r) {
-        const int qi = query_of(r, d.group);
-        return (int64_t)qi * d.heads + r - qi * d.group;
-    };
-    Chunk<T> kf[KS][DP / 32], vf[KS][DP / 32];
-    bool open_key[KS];
-    f32x4 ak[KS][DP / 16], av[KS][DP / 16];
+        if (hk > h0) lds_barrier();  // the tiles of the last head have been read
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+        const int key = k0 + wave * 16 + c;
+        const uint8_t* no = nullptr;
+        const Rows<T> qr = rows_of(q, d.q_row, d.q_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.qvw);
+        const Rows<T> gr = rows_of(dout, d.do_row, d.do_head, sp.qs, nrows, hk * d.group, d.group, d.dim, no, d.dovw);
+        const Rows<T> kr = rows_of(k, d.k_row, d.k_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.kvw);
+        const Rows<T> vr = rows_of(v, d.v_row, d.v_head, sp.ks, nkeys, hk, 1, d.dim, d.mask, d.vvw);
+        // row r's statistics lie at (qs + r / group) heads + hk group + r % group
+        const int64_t stat0 = (int64_t)sp.qs * d.heads + hk * d.group;
+        auto stat_at = [&](int r) {
+            const int qi = query_of(r, d.group);
+            return (int64_t)qi * d.heads + r - qi * d.group;
+        };
+        Chunk<T> kf[DP / 32], vf[DP / 32];
+        f32x4 ak[DP / 16], av[DP / 16];
+        row_chunks<T, DP>(kf, kr, key);
+        row_chunks<T, DP>(vf, vr, key);
+        const bool open_key = kr.has(key);
 #pragma unroll
-    for (int x = 0; x < KS; ++x) {
-        row_chunks<T, DP>(kf[x], kr, key0 + x * 16);
-        row_chunks<T, DP>(vf[x], vr, key0 + x * 16);
-        open_key[x] = kr.has(key0 + x * 16);
+        for (int t = 0; t < DP / 16; ++t) ak[t] = av[t] = f32x4{0, 0, 0, 0};
+        Stage qs, gs;
+        float stat_reg = 0.f;
+        const uint32_t at_lds = lds_offset(lds);
+        int tb, te;
+        split_range(nrows, RT, d.splits, blockIdx.z, &tb, &te);
+        uint64_t any = 0;
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) ak[x][t] = av[x][t] = f32x4{0, 0, 0, 0};
-    }
-    Stage qs, gs;
-    float stat_reg = 0.f;
-    const uint32_t at_lds = lds_offset(lds);
-    int tb, te;
-    split_range(nrows, RT, d.splits, blockIdx.z, &tb, &te);
-    uint64_t any = 0;
+        for (int i = 0; i < TK; i += 64) any |= kr.template open<(TK < 64 ? TK : 64)>(k0 + i);
+        if (any == 0) te = tb;  // nobody attends to these keys
+        over_tiles<2 * Stage::U + STATS, Stage::DMA>(
+            tb, te, [&](int i) { return qr.there(i * RT); },
+            [&](int i, uint64_t open, int buf) {
+                qs.load(qr, i * RT, open, at_lds + buf * BUF);
+                gs.load(gr, i * RT, open, at_lds + buf * BUF + RTile::BYTES);
+                // a missing row: its Q, dO, L and delta are zeros, and so is what it adds
+                if constexpr (Stage::DMA) {
+                    const int64_t first = stat_at(i * RT);
+                    const uint32_t off = (open >> lane & 1) && lane < RT ? (uint32_t)((stat_at(i * RT + lane) - first) * 4) : DMA_NOWHERE;
 #pragma unroll
-    for (int i = 0; i < TK; i += 64) any |= kr.template open<(TK < 64 ? TK : 64)>(k0 + i);
-    if (any == 0) te = tb;  // nobody attends to these keys
-    over_tiles<2 * Stage::U + STATS, Stage::DMA>(
-        tb, te, [&](int i) { return qr.there(i * RT); },
-        [&](int i, uint64_t open, int buf) {
-            qs.load(qr, i * RT, open, at_lds + buf * BUF);
-            gs.load(gr, i * RT, open, at_lds + buf * BUF + RTile::BYTES);
-            // a missing row: its Q, dO, L and delta are zeros, and so is what it adds
-            if constexpr (Stage::DMA) {
-                const int64_t first = stat_at(i * RT);
-                const uint32_t off = (open >> lane & 1) && lane < RT ? (uint32_t)((stat_at(i * RT + lane) - first) * 4) : DMA_NOWHERE;
-#pragma unroll
-                for (int w = 0; w < STATS; ++w) {
-                    const int which = STATS == 2 ? w : wave & 1;
-                    dma_load4(dma_buffer((which ? delta : lse) + stat0 + first), off, at_lds + buf * BUF + STAT + which * 256);
+                    for (int w = 0; w < STATS; ++w) {
+                        const int which = STATS == 2 ? w : wave & 1;
+                        dma_load4(dma_buffer((which ? delta : lse) + stat0 + first), off, at_lds + buf * BUF + STAT + which * 256);
+                    }
+                } else if (threadIdx.x < 2 * RT) {
+                    static_assert(NT >= 2 * RT, "a thread a value");
+                    const int r = threadIdx.x % RT;
+                    stat_reg = open >> r & 1 ? (threadIdx.x / RT ? delta : lse)[stat0 + stat_at(i * RT + r)] : 0.f;
                 }
-            } else if (threadIdx.x < 2 * RT || NT < 2 * RT) {
-                static_assert(NT >= 2 * RT, "a thread a value");
-                const int r = threadIdx.x % RT;
-                stat_reg = open >> r & 1 ? (threadIdx.x / RT ? delta : lse)[stat0 + stat_at(i * RT + r)] : 0.f;
-            }
-        },
-        [&](int buf) {
-            qs.store(lds + buf * BUF);
-            gs.store(lds + buf * BUF + RTile::BYTES);
-            if (!Stage::DMA && threadIdx.x < 2 * RT)
-                reinterpret_cast<float*>(lds + buf * BUF + STAT)[threadIdx.x / RT * 64 + threadIdx.x % RT] = stat_reg;
-        },
-        [&](int, uint64_t, int buf) {
-            const char* ql = lds + buf * BUF;
-            const char* gl = ql + RTile::BYTES;
-            const float* stat = reinterpret_cast<const float*>(ql + STAT);
+            },
+            [&](int buf) {
+                qs.store(lds + buf * BUF);
+                gs.store(lds + buf * BUF + RTile::BYTES);
+                if (!Stage::DMA && threadIdx.x < 2 * RT)
+                    reinterpret_cast<float*>(lds + buf * BUF + STAT)[threadIdx.x / RT * 64 + threadIdx.x % RT] = stat_reg;
+            },
+            [&]() {
+                in_registers<T>(kf);
+                in_registers<T>(vf);
+            },
+            [&](int, uint64_t, int buf) {
+                const char* ql = lds + buf * BUF;
+                const char* gl = ql + RTile::BYTES;
+                const float* stat = reinterpret_cast<const float*>(ql + STAT);
 #pragma unroll
-            for (int p = 0; p < RT / 32; ++p) {
-                f32x4 s[KS][2], dp[KS][2];
+                for (int p = 0; p < RT / 32; ++p) {
+                    f32x4 s[2], dp[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < 2; ++u) {
+                        s[u] = dp[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int x = 0; x < KS; ++x) s[x][u] = dp[x][u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int b = 0; b < DP / 32; ++b) {
-                        const Chunk<T> qf = RTile::get(ql, sub_row(2 * p + u), b * 4 + g);
-                        const Chunk<T> gf = RTile::get(gl, sub_row(2 * p + u), b * 4 + g);
-#pragma unroll
-                        for (int x = 0; x < KS; ++x) {
-                            s[x][u] = mma(qf, kf[x][b], s[x][u]);
-                            dp[x][u] = mma(gf, vf[x][b], dp[x][u]);
+                        for (int b = 0; b < DP / 32; ++b) {
+                            const Chunk<T> qf = RTile::get(ql, sub_row(2 * p + u), b * 4 + g);
+                            const Chunk<T> gf = RTile::get(gl, sub_row(2 * p + u), b * 4 + g);
+                            s[u] = mma(qf, kf[b], s[u]);
+                            dp[u] = mma(gf, vf[b], dp[u]);
                         }
                     }
-                }
-                Weights<T, att_rest<T, WAVES>()> pf[KS], df[KS];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const f32x4 L = *reinterpret_cast<const f32x4*>(stat + 32 * p + 8 * g + 4 * u);
-                    const f32x4 del = *reinterpret_cast<const f32x4*>(stat + 64 + 32 * p + 8 * g + 4 * u);
-#pragma unroll
-                    for (int x = 0; x < KS; ++x)
+                    for (int u = 0; u < 2; ++u) {
+                        const f32x4 L = *reinterpret_cast<const f32x4*>(stat + 32 * p + 8 * g + 4 * u);
+                        const f32x4 del = *reinterpret_cast<const f32x4*>(stat + 64 + 32 * p + 8 * g + 4 * u);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float w = exp2_fast(__builtin_fmaf(s[x][u][e], d.scale2, -L[e]));
-                            s[x][u][e] = open_key[x] ? w : 0.f;
-                            dp[x][u][e] = open_key[x] ? w * (dp[x][u][e] - del[e]) : 0.f;
+                            const float w = exp2_fast(__builtin_fmaf(s[u][e], d.scale2, -L[e]));
+                            s[u][e] = open_key ? w : 0.f;
+                            dp[u][e] = open_key ? w * (dp[u][e] - del[e]) : 0.f;
                         }
+                    }
+                    const Weights<T, att_rest<T, WAVES>()> pf = {s[0], s[1]}, df = {dp[0], dp[1]};
+#pragma unroll
+                    for (int t = 0; t < DP / 16; ++t) {
+                        const Chunk<T> gc = RTile::get_across(gl, p * 32, t);
+                        av[t] = pf.times(gc, av[t]);
+                        const Chunk<T> qc = RTile::get_across(ql, p * 32, t);
+                        ak[t] = df.times(qc, ak[t]);
+                    }
                 }
-#pragma unroll
-                for (int x = 0; x < KS; ++x) {
-                    pf[x] = {s[x][0], s[x][1]};
-                    df[x] = {dp[x][0], dp[x][1]};
-                }
-#pragma unroll
-                for (int t = 0; t < DP / 16; ++t) {
-                    const Chunk<T> gc = RTile::get_across(gl, p * 32, t);
-#pragma unroll
-                    for (int x = 0; x < KS; ++x) av[x][t] = pf[x].times(gc, av[x][t]);
-                    const Chunk<T> qc = RTile::get_across(ql, p * 32, t);
-#pragma unroll
-                    for (int x = 0; x < KS; ++x) ak[x][t] = df[x].times(qc, ak[x][t]);
-                }
-            }
-        });
-    const int64_t all = (int64_t)d.rows_k * d.kv_heads;
-#pragma unroll
-    for (int x = 0; x < KS; ++x) {
-        const int key = key0 + x * 16;
+            });
+        const int64_t all = (int64_t)d.rows_k * d.kv_heads;
         if (key >= nkeys) continue;
         const int64_t at = (int64_t)(sp.ks + key) * d.kv_heads + hk;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             const int y = t * 16 + g * 4, n = d.dim - y;
             // a masked key's gradients are 0 whatever the rows that do not read it hold
-            const f32x4 zero = {0, 0, 0, 0}, rk = open_key[x] ? ak[x][t] * d.scale : zero, rv = open_key[x] ? av[x][t] : zero;
+            const f32x4 zero = {0, 0, 0, 0}, rk = open_key ? ak[t] * d.scale : zero, rv = open_key ? av[t] : zero;
             if (d.splits > 1) {
                 store4(part + (blockIdx.z * all + at) * d.dim + y, rk, n, d.dim % 4 == 0);
                 store4(part + ((d.splits + blockIdx.z) * all + at) * d.dim + y, rv, n, d.dim % 4 == 0);
@@ -814,22 +785,20 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
             }
         }
     }
-    }
 }
 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
 // How a side (queries of all heads of a group, or keys) is cut into tiles
-enum { SIDE_16, SIDE_64, SIDE_128 };
-static const int SIDE_ROWS[3] = {16, 64, 128};
-// One wave of 16 rows where the graphs are small (its tile is filled at least as well as one of 64 rows), 32 rows a wave where
-// they are long (each tile of the other side then feeds twice the products an LDS read).  Values that no 16-byte load fits
-// have the middle instance alone; f32 has no 128 (its three planes of twice the rows do not fit the registers).
-static int att_side(int64_t rows, int graphs, bool f32, bool aligned) {
-    const int64_t each = rows / (graphs < 1 ? 1 : graphs);
-    if (!aligned) return SIDE_64;
-    return each <= 32 ? SIDE_16 : each < 256 || f32 ? SIDE_64 : SIDE_128;
+enum { SIDE_16, SIDE_64 };
+static const int SIDE_ROWS[2] = {16, 64};
+// One wave of 16 rows where the graphs are small (its tile is filled at least as well as one of 64 rows), four waves that share
+// the other side's tiles otherwise.  (32 rows a wave read a tile half as often, but two workgroups less fit a CU: 145 us
+// against 105 for the forward of 4 graphs of 1000 .. 2000 nodes, 8 heads of 128 bf16 values.)  Values that no 16-byte load
+// fits have the second instance alone.
+static int att_side(int64_t rows, int graphs, bool aligned) {
+    return aligned && rows <= 32 * (int64_t)(graphs < 1 ? 1 : graphs) ? SIDE_16 : SIDE_64;
 }
 // Workgroups of a launch.  Where there are many, each goes over several key heads: looking the graph up, and the workgroups
 // that find no tile, are then paid for less often.
@@ -840,9 +809,9 @@ static int att_grid(AttDims& d, int64_t rows, int tile) {
     while (d.heads_a_wg < d.kv_heads && slots * d.splits * (d.kv_heads / (2 * d.heads_a_wg)) >= 2048) d.heads_a_wg *= 2;
     return (int)(slots * ((d.kv_heads + d.heads_a_wg - 1) / d.heads_a_wg));
 }
-// Shares of the other side's tiles: two waves for each of the 1024 SIMDs, and 256 rows a share at least.
-static int att_splits(int64_t waves, int64_t other, int graphs) {
-    const int64_t want = 2048 / (waves < 1 ? 1 : waves), most = other / (graphs < 1 ? 1 : graphs) / 256;
+// Shares of the other side's tiles: so many waves for the 1024 SIMDs as `target`, and 256 rows a share at least.
+static int att_splits(int64_t waves, int64_t other, int graphs, int target) {
+    const int64_t want = target / (waves < 1 ? 1 : waves), most = other / (graphs < 1 ? 1 : graphs) / 256;
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
@@ -855,7 +824,7 @@ static int att_width(const void* p, int64_t row, int64_t head, int dim, int es) 
 // 16-byte loads, and what a tile spans within the 2 GiB that a buffer's offsets reach
 static bool att_aligned(const tsd_attention& a, const void* dout, int64_t do_row, int64_t do_head) {
     const int es = a.dtype == TSD_F32 ? 4 : 2, group = a.heads / a.kv_heads;
-    auto near = [&](int64_t row, int64_t head) { return row >= 0 && head >= 0 && 129 * row + group * head < (1ll << 29); };
+    auto near = [&](int64_t row, int64_t head) { return row >= 0 && head >= 0 && 65 * row + group * head < (1ll << 29); };
     return att_width(a.q, a.q_row, a.q_head, a.dim, es) == 8 && att_width(a.k, a.k_row, a.k_head, a.dim, es) == 8 &&
            att_width(a.v, a.v_row, a.v_head, a.dim, es) == 8 && near(a.q_row, a.q_head) && near(a.k_row, a.k_head) &&
            near(a.v_row, a.v_head) &&
@@ -871,16 +840,15 @@ struct AttPlan {
 static AttPlan att_plan(const tsd_attention& a, bool aligned) {
     AttPlan p = {};
     const int group = a.heads / a.kv_heads;
-    const bool f32 = a.dtype == TSD_F32;
     const int64_t rows = (int64_t)a.num_queries * group, keys = a.num_keys;
     auto waves = [&](int64_t n) {
-        const int side = att_side(n, a.num_graphs, f32, true);
+        const int side = att_side(n, a.num_graphs, true);
         return (n / SIDE_ROWS[side] + a.num_graphs) * a.kv_heads * (side == SIDE_16 ? 1 : 4);
     };
-    p.side_q = att_side(rows, a.num_graphs, f32, aligned);
-    p.side_k = att_side(keys, a.num_graphs, f32, aligned);
-    p.splits_q = att_splits(waves(rows), keys, a.num_graphs);
-    p.splits_k = att_splits(waves(keys), rows, a.num_graphs);
+    p.side_q = att_side(rows, a.num_graphs, aligned);
+    p.side_k = att_side(keys, a.num_graphs, aligned);
+    p.splits_q = att_splits(waves(rows), keys, a.num_graphs, 2048);
+    p.splits_k = att_splits(waves(keys), rows, a.num_graphs, 4096);
     const size_t nq = (size_t)a.num_queries * a.heads, nk = (size_t)keys * a.kv_heads;
     p.fwd = p.splits_q > 1 ? p.splits_q * nq * (a.dim + 2) : 0;
     const size_t q = p.splits_q > 1 ? p.splits_q * nq * a.dim : 0, k = p.splits_k > 1 ? 2 * p.splits_k * nk * a.dim : 0;
@@ -896,8 +864,8 @@ static int att_check(const char* name, const tsd_attention* a) {
                     a->heads % a->kv_heads == 0 && a->dim >= 1,
                 "%s: bad sizes: %d graphs, %d queries, %d keys, %d heads, %d key heads, dim %d", name, a->num_graphs,
                 a->num_queries, a->num_keys, a->heads, a->kv_heads, a->dim);
-    if (a->dim > TSD_ATTENTION_MAX_DIM || (int64_t)a->num_queries * a->heads > (1 << 30) ||
-        (int64_t)a->num_keys * a->heads > (1 << 30) || (int64_t)a->num_graphs * a->kv_heads > (1 << 22)) {
+    if (a->dim > TSD_ATTENTION_MAX_DIM || (int64_t)a->num_queries * a->heads > (1 << 29) ||
+        (int64_t)a->num_keys * a->heads > (1 << 29) || (int64_t)a->num_graphs * a->kv_heads > (1 << 22) || a->heads > (1 << 16)) {
         set_error("%s: head dim %d (at most %d), %d queries, %d keys, %d heads, %d graphs", name, a->dim, TSD_ATTENTION_MAX_DIM,
                   a->num_queries, a->num_keys, a->heads, a->num_graphs);
         return TSD_ERR_UNSUPPORTED;
@@ -925,6 +893,7 @@ static AttDims att_dims(const tsd_attention& a) {
     d.v_head = a.v_head;
     d.scale = a.scale;
     d.scale2 = a.scale * LOG2E;
+    if (d.scale2 == 0.f) d.scale2 = 0x1p-126f;  // (a closed key's infinite score stays one, every other score vanishes)
     d.qvw = att_width(a.q, a.q_row, a.q_head, a.dim, es);
     d.kvw = att_width(a.k, a.k_row, a.k_head, a.dim, es);
     d.vvw = att_width(a.v, a.v_row, a.v_head, a.dim, es);
@@ -936,54 +905,52 @@ static AttDims att_dims(const tsd_attention& a) {
 
 // rows of a tile of the other side: what keeps three workgroups on a CU
 template <class T, int DP, int WAVES> constexpr int att_tile() { return WAVES == 1 || DP == 128 || sizeof(T) == 4 ? 32 : 64; }
-template <class T, int DP, int WAVES, int RS, bool FAST>
-static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, T* rest, float* lse, float* scratch,
-                          hipStream_t st) {
+template <class T, int DP, int WAVES, bool FAST>
+static int att_launch_fwd(AttDims d, const tsd_attention& a, T* out, T* rest, float* lse, float* scratch, hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
     constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
-    auto k = att_fwd_kernel<T, DP, WAVES, RS, KT, FAST>;
+    auto k = att_fwd_kernel<T, DP, WAVES, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
-                       (const T*)a.v, out, rest, lse, scratch);
+    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d,
+                       (const T*)a.q, (const T*)a.k, (const T*)a.v, out, rest, lse, scratch);
     TSD_LAUNCH_CHECK("attention_fwd");
     return TSD_OK;
 }
-template <class T, int DP, int WAVES, int RS, bool FAST>
-static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* rest, const T* dout, const float* lse, float* delta,
-                         T* dq, float* part, hipStream_t st) {
+template <class T, int DP, int WAVES, bool FAST>
+static int att_launch_dq(AttDims d, const tsd_attention& a, const T* out, const T* rest, const T* dout, const float* lse,
+                         float* delta, T* dq, float* part, hipStream_t st) {
     constexpr int KT = att_tile<T, DP, WAVES>();
     constexpr int lds = att_buffers<T, FAST>() * 2 * Tile<T, KT, DP / 8>::BYTES + MASK_BYTES;
     static DeviceOnce once;
-    auto k = att_dq_kernel<T, DP, WAVES, RS, KT, FAST>;
+    auto k = att_dq_kernel<T, DP, WAVES, KT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * RS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
-                       (const T*)a.v, out, rest, dout, lse, delta, dq, part);
+    hipLaunchKernelGGL(k, dim3(att_grid(d, (int64_t)d.rows_q * d.group, WAVES * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d,
+                       (const T*)a.q, (const T*)a.k, (const T*)a.v, out, rest, dout, lse, delta, dq, part);
     TSD_LAUNCH_CHECK("attention_dq");
     return TSD_OK;
 }
-template <class T, int DP, int WAVES, int KS, bool FAST>
+template <class T, int DP, int WAVES, bool FAST>
 static int att_launch_dkv(AttDims d, const tsd_attention& a, const T* dout, const float* lse, const float* delta, T* dk, T* dv,
                           float* part, hipStream_t st) {
     constexpr int RT = 32;
     constexpr int lds = att_buffers<T, FAST>() * (2 * Tile<T, RT, DP / 8>::BYTES + 512);
     static DeviceOnce once;
-    auto k = att_dkv_kernel<T, DP, WAVES, KS, RT, FAST>;
+    auto k = att_dkv_kernel<T, DP, WAVES, RT, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
-    hipLaunchKernelGGL(k, dim3(att_grid(d, d.rows_k, WAVES * KS * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d, (const T*)a.q, (const T*)a.k,
-                       (const T*)a.v, dout, lse, delta, dk, dv, part);
+    hipLaunchKernelGGL(k, dim3(att_grid(d, d.rows_k, WAVES * 16), 1, d.splits), dim3(WAVES * 64), lds, st, d,
+                       (const T*)a.q, (const T*)a.k, (const T*)a.v, dout, lse, delta, dk, dv, part);
     TSD_LAUNCH_CHECK("attention_dkv");
     return TSD_OK;
 }
-// launch<T, DP, waves, subtiles of 16 a wave, FAST> of a side
-#define ATT_BY_SIDE(rc, side, aligned, launch, ...)                                      \
-    if (!(aligned)) rc = launch<T, DP, 4, 1, false>(__VA_ARGS__);                        \
-    else if (side == SIDE_16) rc = launch<T, DP, 1, 1, true>(__VA_ARGS__);               \
-    else if (sizeof(T) == 4 || side == SIDE_64) rc = launch<T, DP, 4, 1, true>(__VA_ARGS__); \
-    else if constexpr (sizeof(T) == 2) rc = launch<T, DP, 4, 2, true>(__VA_ARGS__);
+// launch<T, DP, waves, FAST> of a side
+#define ATT_BY_SIDE(rc, side, aligned, launch, ...)                           \
+    if (!(aligned)) rc = launch<T, DP, 4, false>(__VA_ARGS__);                \
+    else if (side == SIDE_16) rc = launch<T, DP, 1, true>(__VA_ARGS__);       \
+    else rc = launch<T, DP, 4, true>(__VA_ARGS__);
 
 template <class T, int DP>
 static int att_fwd(AttDims d, const tsd_attention& a, void* out, void* rest, float* lse, float* scratch, hipStream_t st) {
@@ -1002,8 +969,8 @@ static int att_fwd(AttDims d, const tsd_attention& a, void* out, void* rest, flo
     return rc;
 }
 template <class T, int DP>
-static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const void* rest, const void* dout, int64_t do_row, int64_t do_head,
-                   const float* lse, void* dq, void* dk, void* dv, float* scratch, hipStream_t st) {
+static int att_bwd(AttDims d, const tsd_attention& a, const void* out, const void* rest, const void* dout, int64_t do_row,
+                   int64_t do_head, const float* lse, void* dq, void* dk, void* dv, float* scratch, hipStream_t st) {
     const bool aligned = att_aligned(a, dout, do_row, do_head);
     const AttPlan p = att_plan(a, aligned);
     float *delta = scratch, *part = scratch + p.part;
@@ -1050,7 +1017,8 @@ size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backwa
     return backward ? p.bwd : p.fwd;
 }
 
-int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats, void* stream) {
+int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats,
+                            void* stream) {
     const int rc = att_check("tsd_graph_attention_fwd", a);
     if (rc != TSD_OK) return rc;
     if (a->num_queries == 0) return TSD_OK;
@@ -1068,8 +1036,8 @@ int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, f
     return TSD_OK;
 }
 
-int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const void* out_rest, const float* lse, const void* dout, int64_t do_row,
-                            int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream) {
+int tsd_graph_attention_bwd(const tsd_attention* a, const void* out, const void* out_rest, const float* lse, const void* dout,
+                            int64_t do_row, int64_t do_head, void* dq, void* dk, void* dv, float* scratch, size_t scratch_floats, void* stream) {
     const int rc = att_check("tsd_graph_attention_bwd", a);
     if (rc != TSD_OK) return rc;
     const AttPlan p = att_plan(*a, true);
