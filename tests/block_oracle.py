@@ -5,13 +5,15 @@ Every function returns {name: (value, tolerance)}, tolerances element by element
     rounds an intermediate to feed a matrix product (the weights P and dS, D = [dg | du]), its magnitude times u beside it;
   * e = 2^-24: a sum of n products in fp32 is off by at most (n + PAD) e times the sum of the products' magnitudes; PAD
     covers the three-plane operands of fp32 products (each product off by < 4 e) and the handful of operations around a sum;
-  * exp2 and the reciprocal of the hardware are good to one unit of the last place (2 e), of an argument off by its own e.
+  * exp2 and the reciprocal of the hardware are good to one unit of the last place (2 e), of an argument off by its own e; a
+    result of exp2 below the smallest normal number of fp32 is 0, which TINY = 2^-126 beside a weight covers.
 Second-order terms are covered by the factor SAFE."""
 import math
 
 import torch
 
 E = 2.0 ** -24
+TINY = 2.0 ** -126
 PAD = 16
 SAFE = 1.05
 
@@ -122,7 +124,7 @@ def attention(q, k, v, q_ptr, k_ptr, mask, scale, dout=None, dtype=torch.float32
             P = torch.softmax(S, -1)
             # relative error of a weight: its score's and the maximum's and sum's own, the sum over keys, exp2
             eP = eS + (P * eS).sum(-1, keepdim=True) + 2 * eS.amax(-1, keepdim=True) + (L + PAD) * E
-            wP = P * eP + rounded(P, dtype)  # as the matrix operand of P V, P^T dO
+            wP = P * eP + TINY + rounded(P, dtype)  # as the matrix operand of P V, P^T dO
             O = P @ V
             eO = SAFE * (wP @ V.abs() + (L + PAD) * E * (P @ V.abs()))
             got["out"][0][a:b, h], got["out"][1][a:b, h] = O, eO + rounded(O, dtype)
@@ -134,7 +136,7 @@ def attention(q, k, v, q_ptr, k_ptr, mask, scale, dout=None, dtype=torch.float32
             e1 = (D + PAD) * E * (G.abs() @ V.abs().t())
             e2 = (G.abs() * (eO + rounded(O, dtype))).sum(-1, keepdim=True) + (D + PAD) * E * (G * O).abs().sum(-1, keepdim=True)
             dS = P * (dP - delta)
-            edS = SAFE * (P * (e1 + e2) + (eP + 4 * E) * P * (dP.abs() + delta.abs())) + rounded(dS, dtype)
+            edS = SAFE * (P * (e1 + e2) + ((eP + 4 * E) * P + TINY) * (dP.abs() + delta.abs())) + rounded(dS, dtype)
             dQ = scale * (dS @ K)
             eQ = SAFE * abs(scale) * (edS @ K.abs() + (L + PAD) * E * (dS.abs() @ K.abs())) + rounded(dQ, dtype)
             got["dq"][0][a:b, h], got["dq"][1][a:b, h] = dQ, eQ

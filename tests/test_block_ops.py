@@ -99,6 +99,20 @@ def test_c_entries_refuse_before_any_launch():
     assert n > 0 and af(att(**long), p, None, None, p, n - 1, None) == bad
 
 
+def test_c_attention_refuses_what_its_launches_and_offsets_do_not_reach():
+    from tsdiff_amd import _lib
+    lib = _lib.load()
+    p = 4096
+    for sizes in (dict(num_queries=1 << 29), dict(num_keys=1 << 29), dict(num_graphs=1 << 23), dict(heads=1 << 17, kv_heads=1 << 17)):
+        a = dict(dtype=1, num_graphs=2, num_queries=4, num_keys=4, heads=4, kv_heads=1, dim=8, scale=1.0, q=p, k=p, v=p, q_ptr=p,
+                 k_ptr=p)
+        a.update(sizes)
+        a = C.byref(_lib.Attention(**a))
+        assert lib.tsd_graph_attention_scratch_floats(a, 1) == 0
+        assert lib.tsd_graph_attention_fwd(a, p, None, None, None, 0, None) == _lib.TSD_ERR_UNSUPPORTED
+        assert lib.tsd_graph_attention_bwd(a, p, None, p, p, 32, 8, p, p, p, p, 1 << 40, None) == _lib.TSD_ERR_UNSUPPORTED
+
+
 def close(got, want, tol=1e-6):
     assert float((got - want).abs().max()) <= tol * max(1.0, float(want.abs().max()))
 

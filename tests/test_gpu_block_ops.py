@@ -149,6 +149,21 @@ def test_gated_linear_strides_and_single_gradients(dtype):
         O.check(g, want[n], n)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_linear_copies_odd_rows_of_strided_inputs(dtype):
+    """rows that no 16-byte load fits, long products: a slice of wider rows, weights between two borders"""
+    from tsdiff_amd.block_ops import gated_linear
+    x, wg, wu, bg, bu, dh, want = gated_case(600, 121, 77, dtype, "swish", True, seed=5)
+    xd = torch.full((600, 130), float("nan"), dtype=dtype)
+    xd[:, 3:124] = x
+    xd = xd.to(DEV)[:, 3:124].requires_grad_()
+    w = torch.cat((torch.zeros(1, dtype=dtype), wg.flatten(), wu.flatten())).to(DEV)
+    rest = [w[1:1 + wg.numel()].view(77, 121).requires_grad_(), w[1 + wg.numel():].view(77, 121).requires_grad_()] + dev(bg, bu)
+    h = gated_linear(xd, *rest)
+    grads = torch.autograd.grad(h, [xd] + rest, dh.to(DEV))
+    gated_check(h, dict(zip(("dx", "dwg", "dwu", "dbg", "dbu"), grads)), want)
+
+
 def test_gated_linear_without_rows_and_in_three_dimensions():
     from tsdiff_amd.block_ops import gated_linear
     x, wg, wu, bg, bu, dh, want = gated_case(6, 16, 24, torch.float32, "swish", True)
@@ -299,6 +314,73 @@ def test_large_scores_do_not_overflow():
     for scale in (100.0, -100.0, 0.0):
         want = O.attention(q, k, v, [0, 40], [0, 40], None, scale)
         O.check(graph_attention(*dev(q, k, v), ptr, scale=scale), want["out"], f"scale {scale}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.4, 60.0, -60.0])
+def test_attention_of_any_scale_with_masks(scale, dtype):
+    """whatever the scale makes of the largest score, a masked key's is no candidate"""
+    from tsdiff_amd.block_ops import graph_attention
+    q, k, v, do, qp, kp, mask, _ = attention_case([20, 70, 9], None, 2, 1, 24, dtype, True, extra=4)
+    want = O.attention(q, k, v, qp, kp, mask, scale, do, dtype)
+    k, v = k.clone(), v.clone()
+    k[~mask] = v[~mask] = float("nan")
+    t = dev(q, k, v)
+    out = graph_attention(*t, torch.tensor(qp, device=DEV), key_mask=mask.to(DEV).to(torch.uint8) * 254, scale=scale)
+    O.check(out, want["out"], "out")
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, t, do.to(DEV))):
+        O.check(g, want[n], n)
+
+
+@pytest.mark.parametrize("n", [20, 200])
+def test_rows_whose_scores_are_all_minus_infinity_count_as_rows_without_keys(n):
+    from tsdiff_amd.block_ops import graph_attention
+    q, k, v, do = (normal(s, 2 * n, 1, 32, dtype=torch.bfloat16) for s in (1, 2, 3, 4))
+    q[:n] = q[:n].abs() + 1
+    k[:n] = float("-inf")  # every key of the first graph
+    t = dev(q, k, v)
+    out = graph_attention(*t, torch.tensor([0, n, 2 * n], device=DEV))
+    grads = torch.autograd.grad(out, t, do.to(DEV))
+    want = O.attention(q[n:], k[n:], v[n:], [0, n], [0, n], None, 32 ** -0.5, do[n:], torch.bfloat16)
+    for name, g in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        assert not g[:n].any(), name
+        O.check(g[n:], want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_with_key_heads_that_no_power_of_two_divides(dtype):
+    """5 key heads of 3 heads each, and so many graphs that a workgroup goes over several key heads"""
+    attention_run(*attention_case([(7 * i) % 4 for i in range(700)], None, 15, 5, 8, dtype, False), same=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_c_attention_without_what_the_rounding_left(dtype):
+    """the C entries, into the middle of buffers that nothing else of may change; out_rest and the forward's lse left out"""
+    import ctypes as C
+
+    from tsdiff_amd import _lib
+    lib = _lib.load()
+    q, k, v, do, qp, kp, mask, want = attention_case([20, 33], None, 2, 2, 32, dtype, False)
+    t = dev(q, k, v, do, grad=False)
+    ptr = torch.tensor(qp, dtype=torch.int32, device=DEV)
+    a = _lib.Attention(dtype=1 if dtype == torch.bfloat16 else 2, num_graphs=2, num_queries=53, num_keys=53, heads=2, kv_heads=2,
+                       dim=32, scale=32 ** -0.5, q=t[0].data_ptr(), k=t[1].data_ptr(), v=t[2].data_ptr(), q_row=64, q_head=32,
+                       k_row=64, k_head=32, v_row=64, v_head=32, q_ptr=ptr.data_ptr(), k_ptr=ptr.data_ptr(), key_mask=None)
+    n = 53 * 64
+    whole = [torch.full((n + 128,), 5.0, dtype=dtype, device=DEV) for _ in range(5)]
+    at = [w[64:].data_ptr() for w in whole]
+    lse = torch.empty(53, 2, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.tsd_graph_attention_fwd(C.byref(a), at[4], None, None, None, 0, stream) == 0
+    assert lib.tsd_graph_attention_fwd(C.byref(a), at[0], None, lse.data_ptr(), None, 0, stream) == 0
+    floats = lib.tsd_graph_attention_scratch_floats(C.byref(a), 1)
+    scratch = torch.empty(floats, device=DEV)
+    assert lib.tsd_graph_attention_bwd(C.byref(a), at[0], None, lse.data_ptr(), t[3].data_ptr(), 64, 32, at[1], at[2], at[3],
+                                       scratch.data_ptr(), floats, stream) == 0
+    assert torch.equal(whole[0], whole[4])
+    for name, w in zip(("out", "dq", "dk", "dv"), whole):
+        assert (w[:64] == 5).all() and (w[64 + n:] == 5).all()
+        O.check(w[64:64 + n].view(53, 2, 32), want[name], name)
 
 
 # ---- all of them ----------------------------------------------------------------------------------------------

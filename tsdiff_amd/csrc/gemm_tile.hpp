@@ -31,11 +31,9 @@ template <class T> struct RowOperand {
         return (two ? first2 + r - split : first + r) < rows ? (uint32_t)(((two ? r - split : r) * ld + c * 8) * (int)sizeof(T))
                                                               : DMA_NOWHERE;
     }
-    __device__ __forceinline__ bool inside(int, int c, int k) const { return k + c * 8 < kmax; }
     __device__ __forceinline__ const T* base(bool two, int k) const {
         return (two ? p2 + (int64_t)first2 * ld : p + (int64_t)first * ld) + k;
     }
-    __device__ __forceinline__ bool second(int r, int) const { return r >= split; }
 };
 // Rows of the contraction, from `ksplit` on those of a second matrix (kmax rows each), from `wrap` on all of them once more
 // (wrap: a multiple of 16); columns first ..

@@ -729,7 +729,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                 in_registers<T>(kf);
                 in_registers<T>(vf);
             },
-            [&](int, uint64_t, int buf) {
+            [&](int, uint64_t open, int buf) {
                 const char* ql = lds + buf * BUF;
                 const char* gl = ql + RTile::BYTES;
                 const float* stat = reinterpret_cast<const float*>(ql + STAT);
@@ -754,9 +754,21 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float w = exp2_fast(__builtin_fmaf(s[u][e], d.scale2, -L[e]));
-                            s[u][e] = open_key ? w : 0.f;
-                            dp[u][e] = open_key ? w * (dp[u][e] - del[e]) : 0.f;
+                            s[u][e] = w;
+                            dp[u][e] = w * (dp[u][e] - del[e]);
                         }
+                    }
+                    if ((uint32_t)(open >> (32 * p)) != 0xffffffffu) {  // what zeros make of infinite keys is no row's
+                        const int bits = (int)(uint32_t)(open >> (32 * p + 8 * g));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe(bits, 4 * u + e, 1);
+                                const float w = s[u][e], ds = dp[u][e];
+                                s[u][e] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, w) & m);
+                                dp[u][e] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, ds) & m);
+                            }
                     }
                     const Weights<T, att_rest<T, WAVES>()> pf = {s[0], s[1]}, df = {dp[0], dp[1]};
 #pragma unroll
@@ -774,7 +786,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             const int y = t * 16 + g * 4, n = d.dim - y;
-            // a masked key's gradients are 0 whatever the rows that do not read it hold
+            // a masked key's gradients are 0 whatever the rows that do not read it hold (a lane's sums are one key's)
             const f32x4 zero = {0, 0, 0, 0}, rk = open_key ? ak[t] * d.scale : zero, rv = open_key ? av[t] : zero;
             if (d.splits > 1) {
                 store4(part + (blockIdx.z * all + at) * d.dim + y, rk, n, d.dim % 4 == 0);
