@@ -231,10 +231,16 @@ template <class T, int ROWS_, int C_> struct Tile {
 // ---------------------------------------------------------------------------------------------
 using i32x4 = int __attribute__((ext_vector_type(4)));
 constexpr uint32_t DMA_NOWHERE = 0x80000000u;
-__device__ __forceinline__ i32x4 dma_buffer(const void* p) {  // 2 GiB from p on; p the same in all lanes
+__device__ __forceinline__ i32x4 dma_buffer(const void* p) {  // 2 GiB from p on; p (48 bits) the same in all lanes
     const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff),
-                 0x7fffffff, 0x00027000};
+    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)), 0x7fffffff,
+                 0x00027000};
+}
+__device__ __forceinline__ void dma_advance(i32x4& buf, int64_t bytes) {
+    const int lo = buf[0], hi = buf[1];
+    const uint64_t a = ((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo) + (uint64_t)bytes;
+    buf[0] = (int)(uint32_t)a;
+    buf[1] = (int)(a >> 32);
 }
 // the same bounds for loads to registers
 __device__ __forceinline__ f32x4 buffer_load(i32x4 buf, uint32_t off) {

@@ -12,33 +12,40 @@ namespace blk {
 constexpr int GEMM_WG = 256;  // four waves, two by two over the output tile
 constexpr int GEMM_K = 32;    // steps of the contraction a tile
 
-// Tile row r is matrix row first + r (r < split) or row first2 + r - split of a second matrix; k along the rows
-template <class T> struct RowOperand {
-    static constexpr bool ACROSS = false;
+// Tile row r is matrix row first + r (r < split) or, TWO, row first2 + r - split of a second matrix; k along the rows
+template <class T, bool TWO> struct RowOperand {
+    static constexpr bool ACROSS = false, BASES = TWO;
     const T *p, *p2;
     int64_t ld;
     int rows, kmax, first, split, first2;
     int vw;  // load_raw's
     template <int N> using TileOf = Tile<T, N, GEMM_K / 8>;
     __device__ __forceinline__ void load(Raw<T>& raw, int r, int c, int k) const {
-        const bool two = r >= split;
+        const bool two = TWO && r >= split;
         const int row = two ? first2 + r - split : first + r, kk = k + c * 8, n = row < rows ? kmax - kk : 0;
         load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)row * ld + kk : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
     }
     // bytes from the tile's first matrix (both matrices' tiles fit 2 GiB: the caller has seen to it)
     __device__ __forceinline__ uint32_t offset(int r, int c) const {
-        const bool two = r >= split;
+        const bool two = TWO && r >= split;
         return (two ? first2 + r - split : first + r) < rows ? (uint32_t)(((two ? r - split : r) * ld + c * 8) * (int)sizeof(T))
                                                               : DMA_NOWHERE;
     }
-    __device__ __forceinline__ const T* base(bool two, int k) const {
-        return (two ? p2 + (int64_t)first2 * ld : p + (int64_t)first * ld) + k;
+    // the first value of the tile at k that a load of rows `row` .. reads from, and how many k's its matrix has from there on
+    __device__ __forceinline__ const T* base(int row, int k, int& left) const {
+        left = kmax - k;
+        return (TWO && row >= split ? p2 + (int64_t)first2 * ld : p + (int64_t)first * ld) + k;
     }
+    // from the tile at k to the result they follow each other in memory and lie inside of one matrix
+    __device__ __forceinline__ int whole_until(int) const { return kmax; }
+    __device__ __forceinline__ int64_t step() const { return GEMM_K; }
+    // is k + r (or chunk c of row r at k) there
+    __device__ __forceinline__ static bool has(int, int c, int left) { return c * 8 < left; }
 };
 // Rows of the contraction, from `ksplit` on those of a second matrix (kmax rows each), from `wrap` on all of them once more
 // (wrap: a multiple of 16); columns first ..
 template <class T> struct ColOperand {
-    static constexpr bool ACROSS = true;
+    static constexpr bool ACROSS = true, BASES = false;
     const T *p, *p2;
     int64_t ld;
     int cols, kmax, first, ksplit, wrap;
@@ -50,6 +57,25 @@ template <class T> struct ColOperand {
         const int kk = kr - (two ? ksplit : 0), col = first + c * 8, n = kk < kmax ? cols - col : 0;
         load_raw(raw, (two ? p2 : p) + (n > 0 ? (int64_t)kk * ld + col : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
     }
+    __device__ __forceinline__ uint32_t offset(int r, int c) const {
+        return first + c * 8 < cols ? (uint32_t)((r * ld + c * 8) * (int)sizeof(T)) : DMA_NOWHERE;
+    }
+    // ksplit and wrap are multiples of 8, as few rows as a wave's load may hold: it lies on one side
+    __device__ __forceinline__ const T* base(int row, int k, int& left) const {
+        const int kw = k - (k + row >= wrap ? wrap : 0);
+        const bool two = kw + row >= ksplit;
+        const int kk = kw - (two ? ksplit : 0);
+        left = kmax - kk;
+        return (two ? p2 : p) + (int64_t)kk * ld + first;
+    }
+    __device__ __forceinline__ int whole_until(int k) const {
+        const bool again = k >= wrap;
+        const int kw = again ? k - wrap : k, kk = kw < ksplit ? kw : kw - ksplit;
+        const int edge = kw < ksplit ? ksplit - kw : again ? 1 << 30 : wrap - k, rows = kmax - kk;
+        return k + (edge < rows ? edge : rows);
+    }
+    __device__ __forceinline__ int64_t step() const { return GEMM_K * ld; }
+    __device__ __forceinline__ static bool has(int r, int, int left) { return r < left; }
 };
 
 // Where the chunks of a tile of N output rows (or columns) lie, for 32-bit offsets from a base that is the same for a wave;
@@ -60,36 +86,41 @@ template <class T, int N, class Op, bool PERMUTED> struct Places {
     static constexpr int UNITS = Lds::ROWS * Lds::C, U = UNITS < GEMM_WG ? 1 : UNITS / GEMM_WG;
     // (a tile smaller than the workgroup is loaded by several waves alike: every wave counts the same loads)
     static_assert(UNITS % GEMM_WG == 0 || (GEMM_WG % UNITS == 0 && UNITS % 64 == 0), "whole loads");
+    static constexpr int B = Op::BASES ? U : 1;  // bases of a wave's loads
     uint32_t off[U];
     int row[U], chunk[U];
+    // The tiles of a whole part of the operand (most of them) follow each other by the same distance, with no bounds to look
+    // at: `left` of them are still to come.
+    i32x4 at[B];
+    int left;
     __device__ __forceinline__ void init(const Op& op) {
+        left = 0;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int u = (threadIdx.x + i * GEMM_WG) % UNITS;
             row[i] = u / Lds::C;
             chunk[i] = PERMUTED ? (u % Lds::C) ^ Lds::swizzle(row[i]) : u % Lds::C;
-            if constexpr (!Op::ACROSS) {
-                off[i] = op.offset(row[i], chunk[i]);
-            } else {
-                const int col = op.first + chunk[i] * 8;
-                off[i] = col < op.cols ? (uint32_t)((row[i] * op.ld + chunk[i] * 8) * (int)sizeof(T)) : DMA_NOWHERE;
-            }
+            off[i] = op.offset(row[i], chunk[i]);
         }
     }
-    // One matrix a load: the 64 places of a wave lie on one side of the operand's split
-    template <class F> __device__ __forceinline__ void each(const Op& op, int k, F f) const {
+    // The tile at k; the one before it was at k - GEMM_K.  One matrix a load: the 64 places of a wave lie on one side of the
+    // operand's split.
+    template <class F> __device__ __forceinline__ void each(const Op& op, int k, F f) {
+        if (--left >= 0) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) dma_advance(at[b], op.step() * (int64_t)sizeof(T));
+#pragma unroll
+            for (int i = 0; i < U; ++i) f(i, at[Op::BASES ? i : 0], off[i]);
+            return;
+        }
+        left = (op.whole_until(k) - k) / GEMM_K - 1;
+        left = left < 0 ? 0 : left;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int wave_row = __builtin_amdgcn_readfirstlane(row[i]);
-            if constexpr (!Op::ACROSS) {
-                f(i, dma_buffer(op.base(wave_row >= op.split, k)), k + chunk[i] * 8 < op.kmax ? off[i] : DMA_NOWHERE);
-            } else {  // ksplit and wrap are multiples of 8, as few rows as a wave's load may hold: it lies on one side
-                const int kw = k - (k + wave_row >= op.wrap ? op.wrap : 0);
-                const bool two = kw + wave_row >= op.ksplit;
-                const int kk = kw - (two ? op.ksplit : 0);
-                f(i, dma_buffer((two ? op.p2 : op.p) + (int64_t)kk * op.ld + op.first),
-                  kk + row[i] < op.kmax ? off[i] : DMA_NOWHERE);
-            }
+            int rest;
+            const i32x4 buf = dma_buffer(op.base(__builtin_amdgcn_readfirstlane(row[i]), k, rest));
+            if (i < B) at[i] = buf;  // (of a tile in one matrix: all are the same)
+            f(i, buf, Op::has(row[i], chunk[i], rest) ? off[i] : DMA_NOWHERE);
         }
     }
 };
@@ -130,11 +161,15 @@ template <class T, int N, class Op> struct DmaStage {
     using At = Places<T, N, Op, true>;
     static constexpr int U = At::U;
     At places;
-    __device__ __forceinline__ void init(const Op& op) { places.init(op); }
-    __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) const {
-        places.each(op, k, [&](int i, i32x4 buf, uint32_t off) {
-            dma_load(buf, off, lds + (threadIdx.x / 64 * 64 + i * GEMM_WG) % At::UNITS * 16);
-        });
+    int at[U];  // LDS bytes of a wave's load
+    __device__ __forceinline__ void init(const Op& op) {
+        places.init(op);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            at[i] = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * 64 + i * GEMM_WG) % At::UNITS * 16);
+    }
+    __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) {
+        places.each(op, k, [&](int i, i32x4 buf, uint32_t off) { dma_load(buf, off, lds + at[i]); });
     }
 };
 

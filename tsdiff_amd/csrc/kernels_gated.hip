@@ -117,8 +117,8 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
     const int m0 = at.lo * BM, f0 = at.sh * FT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave & 1, wm = wave >> 1;
     const int nbase = wn * (FT / 2), mrow = wm * (BM / 2);
-    const RowOperand<T> ns = {wg, wu, d.ldw, d.out, d.inw, f0, FT, f0, d.wvw};
-    const RowOperand<T> ms = {x, x, d.ldx, d.rows, d.inw, m0, BM, 0, d.xvw};
+    const RowOperand<T, true> ns = {wg, wu, d.ldw, d.out, d.inw, f0, FT, f0, d.wvw};
+    const RowOperand<T, false> ms = {x, x, d.ldx, d.rows, d.inw, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     f32x4 vbg[TN], vbu[TN];
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktil
     const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
     const int width = d.planes * 2 * d.outp;  // of D
     const ColOperand<T> ns = {wg, wu, d.ldw, d.inw, d.out, k0, d.outp, 2 * d.outp, d.wvw};
-    const RowOperand<T> ms = {D, D, width, d.rows, width, m0, BM, 0, 8};
+    const RowOperand<T, false> ms = {D, D, width, d.rows, width, m0, BM, 0, 8};
     f32x4 acc[BN / 32][BM / 32];
     const int fb = blockIdx.y * share, fe = fb + share < width ? fb + share : width;
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
