@@ -118,6 +118,17 @@ def test_gated_linear(rows, fin, out, dtype):
     gated_check(h, dict(zip(("dx", "dwg", "dwu", "dbg", "dbu"), torch.autograd.grad(h, t, dh.to(DEV)))), want)
 
 
+@pytest.mark.parametrize("dtype,rows,fin,out", [(torch.bfloat16, 16300, 1020, 136), (torch.float16, 56000, 240, 124),
+                                                (torch.bfloat16, 8100, 40, 1016), (torch.float32, 9001, 72, 264)])
+def test_gated_linear_of_many_rows(dtype, rows, fin, out):
+    """the largest tiles, each ending inside of one"""
+    from tsdiff_amd.block_ops import gated_linear
+    x, wg, wu, bg, bu, dh, want = gated_case(rows, fin, out, dtype, "swish", True)
+    t = dev(x, wg, wu, bg, bu)
+    h = gated_linear(*t)
+    gated_check(h, dict(zip(("dx", "dwg", "dwu", "dbg", "dbu"), torch.autograd.grad(h, t, dh.to(DEV)))), want)
+
+
 @pytest.mark.parametrize("act", ["swish", "ssp", "ReLU", "Softplus"])
 def test_gated_linear_activations_without_biases(act):
     from tsdiff_amd.block_ops import gated_linear

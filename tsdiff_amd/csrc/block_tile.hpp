@@ -184,13 +184,13 @@ using s16x4 = short __attribute__((ext_vector_type(4)));
 using s16x8 = short __attribute__((ext_vector_type(8)));
 template <class T, int ROWS_, int C_> struct Tile {
     static constexpr int ROWS = ROWS_, C = C_;
-    static_assert(C == 4 || C == 8 || C == 16, "chunks of a row");
+    static_assert(C == 4 || C == 8 || C == 16 || C == 32, "chunks of a row");
     static constexpr int P = Elem<T>::P;
     static constexpr int PLANE = ROWS * C * 16, BYTES = P * PLANE;
     using vec = typename Elem<T>::vec;
     __device__ __forceinline__ static int swizzle(int r) {
         const int low = ((r >> 2) ^ (r >> 4)) & 1, b3 = (r >> 3) & 1;
-        if constexpr (C == 16) return low | (r & 3) << 1 | b3 << 3;
+        if constexpr (C >= 16) return low | (r & 3) << 1 | b3 << 3;
         if constexpr (C == 8) return low | ((r >> 1) & 1) << 1 | b3 << 2;
         return low | b3 << 1;
     }

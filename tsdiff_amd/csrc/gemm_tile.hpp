@@ -9,7 +9,9 @@
 namespace tsd {
 namespace blk {
 
-constexpr int GEMM_WG = 256;  // four waves, two by two over the output tile
+// Waves over one side of the output tile: two, of 64 rows or columns at most
+constexpr int gemm_waves(int n) { return n > 128 ? n / 64 : 2; }
+constexpr int gemm_wg(int bm, int bn) { return 64 * gemm_waves(bm) * gemm_waves(bn); }
 constexpr int GEMM_K = 32;    // steps of the contraction a tile
 
 // Tile row r is matrix row first + r (r < split) or, TWO, row first2 + r - split of a second matrix; k along the rows
@@ -81,23 +83,24 @@ template <class T> struct ColOperand {
 // Where the chunks of a tile of N output rows (or columns) lie, for 32-bit offsets from a base that is the same for a wave;
 // places outside of the matrix are NOWHERE.  LDS places for loads straight to LDS (PERMUTED): a wave's 64 lanes fill 64
 // neighbouring places, so the lane of place p of row r fetches chunk p ^ swizzle(r).
-template <class T, int N, class Op, bool PERMUTED> struct Places {
+template <class T, int N, int WG, class Op, bool PERMUTED> struct Places {
     using Lds = typename Op::template TileOf<N>;
-    static constexpr int UNITS = Lds::ROWS * Lds::C, U = UNITS < GEMM_WG ? 1 : UNITS / GEMM_WG;
+    static constexpr int UNITS = Lds::ROWS * Lds::C, U = UNITS < WG ? 1 : UNITS / WG;
     // (a tile smaller than the workgroup is loaded by several waves alike: every wave counts the same loads)
-    static_assert(UNITS % GEMM_WG == 0 || (GEMM_WG % UNITS == 0 && UNITS % 64 == 0), "whole loads");
+    static_assert(UNITS % WG == 0 || (WG % UNITS == 0 && UNITS % 64 == 0), "whole loads");
     static constexpr int B = Op::BASES ? U : 1;  // bases of a wave's loads
     uint32_t off[U];
     int row[U], chunk[U];
     // The tiles of a whole part of the operand (most of them) follow each other by the same distance, with no bounds to look
-    // at: `left` of them are still to come.
+    // at: `left` of them are still to come.  (Not for f32, where a second way to the registers costs more than it saves:
+    // forward of 3600 x 256 -> 2 x 1024 34 us against 31.)
     i32x4 at[B];
     int left;
     __device__ __forceinline__ void init(const Op& op) {
         left = 0;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = (threadIdx.x + i * GEMM_WG) % UNITS;
+            const int u = (threadIdx.x + i * WG) % UNITS;
             row[i] = u / Lds::C;
             chunk[i] = PERMUTED ? (u % Lds::C) ^ Lds::swizzle(row[i]) : u % Lds::C;
             off[i] = op.offset(row[i], chunk[i]);
@@ -106,15 +109,17 @@ template <class T, int N, class Op, bool PERMUTED> struct Places {
     // The tile at k; the one before it was at k - GEMM_K.  One matrix a load: the 64 places of a wave lie on one side of the
     // operand's split.
     template <class F> __device__ __forceinline__ void each(const Op& op, int k, F f) {
-        if (--left >= 0) {
+        if constexpr (PERMUTED) {
+            if (--left >= 0) {
 #pragma unroll
-            for (int b = 0; b < B; ++b) dma_advance(at[b], op.step() * (int64_t)sizeof(T));
+                for (int b = 0; b < B; ++b) dma_advance(at[b], op.step() * (int64_t)sizeof(T));
 #pragma unroll
-            for (int i = 0; i < U; ++i) f(i, at[Op::BASES ? i : 0], off[i]);
-            return;
+                for (int i = 0; i < U; ++i) f(i, at[Op::BASES ? i : 0], off[i]);
+                return;
+            }
+            left = (op.whole_until(k) - k) / GEMM_K - 1;
+            left = left < 0 ? 0 : left;
         }
-        left = (op.whole_until(k) - k) / GEMM_K - 1;
-        left = left < 0 ? 0 : left;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             int rest;
@@ -126,11 +131,11 @@ template <class T, int N, class Op, bool PERMUTED> struct Places {
 };
 
 // A tile by way of registers, DEPTH tiles under way.  FAST (f32): branch-free loads with the bounds in the buffer.
-template <class T, int N, class Op, int DEPTH, bool FAST> struct RegStage {
+template <class T, int N, int WG, class Op, int DEPTH, bool FAST> struct RegStage {
     using Lds = typename Op::template TileOf<N>;
-    static constexpr int UNITS = Lds::ROWS * Lds::C, U = (UNITS + GEMM_WG - 1) / GEMM_WG;
+    static constexpr int UNITS = Lds::ROWS * Lds::C, U = (UNITS + WG - 1) / WG;
     Raw<T> raw[DEPTH][U];
-    Places<T, N, Op, false> places;
+    Places<T, N, WG, Op, false> places;
     __device__ __forceinline__ void init(const Op& op) {
         if constexpr (FAST) places.init(op);
     }
@@ -143,22 +148,22 @@ template <class T, int N, class Op, int DEPTH, bool FAST> struct RegStage {
         } else {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                const int u = threadIdx.x + i * GEMM_WG;
-                if (UNITS % GEMM_WG == 0 || u < UNITS) op.load(raw[d][i], u / Lds::C, u % Lds::C, k);
+                const int u = threadIdx.x + i * WG;
+                if (UNITS % WG == 0 || u < UNITS) op.load(raw[d][i], u / Lds::C, u % Lds::C, k);
             }
         }
     }
     __device__ __forceinline__ void store(int d, char* lds) const {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS) Lds::put(lds, u / Lds::C, u % Lds::C, raw_chunk(raw[d][i]));
+            const int u = threadIdx.x + i * WG;
+            if (UNITS % WG == 0 || u < UNITS) Lds::put(lds, u / Lds::C, u % Lds::C, raw_chunk(raw[d][i]));
         }
     }
 };
 // Straight to LDS
-template <class T, int N, class Op> struct DmaStage {
-    using At = Places<T, N, Op, true>;
+template <class T, int N, int WG, class Op> struct DmaStage {
+    using At = Places<T, N, WG, Op, true>;
     static constexpr int U = At::U;
     At places;
     int at[U];  // LDS bytes of a wave's load
@@ -166,7 +171,7 @@ template <class T, int N, class Op> struct DmaStage {
         places.init(op);
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            at[i] = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * 64 + i * GEMM_WG) % At::UNITS * 16);
+            at[i] = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * 64 + i * WG) % At::UNITS * 16);
     }
     __device__ __forceinline__ void issue(const Op& op, int k, uint32_t lds) {
         places.each(op, k, [&](int i, i32x4 buf, uint32_t off) { dma_load(buf, off, lds + at[i]); });
@@ -177,32 +182,33 @@ template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
     using NT = typename NS::template TileOf<BN>;
     using MT = typename MS::template TileOf<BM>;
     static constexpr int BUF = NT::BYTES + MT::BYTES;
-    using Acc = f32x4[BN / 32][BM / 32];
+    static constexpr int WG = gemm_wg(BM, BN), MI = BM / gemm_waves(BM) / 16, NJ = BN / gemm_waves(BN) / 16;  // subtiles of a wave
+    using Acc = f32x4[NJ][MI];
 
     template <class NRow>
     __device__ __forceinline__ static void products(const char* nb, int mrow, NRow nrow, Acc& acc) {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
         const char* mb = nb + NT::BYTES;
-        Chunk<T> mf[BM / 32];
+        Chunk<T> mf[MI];
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
+        for (int i = 0; i < MI; ++i) {
             if constexpr (MS::ACROSS) mf[i] = MT::get_across(mb, 0, mrow / 16 + i);
             else mf[i] = MT::get(mb, mrow + i * 16 + r, c);
         }
 #pragma unroll
-        for (int j = 0; j < BN / 32; ++j) {
+        for (int j = 0; j < NJ; ++j) {
             Chunk<T> nf;
             if constexpr (NS::ACROSS) nf = NT::get_across(nb, 0, nrow(j) / 16);
             else nf = NT::get(nb, nrow(j) + r, c);
 #pragma unroll
-            for (int i = 0; i < BM / 32; ++i) acc[j][i] = mma(nf, mf[i], acc[j][i]);
+            for (int i = 0; i < MI; ++i) acc[j][i] = mma(nf, mf[i], acc[j][i]);
         }
     }
     __device__ __forceinline__ static void clear(Acc& acc) {
 #pragma unroll
-        for (int j = 0; j < BN / 32; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int i = 0; i < BM / 32; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < MI; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
     }
     // One output tile: acc[jn][im] of the calling wave, n rows nrow(jn) and m rows mrow + im * 16 of the tile; ends behind a
     // barrier.  The next DEPTH tiles' values are on their way into registers.  BUFS 2: two LDS buffers, one barrier a tile;
@@ -210,8 +216,8 @@ template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
     template <int DEPTH, int BUFS, bool FAST, class NRow>
     __device__ __forceinline__ static void by_registers(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow,
                                                         NRow nrow, Acc& acc) {
-        RegStage<T, BN, NS, DEPTH, FAST> nst;
-        RegStage<T, BM, MS, DEPTH, FAST> mst;
+        RegStage<T, BN, WG, NS, DEPTH, FAST> nst;
+        RegStage<T, BM, WG, MS, DEPTH, FAST> mst;
         nst.init(ns);
         mst.init(ms);
         clear(acc);
@@ -249,9 +255,9 @@ template <class T, int BM, int BN, class NS, class MS> struct GemmTile {
     template <int STAGES, class NRow>
     __device__ __forceinline__ static void by_dma(char* lds, const NS& ns, const MS& ms, int kbegin, int kend, int mrow, NRow nrow,
                                                   Acc& acc) {
-        DmaStage<T, BN, NS> nst;
-        DmaStage<T, BM, MS> mst;
-        constexpr int LOADS = DmaStage<T, BN, NS>::U + DmaStage<T, BM, MS>::U;
+        DmaStage<T, BN, WG, NS> nst;
+        DmaStage<T, BM, WG, MS> mst;
+        constexpr int LOADS = DmaStage<T, BN, WG, NS>::U + DmaStage<T, BM, WG, MS>::U;
         nst.init(ns);
         mst.init(ms);
         clear(acc);

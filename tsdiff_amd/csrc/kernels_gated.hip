@@ -10,6 +10,13 @@
 // written with what the rounding left as a second half of twice the width, which the products go over too, since sums of few
 // terms show one rounding more than large ones, and time is no matter there -- with each row tile's column sums in fp32;
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
+//
+// Measured (GPU time a launch; each product is 4 rows in out operations):
+//   bf16, 65536 x 256 -> 2 x 1024: forward 119 us (580 TFLOP/s, h and x are 170 MB of it), first of the backward 200 us (it
+//   writes D, 268 MB, and reads dh, 134 MB), dx 81 us (850 TFLOP/s), dW 91 us (755 TFLOP/s), sums 14 us.  Bound by what a CU
+//   draws from L2 (about 10 TB/s over the chip), the two first ones by that and by memory.
+//   f32, 3600 x 256 -> 2 x 1024: 30, 38, 31, 30 and 13 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
+//   f32, 17 x 256 -> 2 x 512, forward: 7 us, of which launching and one pass through memory are nearly all.
 #include <type_traits>
 
 #include "gemm_tile.hpp"
@@ -46,36 +53,36 @@ struct GatedDims {
 };
 
 // A tile of BM rows x BC columns in LDS on its way to (from) memory, so that neighbouring lanes touch neighbouring bytes
-template <class T, int BM, int BC> struct OutTile {
+template <class T, int BM, int BC, int WG> struct OutTile {
     static constexpr int LD = BC * (int)sizeof(T) + 16, BYTES = BM * LD, CH = BC / 8, UNITS = BM * CH;
-    static constexpr int U = (UNITS + GEMM_WG - 1) / GEMM_WG;
+    static constexpr int U = (UNITS + WG - 1) / WG;
     __device__ __forceinline__ static T* at(char* lds, int row, int col) { return reinterpret_cast<T*>(lds + row * LD) + col; }
     __device__ __forceinline__ static void fetch(Raw<T> (&raw)[U], const T* p, int64_t ld, int rows, int cols, int vw) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG, r = u / CH, c = (u % CH) * 8, n = u < UNITS && r < rows ? cols - c : 0;
+            const int u = threadIdx.x + i * WG, r = u / CH, c = (u % CH) * 8, n = u < UNITS && r < rows ? cols - c : 0;
             load_raw(raw[i], p + (n > 0 ? r * ld + c : 0), n < 0 ? 0 : n > 8 ? 8 : n, vw);
         }
     }
     __device__ __forceinline__ static void keep(const Raw<T> (&raw)[U], char* lds) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = threadIdx.x + i * GEMM_WG;
-            if (UNITS % GEMM_WG == 0 || u < UNITS)
+            const int u = threadIdx.x + i * WG;
+            if (UNITS % WG == 0 || u < UNITS)
                 __builtin_memcpy(__builtin_assume_aligned(at(lds, u / CH, (u % CH) * 8), 16), &raw[i], sizeof(Raw<T>));
         }
     }
     __device__ __forceinline__ static void write(char* lds, T* p, int64_t ld, int rows, int cols, int vw) {
         if (vw * sizeof(T) >= 16) {
             constexpr int V = 16 / sizeof(T), CV = BC / V;
-            for (int u = threadIdx.x; u < BM * CV; u += GEMM_WG) {
+            for (int u = threadIdx.x; u < BM * CV; u += WG) {
                 const int r = u / CV, c = (u % CV) * V;
                 if (r < rows && c < cols)
                     *reinterpret_cast<u32x4*>(p + r * ld + c) = *reinterpret_cast<const u32x4*>(at(lds, r, c));
             }
             return;
         }
-        for (int u = threadIdx.x; u < BM * BC; u += GEMM_WG) {
+        for (int u = threadIdx.x; u < BM * BC; u += WG) {
             const int r = u / BC, c = u % BC;
             if (r < rows && c < cols) p[r * ld + c] = *at(lds, r, c);
         }
@@ -89,7 +96,7 @@ constexpr int GATED_STAGES = 3;
 template <class T, int BM> constexpr int gated_bufs() { return sizeof(T) == 4 && BM == 128 ? 1 : 2; }
 template <class T, int BM, int BN, bool FAST, class NS, class MS, class NRow>
 __device__ __forceinline__ void gated_gemm(char* lds, const NS& ns, const MS& ms, int kb, int ke, int mrow, NRow nrow,
-                                           f32x4 (&acc)[BN / 32][BM / 32]) {
+                                           typename GemmTile<T, BM, BN, NS, MS>::Acc& acc) {
     using G = GemmTile<T, BM, BN, NS, MS>;
     if constexpr (FAST && sizeof(T) == 2) G::template by_dma<GATED_STAGES>(lds, ns, ms, kb, ke, mrow, nrow, acc);
     else G::template by_registers<gated_depth<BM>(), gated_bufs<T, BM>(), FAST>(lds, ns, ms, kb, ke, mrow, nrow, acc);
@@ -100,23 +107,25 @@ template <class T, int BM, int BN, bool FAST> constexpr int gated_lds(int behind
 }
 template <class T, int BM> constexpr bool gated_rest() { return sizeof(T) == 2 && BM == 32; }  // instances that can write it
 template <class T, int BM, int BN> constexpr int gated_behind(bool bwd) {
-    return (bwd ? gated_rest<T, BM>() ? 4 : 2 : 1) * OutTile<T, BM, BN / 2>::BYTES + (bwd ? 4 * (BN / 2) * 4 : 0);
+    return (bwd ? gated_rest<T, BM>() ? 4 : 2 : 1) * OutTile<T, BM, BN / 2, 64>::BYTES +
+           (bwd ? gemm_waves(BM) * 2 * (BN / 2) * 4 : 0);
 }
 
 template <class T, int BM, int BN, bool FAST, bool BWD>
-__global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
+__global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 : 3) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
                                                         const T* __restrict__ wg, const T* __restrict__ wu,
                                                         const T* __restrict__ bg, const T* __restrict__ bu,
                                                         const T* __restrict__ dh, T* __restrict__ h, T* __restrict__ D,
                                                         float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
-    constexpr int FT = BN / 2, TN = BN / 64, TM = BM / 32;  // columns a tile; gate (and up) subtiles, row subtiles of a wave
-    using Out = OutTile<T, BM, FT>;
+    constexpr int WG = gemm_wg(BM, BN), WM = gemm_waves(BM), WN = gemm_waves(BN);
+    constexpr int FT = BN / 2, TN = FT / WN / 16, TM = BM / WM / 16;  // columns a tile; gate (and up) subtiles, row subtiles of a wave
+    using Out = OutTile<T, BM, FT, WG>;
     const TileAt at = tile_at(blockIdx.x, ftiles);
     if (at.lo >= mtiles) return;
     const int m0 = at.lo * BM, f0 = at.sh * FT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave & 1, wm = wave >> 1;
-    const int nbase = wn * (FT / 2), mrow = wm * (BM / 2);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wm = wave / WN;
+    const int nbase = wn * (FT / WN), mrow = wm * (BM / WM);
     const RowOperand<T, true> ns = {wg, wu, d.ldw, d.out, d.inw, f0, FT, f0, d.wvw};
     const RowOperand<T, false> ms = {x, x, d.ldx, d.rows, d.inw, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
@@ -135,7 +144,7 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
                                [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     char* second = lds + Out::BYTES;
     constexpr bool REST = BWD && gated_rest<T, BM>();
-    float* red = reinterpret_cast<float*>(lds + (REST ? 4 : 2) * Out::BYTES);  // [2 (wm)][2][FT] column sums
+    float* red = reinterpret_cast<float*>(lds + (REST ? 4 : 2) * Out::BYTES);  // [WM][2][FT] column sums
     if constexpr (BWD) {
         Out::keep(dhr, lds);
         __syncthreads();
@@ -215,59 +224,64 @@ __global__ __launch_bounds__(GEMM_WG, sizeof(T) == 2 ? 3 : 2) void gated_kernel(
             Out::write(second + 2 * Out::BYTES, o + 3 * d.outp, ldd, d.rows - m0, d.outp - f0, 8);
         }
         if (part == nullptr) return;
-        for (int t = threadIdx.x; t < 2 * FT; t += GEMM_WG) {
+        for (int t = threadIdx.x; t < 2 * FT; t += WG) {
             const int f = f0 + t % FT;
-            if (f < d.outp) part[(int64_t)at.lo * 2 * d.outp + (t / FT) * d.outp + f] = red[t] + red[2 * FT + t];
+            float s = red[t];
+#pragma unroll
+            for (int w = 1; w < WM; ++w) s += red[2 * FT * w + t];
+            if (f < d.outp) part[(int64_t)at.lo * 2 * d.outp + (t / FT) * d.outp + f] = s;
         }
     }
 }
 
 // dx[m][k] = sum over f < 2 outp of D[m][f] [Wg; Wu][f][k]; several shares of f (blockIdx.y): their sums in fp32 to part
 template <class T, int BM, int BN, bool FAST>
-__global__ __launch_bounds__(GEMM_WG) void gated_dx_kernel(GatedDims d, int ktiles, int mtiles, const T* __restrict__ D,
+__global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dx_kernel(GatedDims d, int ktiles, int mtiles, const T* __restrict__ D,
                                                            const T* __restrict__ wg, const T* __restrict__ wu,
                                                            T* __restrict__ dx, int share, float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
-    using Out = OutTile<T, BM, BN>;
+    using Out = OutTile<T, BM, BN, gemm_wg(BM, BN)>;
     const TileAt at = tile_at(blockIdx.x, ktiles);
     if (at.lo >= mtiles) return;
     const int m0 = at.lo * BM, k0 = at.sh * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
+    constexpr int WM = gemm_waves(BM), WN = gemm_waves(BN), MI = BM / WM / 16, NJ = BN / WN / 16;
+    const int nbase = wave % WN * (BN / WN), mrow = wave / WN * (BM / WM);
     const int width = d.planes * 2 * d.outp;  // of D
     const ColOperand<T> ns = {wg, wu, d.ldw, d.inw, d.out, k0, d.outp, 2 * d.outp, d.wvw};
     const RowOperand<T, false> ms = {D, D, width, d.rows, width, m0, BM, 0, 8};
-    f32x4 acc[BN / 32][BM / 32];
+    f32x4 acc[NJ][MI];
     const int fb = blockIdx.y * share, fe = fb + share < width ? fb + share : width;
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     if (gridDim.y > 1) {
         float* o = part + (int64_t)blockIdx.y * d.rows * d.in;
 #pragma unroll
-        for (int j = 0; j < BN / 32; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int i = 0; i < BM / 32; ++i) {
+            for (int i = 0; i < MI; ++i) {
                 const int m = m0 + mrow + i * 16 + r, k = k0 + nbase + j * 16 + c4;
                 if (m < d.rows) store4(o + (int64_t)m * d.in + k, acc[j][i], d.in - k, d.in % 4 == 0);
             }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < BN / 32; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) store4(Out::at(lds, mrow + i * 16 + r, nbase + j * 16 + c4), acc[j][i], 4, true);
+        for (int i = 0; i < MI; ++i) store4(Out::at(lds, mrow + i * 16 + r, nbase + j * 16 + c4), acc[j][i], 4, true);
     __syncthreads();
     Out::write(lds, dx + (int64_t)m0 * d.in + k0, d.in, d.rows - m0, d.in - k0, d.dxvw);
 }
 
 // part[s][f][k] = sum over the rows of split s of D[m][f] x[m][k]
 template <class T, int BM, int BN, bool FAST>
-__global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktiles, int rows_a_split, const T* __restrict__ D,
+__global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dw_kernel(GatedDims d, int ktiles, int rows_a_split, const T* __restrict__ D,
                                                            const T* __restrict__ x, float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
     const int k0 = (blockIdx.x % ktiles) * BN, f0 = (blockIdx.x / ktiles) * BM;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int nbase = (wave & 1) * (BN / 2), mrow = (wave >> 1) * (BM / 2);
+    constexpr int WM = gemm_waves(BM), WN = gemm_waves(BN), MI = BM / WM / 16, NJ = BN / WN / 16;
+    const int nbase = wave % WN * (BN / WN), mrow = wave / WN * (BM / WM);
     const int64_t rb = (int64_t)blockIdx.y * rows_a_split;
     const int n = (int)(d.rows - rb < rows_a_split ? d.rows - rb : rows_a_split);
     // the rows of both halves of D, one behind the other, and x's rows twice
@@ -275,15 +289,15 @@ __global__ __launch_bounds__(GEMM_WG) void gated_dw_kernel(GatedDims d, int ktil
     const T *xb = x + rb * d.ldx, *db = D + rb * width;
     const ColOperand<T> ns = {xb, xb, d.ldx, d.inw, n, k0, half, 1 << 30, d.xvw};
     const ColOperand<T> ms = {db, db + 2 * d.outp, width, 2 * d.outp, n, f0, half, 1 << 30, 8};
-    f32x4 acc[BN / 32][BM / 32];
+    f32x4 acc[NJ][MI];
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.planes == 2 ? half + n : n, mrow, [&](int j) { return nbase + j * 16; },
                                 acc);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + (int64_t)blockIdx.y * 2 * d.outp * d.in;
 #pragma unroll
-    for (int j = 0; j < BN / 32; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
+        for (int i = 0; i < MI; ++i) {
             const int f = f0 + mrow + i * 16 + r, k = k0 + nbase + j * 16 + c4;
             if (f < 2 * d.outp) store4(o + (int64_t)f * d.in + k, acc[j][i], d.in - k, d.in % 4 == 0);
         }
@@ -323,16 +337,22 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblo
         return;
     }
     b -= xblocks;
-    if (b < wblocks) {
-        const int64_t size = (int64_t)2 * d.outp * d.in, i = ((int64_t)b * 256 + threadIdx.x);
-        if (i >= size) return;
-        const int f = (int)(i / d.in), k = (int)(i % d.in), half = f >= d.outp, ff = f - half * d.outp;
-        if (ff >= d.out) return;
-        float s = 0.f;
-#pragma unroll 8
-        for (int p = 0; p < splits; ++p) s += wpart[p * size + i];
+    __shared__ f32x4 red4[4][64];
+    if (b < wblocks) {  // 256 places a workgroup, four a load, four threads share the parts (whole f32x4: size is a multiple of 8)
+        const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+        const int64_t size = (int64_t)2 * d.outp * d.in, i = (int64_t)b * 256 + lane * 4;
+        f32x4 s = {0, 0, 0, 0};
+        if (i < size) {
+#pragma unroll 4
+            for (int p = q; p < splits; p += 4) s += *reinterpret_cast<const f32x4*>(wpart + p * size + i);
+        }
+        red4[q][lane] = s;
+        __syncthreads();
+        const int64_t at = (int64_t)b * 256 + threadIdx.x;
+        if (at >= size) return;
+        const int f = (int)(at / d.in), k = (int)(at % d.in), half = f >= d.outp, ff = f - half * d.outp, l = threadIdx.x >> 2, e = threadIdx.x & 3;
         T* o = half ? dwu : dwg;
-        if (o != nullptr) o[(int64_t)ff * d.in + k] = (T)s;
+        if (ff < d.out && o != nullptr) o[(int64_t)ff * d.in + k] = (T)(red4[0][l][e] + red4[1][l][e] + red4[2][l][e] + red4[3][l][e]);
         return;
     }
     b -= wblocks;
@@ -355,18 +375,27 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblo
     }
 }
 
-// Tiles of an output of m x n: 128 x 128 where they fill the 256 CUs, else 64 x 64, else 32 x 64; guarded loads: 32 x 64.
-enum { TILE_128, TILE_64, TILE_32, TILE_GUARDED };
-static const int TILE_M[4] = {128, 64, 32, 32}, TILE_N[4] = {128, 64, 64, 64};
+// Tiles of an output.  A tile of 128 x 128 draws 16 KB from L2 for 16 instructions of each of its four waves, and that is what
+// bounds the long products: 65536 x 256 -> 2 x 1024 in bf16, the same time with two, three or four tiles under way.  So the
+// 16-bit types take 256 x 256 (dx 106 -> 83 us, dW 106 -> 91) or, where an epilogue wants a second workgroup on the CU,
+// 256 x 128 (forward 127 -> 113; the backward's first launch has too many values in hand for eight waves: 282 against 201),
+// as long as their rounds over the chip and their edges leave little idle.  Else 128 x 128 where they fill the 256 CUs, else
+// 64 x 64, else 32 x 64; guarded loads: 32 x 64.
+enum { TILE_256, TILE_TALL, TILE_128, TILE_64, TILE_32, TILE_GUARDED };
+static const int TILE_M[6] = {256, 256, 128, 64, 32, 32}, TILE_N[6] = {256, 128, 128, 64, 64, 64};
 static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
-static int gated_tile(int64_t m, int64_t n, int64_t times, bool guarded) {
-    if (guarded) return TILE_GUARDED;
-    for (int t = TILE_128; t < TILE_32; ++t)
-        if (times * div_up(m, TILE_M[t]) * div_up(n, TILE_N[t]) >= 256) return t;
-    return TILE_32;
+static int64_t gated_tiles(int64_t m, int64_t n, int t) { return (int64_t)div_up(m, TILE_M[t]) * div_up(n, TILE_N[t]); }
+static bool gated_fills(int64_t m, int64_t n, int t, int64_t times) {
+    const int64_t tiles = gated_tiles(m, n, t), slots = t == TILE_256 ? 256 : 512, wgs = tiles * times;
+    if (t > TILE_TALL) return wgs >= 256;
+    return 5 * wgs >= 4 * slots * div_up(wgs, slots) && 4 * tiles * TILE_M[t] * TILE_N[t] <= 5 * m * n;
 }
 #define GATED_BY_TILE(tile, BM, BN, ...)                                               \
     switch (tile) {                                                                    \
+        case TILE_256:                                                                 \
+            if constexpr (sizeof(T) == 2) { constexpr int BM = 256, BN = 256; __VA_ARGS__; } break; \
+        case TILE_TALL:                                                                \
+            if constexpr (sizeof(T) == 2) { constexpr int BM = 256, BN = 128; __VA_ARGS__; } break; \
         case TILE_128: { constexpr int BM = 128, BN = 128; __VA_ARGS__; } break;       \
         case TILE_64: { constexpr int BM = 64, BN = 64; __VA_ARGS__; } break;          \
         case TILE_32: { constexpr int BM = 32, BN = 64; __VA_ARGS__; } break;          \
@@ -381,38 +410,45 @@ struct GatedScratch {  // bytes from the start
     int planes;                        // of D
 };
 // Rows that no 16-byte load fits are copied to rows that it does where the products are long enough to pay for the launch;
-// below, their tiles come in by narrower, guarded loads (2 rows of 19 -> 177 f32 values, forward: 6 us against 9; 2066 of
-// 965 -> 1292 f16, forward and backward: 570 us against 110).
+// below, their tiles come in by narrower, guarded loads (2066 rows of 965 -> 1292 f16, forward and backward: 572 us by guarded
+// loads, 197 with the copies).
 static bool gated_packed(int rows, int in, int out) { return (int64_t)rows * in * out >= (1 << 22); }
 static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fast, bool bwd) {
     GatedScratch s = {};
     const size_t outp = ((size_t)out + 7) / 8 * 8, inp = ((size_t)in + 7) / 8 * 8, es = dtype == TSD_F32 ? 4 : 2;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const bool guarded = !fast && !gated_packed(rows, in, out);
-    s.tile = gated_tile(rows, 2 * outp, 1, guarded);
+    const int first = guarded ? TILE_GUARDED : es == 4 || bwd ? TILE_128 : TILE_TALL;
+    for (s.tile = first; s.tile < TILE_32 && !gated_fills(rows, 2 * outp, s.tile, 1);) ++s.tile;
     s.mtiles = div_up(rows, TILE_M[s.tile]);
     s.planes = es == 2 && s.tile >= TILE_32 && (int64_t)rows * 2 * outp <= (1 << 18) ? 2 : 1;
     const size_t width = s.planes * 2 * outp;
-    // dW: the rows in shares of at least 256, about two workgroups a CU
-    const int most = div_up(rows, 256);
-    s.wtile = gated_tile(2 * outp, in, most, guarded);
-    if (s.wtile == TILE_32) s.wtile = TILE_64;
-    const int tiles = div_up(2 * outp, TILE_M[s.wtile]) * div_up(in, TILE_N[s.wtile]);
-    int n = div_up(512, tiles);
-    n = n < most ? n : most;
-    n = n < 1 ? 1 : n;
+    // dW: the rows in shares: one workgroup a CU of the largest tiles, 2048 rows each at least (below, the parts cost what the
+    // tile saves: 16300 x 250 -> 2 x 600, 320 rows each: 48 + 27 us against 45 + 16); else about two, of at least 256 rows
+    const int most = div_up(rows, 256), large = guarded ? TILE_GUARDED : es == 4 ? TILE_128 : TILE_256;
+    int n = 0;
+    for (s.wtile = large;; s.wtile += s.wtile == TILE_256 ? 2 : 1) {
+        const int64_t tiles = gated_tiles(2 * outp, in, s.wtile);
+        n = s.wtile == TILE_256 ? (int)(256 / tiles) : (int)((511 + tiles) / tiles);
+        n = n < most ? n : most;
+        n = n < 1 ? 1 : n;
+        if (s.wtile == TILE_GUARDED || s.wtile == TILE_64) break;
+        if (s.wtile == TILE_256 ? gated_fills(2 * outp, in, s.wtile, n) && rows / n >= 2048 : gated_fills(2 * outp, in, s.wtile, most)) break;
+    }
     s.rows_a_split = div_up(div_up(rows > 0 ? rows : 1, n), GEMM_K) * GEMM_K;
     s.splits = div_up(rows, s.rows_a_split);
-    // dx: the largest tiles that fill the chip with shares of at least eight steps of the contraction
+    // dx: the largest tiles that fill the chip; where fewer than 128 of them are to do, with shares of at least eight steps of
+    // the contraction (16300 x 250 -> 2 x 600, 256 tiles: in two shares 33 + 16 us with the sum of the parts, in one 25 + 7;
+    // 10000 x 256 -> 2 x 512: 15 + 14 us, 64 x 64 tiles without shares 16 + 7)
     const int steps = div_up(width, GEMM_K);
-    for (s.xtile = guarded ? TILE_GUARDED : TILE_128;; ++s.xtile) {
-        const int t = div_up(rows, TILE_M[s.xtile]) * div_up(in, TILE_N[s.xtile]);
-        int x = div_up(512, t > 0 ? t : 1);
+    for (s.xtile = large;; ++s.xtile) {
+        const int64_t t = gated_tiles(rows, in, s.xtile);
+        int x = t >= 128 || s.xtile <= TILE_TALL ? 1 : (int)(512 / (t > 0 ? t : 1));
         x = x < steps / 8 ? x : steps / 8;
         x = x < 1 ? 1 : x;
         s.share = div_up(steps, x) * GEMM_K;
         s.xsplits = div_up(width, s.share);
-        if (s.xtile >= TILE_32 || (int64_t)t * s.xsplits >= 256) break;
+        if (s.xtile >= TILE_32 || gated_fills(rows, in, s.xtile, s.xsplits)) break;
     }
     s.pack = 0;
     s.D = up(!fast && gated_packed(rows, in, out) ? ((size_t)rows + 2 * (size_t)out) * inp * es : 0);
@@ -490,7 +526,7 @@ static int gated_first(GatedDims d, const void* x, const void* wg, const void* w
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int ft = div_up(BWD ? d.outp : d.out, BN / 2), mt = div_up(d.rows, BM);
-    hipLaunchKernelGGL(k, dim3(tile_grid(mt, ft)), dim3(GEMM_WG), lds, st, d, ft, mt, (const T*)x, (const T*)wg, (const T*)wu,
+    hipLaunchKernelGGL(k, dim3(tile_grid(mt, ft)), dim3(gemm_wg(BM, BN)), lds, st, d, ft, mt, (const T*)x, (const T*)wg, (const T*)wu,
                        (const T*)bg, (const T*)bu, (const T*)dh, (T*)h, (T*)D, part);
     TSD_LAUNCH_CHECK("gated_linear");
     return TSD_OK;
@@ -499,12 +535,12 @@ template <class T, int BM, int BN, bool FAST>
 static int gated_dx(GatedDims d, const GatedScratch& s, const T* D, const void* wg, const void* wu, void* dx, float* part,
                     hipStream_t st) {
     static DeviceOnce once;
-    constexpr int lds = gated_lds<T, BM, BN, FAST>(OutTile<T, BM, BN>::BYTES);
+    constexpr int lds = gated_lds<T, BM, BN, FAST>(OutTile<T, BM, BN, 64>::BYTES);
     auto k = gated_dx_kernel<T, BM, BN, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), mt = div_up(d.rows, BM);
-    hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt), s.xsplits), dim3(GEMM_WG), lds, st, d, kt, mt, D, (const T*)wg,
+    hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt), s.xsplits), dim3(gemm_wg(BM, BN)), lds, st, d, kt, mt, D, (const T*)wg,
                        (const T*)wu, (T*)dx, s.share, part);
     TSD_LAUNCH_CHECK("gated_dx");
     return TSD_OK;
@@ -517,12 +553,14 @@ static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* 
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), ft = div_up(2 * d.outp, BM);
-    hipLaunchKernelGGL(k, dim3(kt * ft, s.splits), dim3(GEMM_WG), lds, st, d, kt, s.rows_a_split, D, (const T*)x, wpart);
+    hipLaunchKernelGGL(k, dim3(kt * ft, s.splits), dim3(gemm_wg(BM, BN)), lds, st, d, kt, s.rows_a_split, D, (const T*)x, wpart);
     TSD_LAUNCH_CHECK("gated_dw");
     return TSD_OK;
 }
 template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
-    GATED_BY_TILE(tile, BM, BN, { return gated_first<T, BM, BN, true, BWD>(d, a...); });
+    GATED_BY_TILE(tile, BM, BN, {
+        if constexpr (BM <= 128 || (BN <= 128 && !BWD)) return gated_first<T, BM, BN, true, BWD>(d, a...);
+    });
     return gated_first<T, 32, 64, false, BWD>(d, a...);
 }
 
