@@ -112,11 +112,10 @@ template <class T, int BM, int BN> constexpr int gated_behind(bool bwd) {
 }
 
 template <class T, int BM, int BN, bool FAST, bool BWD>
-__global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 : 3) void gated_kernel(GatedDims d, int ftiles, int mtiles, const T* __restrict__ x,
-                                                        const T* __restrict__ wg, const T* __restrict__ wu,
-                                                        const T* __restrict__ bg, const T* __restrict__ bu,
-                                                        const T* __restrict__ dh, T* __restrict__ h, T* __restrict__ D,
-                                                        float* __restrict__ part) {
+__global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 : 3) void gated_kernel(
+    GatedDims d, int ftiles, int mtiles, const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
+    const T* __restrict__ bg, const T* __restrict__ bu, const T* __restrict__ dh, T* __restrict__ h, T* __restrict__ D,
+    float* __restrict__ part) {
     extern __shared__ __align__(16) char lds[];
     constexpr int WG = gemm_wg(BM, BN), WM = gemm_waves(BM), WN = gemm_waves(BN);
     constexpr int FT = BN / 2, TN = FT / WN / 16, TM = BM / WM / 16;  // columns a tile; gate (and up) subtiles, row subtiles of a wave
@@ -350,7 +349,8 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblo
         __syncthreads();
         const int64_t at = (int64_t)b * 256 + threadIdx.x;
         if (at >= size) return;
-        const int f = (int)(at / d.in), k = (int)(at % d.in), half = f >= d.outp, ff = f - half * d.outp, l = threadIdx.x >> 2, e = threadIdx.x & 3;
+        const int f = (int)(at / d.in), k = (int)(at % d.in), half = f >= d.outp, ff = f - half * d.outp;
+        const int l = threadIdx.x >> 2, e = threadIdx.x & 3;
         T* o = half ? dwu : dwg;
         if (ff < d.out && o != nullptr) o[(int64_t)ff * d.in + k] = (T)(red4[0][l][e] + red4[1][l][e] + red4[2][l][e] + red4[3][l][e]);
         return;
@@ -433,7 +433,9 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
         n = n < most ? n : most;
         n = n < 1 ? 1 : n;
         if (s.wtile == TILE_GUARDED || s.wtile == TILE_64) break;
-        if (s.wtile == TILE_256 ? gated_fills(2 * outp, in, s.wtile, n) && rows / n >= 2048 : gated_fills(2 * outp, in, s.wtile, most)) break;
+        if (s.wtile == TILE_256 ? gated_fills(2 * outp, in, s.wtile, n) && rows / n >= 2048
+                                : gated_fills(2 * outp, in, s.wtile, most))
+            break;
     }
     s.rows_a_split = div_up(div_up(rows > 0 ? rows : 1, n), GEMM_K) * GEMM_K;
     s.splits = div_up(rows, s.rows_a_split);
