@@ -426,6 +426,30 @@ def test_the_same_bits_every_time_and_on_other_streams(dtype):
             assert all(torch.equal(a, b) for a, b in zip(first, g))
 
 
+def test_calls_of_several_threads_at_once():
+    import threading
+    want = [[f(*leaves) for f, leaves, _ in three(40 + k, n=60 + 10 * k)] for k in range(4)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def go(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                for (f, leaves, d), w in zip(three(40 + k, n=60 + 10 * k), want[k]):
+                    y = f(*leaves)
+                    torch.autograd.grad(y, leaves, d)
+                    if not torch.equal(y, w):
+                        wrong.append(k)
+
+    threads = [threading.Thread(target=go, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_captured_forward_and_backward_replay(dtype):
     for f, leaves, d in three(40, dtype=dtype):

@@ -51,6 +51,10 @@ int check_hip(hipError_t e, const char* what);
 // may drive several GPUs): first_on_current_device() is true exactly once per device id for each instance.
 struct DeviceOnce {
     std::atomic<uint64_t> mask{0};
+    bool done_on_current_device() const {
+        int d = 0;
+        return hipGetDevice(&d) == hipSuccess && (mask.load() >> (d & 63) & 1);
+    }
     bool first_on_current_device() {
         int d = 0;
         if (hipGetDevice(&d) != hipSuccess) return true;
@@ -60,9 +64,11 @@ struct DeviceOnce {
 };
 template <typename K>
 static inline int allow_lds(K kernel, size_t bytes, DeviceOnce& once) {
-    if (bytes > 48 * 1024 && once.first_on_current_device())
+    if (bytes > 48 * 1024 && !once.done_on_current_device()) {  // (several threads may come here: each sets it before it launches)
         TSD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        once.first_on_current_device();
+    }
     return TSD_OK;
 }
 

@@ -15,7 +15,7 @@
 //   bf16, 65536 x 256 -> 2 x 1024: forward 119 us (580 TFLOP/s, h and x are 170 MB of it), first of the backward 200 us (it
 //   writes D, 268 MB, and reads dh, 134 MB), dx 81 us (850 TFLOP/s), dW 91 us (755 TFLOP/s), sums 14 us.  Bound by what a CU
 //   draws from L2 (about 10 TB/s over the chip), the two first ones by that and by memory.
-//   f32, 3600 x 256 -> 2 x 1024: 30, 38, 31, 30 and 13 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
+//   f32, 3600 x 256 -> 2 x 1024: 30, 38, 31, 30 and 11 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
 //   f32, 17 x 256 -> 2 x 512, forward: 7 us, of which launching and one pass through memory are nearly all.
 #include <type_traits>
 
