@@ -12,10 +12,10 @@
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
 //
 // Measured (GPU time a launch; each product is 4 rows in out operations):
-//   bf16, 65536 x 256 -> 2 x 1024: forward 119 us (580 TFLOP/s, h and x are 170 MB of it), first of the backward 200 us (it
-//   writes D, 268 MB, and reads dh, 134 MB), dx 81 us (850 TFLOP/s), dW 91 us (755 TFLOP/s), sums 14 us.  Bound by what a CU
+//   bf16, 65536 x 256 -> 2 x 1024: forward 119 us (580 TFLOP/s, h and x are 170 MB of it), first of the backward 180 us (it
+//   writes D, 268 MB, and reads dh, 134 MB), dx 82 us (840 TFLOP/s), dW 92 us (747 TFLOP/s), sums 13 us.  Bound by what a CU
 //   draws from L2 (about 10 TB/s over the chip), the two first ones by that and by memory.
-//   f32, 3600 x 256 -> 2 x 1024: 30, 38, 31, 30 and 11 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
+//   f32, 3600 x 256 -> 2 x 1024: 30, 34, 31, 30 and 11 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
 //   f32, 17 x 256 -> 2 x 512, forward: 7 us, of which launching and one pass through memory are nearly all.
 #include <type_traits>
 
@@ -39,7 +39,18 @@ template <int KIND> __device__ __forceinline__ float act_slope(int kind, float g
     if constexpr (KIND >= 0) kind = KIND;
     if (kind == 2) return g > 0.f ? 1.f : 0.f;
     const float s = sigmoid(g);
-    return kind == 0 ? s * (1.f + g * (1.f - s)) : s;
+    return kind == 0 ? s + g * s * (1.f - s) : s;
+}
+
+// sum over the 16 lanes l / 16 * 16 ..: neighbours, pairs, halves of 8, halves of 16, inside of the vector pipe
+template <int CTRL> __device__ __forceinline__ float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float over_16(float v) {
+    v += from_lane<0xB1>(v);   // quad_perm 1 0 3 2
+    v += from_lane<0x4E>(v);   // quad_perm 2 3 0 1
+    v += from_lane<0x141>(v);  // row_half_mirror
+    return v + from_lane<0x140>(v);  // row_mirror
 }
 
 struct GatedDims {
@@ -129,6 +140,9 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
     const RowOperand<T, false> ms = {x, x, d.ldx, d.rows, d.inw, m0, BM, 0, d.xvw};
     f32x4 acc[2 * TN][TM];
     const int r = lane & 15, c4 = (lane >> 4) * 4;
+    Raw<T> dhr[BWD ? Out::U : 1];
+    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.inw, mrow,
+                               [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     f32x4 vbg[TN], vbu[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -137,25 +151,22 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
         vbg[j] = bg != nullptr ? load4(bg + f, nf, d.bvec) : zero;
         vbu[j] = bu != nullptr ? load4(bu + f, nf, d.bvec) : zero;
     }
-    Raw<T> dhr[BWD ? Out::U : 1];
-    if constexpr (BWD) Out::fetch(dhr, dh + (int64_t)m0 * d.lddh + f0, d.lddh, d.rows - m0, d.out - f0, d.dhvw);
-    gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.inw, mrow,
-                               [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
     char* second = lds + Out::BYTES;
     constexpr bool REST = BWD && gated_rest<T, BM>();
     float* red = reinterpret_cast<float*>(lds + (REST ? 4 : 2) * Out::BYTES);  // [WM][2][FT] column sums
     if constexpr (BWD) {
+        Out::fetch(dhr, dh + (int64_t)m0 * d.lddh + f0, d.lddh, d.rows - m0, d.out - f0, d.dhvw);
         Out::keep(dhr, lds);
         __syncthreads();
     }
-    // (swish has code of its own: with all kinds' in every place of the unrolled loops the code outgrows its cache)
+    const bool whole = m0 + BM <= d.rows && f0 + FT <= d.out;
+    // (a tile without edges needs no looks at them; swish has code of its own: with all kinds' in every place of the unrolled loops the code outgrows its cache)
     auto epilogue = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int fl = nbase + j * 16 + c4, f = f0 + fl, nf = d.out - f;
-            const f32x4 zero = {0, 0, 0, 0};
-            f32x4 sg = zero, su = zero;
+            f32x4 sg = {0, 0, 0, 0}, su = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int ml = mrow + i * 16 + r;
@@ -168,14 +179,20 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
                     store4(o, v, 4, true);
                 } else {  // dh's place takes dg; columns and rows outside hold zeros, whatever g and u are there
                     const f32x4 v = load4(o, 4, true);
-                    const bool real = m0 + ml < d.rows;
-                    f32x4 og = zero, ou = zero;
+                    f32x4 og, ou;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (real && e < nf) {
-                            ou[e] = v[e] * act_value<KIND>(d.kind, g[e]);
-                            og[e] = v[e] * u[e] * act_slope<KIND>(d.kind, g[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        ou[e] = v[e] * act_value<KIND>(d.kind, g[e]);
+                        og[e] = v[e] * u[e] * act_slope<KIND>(d.kind, g[e]);
+                    }
+                    if (!whole) {
+                        const bool real = m0 + ml < d.rows;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            ou[e] = real && e < nf ? ou[e] : 0.f;
+                            og[e] = real && e < nf ? og[e] : 0.f;
                         }
+                    }
                     store4(o, og, 4, true);
                     store4(Out::at(second, ml, fl), ou, 4, true);
                     if constexpr (REST) {
@@ -193,16 +210,14 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
                 }
             }
             if constexpr (BWD) {
+                if (part != nullptr) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                    for (int s = 1; s < 16; s *= 2) {
-                        sg[e] += __shfl_xor(sg[e], s, 64);
-                        su[e] += __shfl_xor(su[e], s, 64);
-                    }
-                    if (r == 0) {
-                        red[(wm * 2) * FT + fl + e] = sg[e];
-                        red[(wm * 2 + 1) * FT + fl + e] = su[e];
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = over_16(sg[e]), b = over_16(su[e]);
+                        if (r == 0) {
+                            red[(wm * 2) * FT + fl + e] = a;
+                            red[(wm * 2 + 1) * FT + fl + e] = b;
+                        }
                     }
                 }
             }
@@ -382,9 +397,9 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(GatedDims d, int xblo
 // Tiles of an output.  A tile of 128 x 128 draws 16 KB from L2 for 16 instructions of each of its four waves, and that is what
 // bounds the long products: 65536 x 256 -> 2 x 1024 in bf16, the same time with two, three or four tiles under way.  So the
 // 16-bit types take 256 x 256 (dx 106 -> 83 us, dW 106 -> 91) or, where an epilogue wants a second workgroup on the CU,
-// 256 x 128 (forward 127 -> 113; the backward's first launch has too many values in hand for eight waves: 282 against 201),
-// as long as their rounds over the chip and their edges leave little idle.  Else 128 x 128 where they fill the 256 CUs, else
-// 64 x 64, else 32 x 64; guarded loads: 32 x 64.
+// 256 x 128 (forward 127 -> 119; the backward's first launch 188 -> 180, with dh and the biases fetched behind the product:
+// eight waves have no registers for them before), as long as their rounds over the chip and their edges leave little idle.
+// Else 128 x 128 where they fill the 256 CUs, else 64 x 64, else 32 x 64; guarded loads: 32 x 64.
 enum { TILE_256, TILE_TALL, TILE_128, TILE_64, TILE_32, TILE_GUARDED };
 static const int TILE_M[6] = {256, 256, 128, 64, 32, 32}, TILE_N[6] = {256, 128, 128, 64, 64, 64};
 static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -422,7 +437,7 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
     const size_t outp = ((size_t)out + 7) / 8 * 8, inp = ((size_t)in + 7) / 8 * 8, es = dtype == TSD_F32 ? 4 : 2;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const bool guarded = !fast && !gated_packed(rows, in, out);
-    const int first = guarded ? TILE_GUARDED : es == 4 || bwd ? TILE_128 : TILE_TALL;
+    const int first = guarded ? TILE_GUARDED : es == 4 ? TILE_128 : TILE_TALL;
     for (s.tile = first; s.tile < TILE_32 && !gated_fills(rows, 2 * outp, s.tile, 1);) ++s.tile;
     s.mtiles = div_up(rows, TILE_M[s.tile]);
     s.planes = es == 2 && s.tile >= TILE_32 && (int64_t)rows * 2 * outp <= (1 << 18) ? 2 : 1;
@@ -565,7 +580,7 @@ static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* 
 }
 template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
     GATED_BY_TILE(tile, BM, BN, {
-        if constexpr (BM <= 128 || (BN <= 128 && !BWD)) return gated_first<T, BM, BN, true, BWD>(d, a...);
+        if constexpr (BN <= 128) return gated_first<T, BM, BN, true, BWD>(d, a...);
     });
     return gated_first<T, 32, 64, false, BWD>(d, a...);
 }
