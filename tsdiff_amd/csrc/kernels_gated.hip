@@ -160,7 +160,8 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
         __syncthreads();
     }
     const bool whole = m0 + BM <= d.rows && f0 + FT <= d.out;
-    // (a tile without edges needs no looks at them; swish has code of its own: with all kinds' in every place of the unrolled loops the code outgrows its cache)
+    // (a tile without edges needs no looks at them; swish has code of its own: with all kinds' in every place of the unrolled
+    // loops the code outgrows its cache)
     auto epilogue = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;
 #pragma unroll
