@@ -6,7 +6,8 @@ float32, bfloat16 and float16 CUDA tensors; one call's tensors share their type 
 fp32 and an output is rounded once.  Work is queued on the current stream of the tensors' device; nothing waits for the
 GPU, no state is kept between calls, and the results of a call are the same bits every time.  Calls may be captured into
 a graph; to capture a backward pass, give the captured forward leaves of its own (x.detach().requires_grad_()), since
-autograd ties a leaf's accumulation to the stream that used it first.  First derivatives only.
+autograd ties a leaf's accumulation to the stream that used it first.  First derivatives in reverse mode only: a second
+derivative and a forward-mode tangent (also under no_grad) raise.
 """
 import os
 

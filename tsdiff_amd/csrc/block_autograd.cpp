@@ -65,6 +65,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// A tangent (forward-mode differentiation, which works under no_grad too) would be lost where raw pointers are handed on, and
+// a lost tangent counts as zero
+void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(/*level=*/0).defined()) throw Unsupported(c10::str(name, " has no forward-mode derivative"));
+}
 // A missing argument is no edge of the graph: the edge of argument `k` is the number of tensors in front of it
 Opt maybe(const Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
 Tensor given(const Opt& t) { return t.has_value() ? *t : Tensor(); }
@@ -113,6 +119,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &stats = saved[3];
         if (!grads[0].defined()) return variable_list(4);
+        no_tangents("layer_norm", {&grads[0]});
         c10::DeviceGuard guard(x.device());
         const Tensor dy = rows_of(grads[0].detach());
         const int32_t rows = (int32_t)x.size(0), dim = (int32_t)x.size(1);
@@ -131,6 +138,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps) {
+    const Tensor w0 = given(weight), b0 = given(bias);
+    no_tangents("layer_norm", {&x, &w0, &b0});
     if (x.dim() < 1 || x.size(-1) < 1) refuse("layer_norm: x has shape ", x.sizes());
     const Tensor w = dense(weight), b = dense(bias);
     for (const Tensor* t : {&w, &b})
@@ -167,6 +176,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &x = s[0], &wg = s[1], &wu = s[2], &bg = s[3], &bu = s[4];
         if (!grads[0].defined()) return variable_list(6);
+        no_tangents("gated_linear", {&grads[0]});
         c10::DeviceGuard guard(x.device());
         const Tensor dh = rows_of(grads[0].detach());
         const int dtype = dtype_of(x.scalar_type());
@@ -187,6 +197,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Opt& b_gate, const Opt& b_up,
                     const std::string& act) {
+    const Tensor bg0 = given(b_gate), bu0 = given(b_up);
+    no_tangents("gated_linear", {&x, &w_gate, &w_up, &bg0, &bu0});
     const int64_t kind = act == "swish" ? 0 : act == "ssp" ? 1 : act == "ReLU" ? 2 : act == "Softplus" ? 3 : -1;  // tsd_act_fwd's
     if (kind < 0) throw Unsupported("gated_linear: activation '" + act + "'");
     if (w_gate.dim() != 2 || w_gate.sizes() != w_up.sizes() || w_gate.numel() == 0 || x.dim() < 1 || x.size(-1) != w_gate.size(1))
@@ -260,6 +272,7 @@ struct GraphAttention : torch::autograd::Function<GraphAttention> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2], &out = s[6], &lse = s[7];
         if (!grads[0].defined()) return variable_list(7);
+        no_tangents("graph_attention", {&grads[0]});
         c10::DeviceGuard guard(q.device());
         const Tensor dout = heads_of(grads[0].detach());
         const tsd_attention a = attention_args(q, k, v, s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
@@ -276,6 +289,7 @@ struct GraphAttention : torch::autograd::Function<GraphAttention> {
 Tensor graph_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& graph_ptr, const Opt& key_ptr,
                        const Opt& key_mask, std::optional<double> scale) {
     const char* name = "graph_attention";
+    no_tangents(name, {&q, &k, &v});
     for (const Tensor* t : {&q, &k, &v})
         if (t->dim() != 3) refuse(name, ": shape ", t->sizes(), ", [nodes, heads, dim] expected");
     if (k.sizes() != v.sizes() || q.size(2) != k.size(2) || q.size(1) < 1 || q.size(2) < 1 || k.size(1) < 1 ||
