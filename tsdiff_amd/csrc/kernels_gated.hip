@@ -9,6 +9,7 @@
 // rounding of an intermediate, since D is the next two products' matrix operand; a small D (at most 2^18 values of 16 bits) is
 // written with what the rounding left as a second half of twice the width, which the products go over too, since sums of few
 // terms show one rounding more than large ones, and time is no matter there -- with each row tile's column sums in fp32;
+// f16 gradients put a launch in front, by which D lies in the middle of f16's range whatever the size of dh (GatedMaxes);
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
 //
 // Measured (GPU time a launch; each product is 4 rows in out operations):
@@ -61,6 +62,63 @@ struct GatedDims {
     int kind;
     bool bvec;  // both biases: four values a load
     int xvw, wvw, dhvw, hvw, dxvw;  // values a load or store of x, the weights, dh, h, dx may take
+};
+
+// f16: D = [dg | du] times a power of two s, by which neither small gradients fall among the subnormal numbers (steps of 2^-24)
+// nor large products beyond 65504 (4096 x 256 -> 2 x 512, dh of 1e-5: dW off by 1.8e-3 without s, by 2.9e-4 with it, as for dh
+// of 1; rounding dW alone: 2.1e-4).  One s for all of D, since its rows and its columns are both summed over; it takes the bound
+//   |D| <= max |dh| (in max |x| max |W| + max |b| + 1) 1.25   (|a'| < 1.1, |a(g)| < |g| + 0.7, the rest is room for roundings)
+// into 2^14 .. 2^15.  The bound lies above D's ordinary values by about 16 sqrt(in), which leaves them 14 to 26 powers of two
+// above the subnormal numbers.  Values that are not finite are left out: their rows are lost either way.
+template <class T> constexpr bool gated_scaled() { return std::is_same<T, f16>::value; }
+struct GatedScale {
+    float by, undo;
+};
+using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
+constexpr int GATED_MAX_WG = 1024, GATED_MAX_WGS = 256;
+struct GatedMax {  // bits of f16 values, which compare like the values: of x and the weights, of the biases and dh
+    u16x2 xw, bd;
+};
+__device__ __forceinline__ u16x2 larger(u16x2 a, u16x2 b) { return __builtin_elementwise_max(a, b); }
+template <int CTRL> __device__ __forceinline__ u16x2 from_lane(u16x2 v) {
+    return __builtin_bit_cast(u16x2, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ u16x2 largest_of_wave(u16x2 v) {
+    v = larger(v, from_lane<0xB1>(v));  // neighbours, pairs, halves of 8 and of 16 lanes, as over_16
+    v = larger(v, from_lane<0x4E>(v));
+    v = larger(v, from_lane<0x141>(v));
+    v = larger(v, from_lane<0x140>(v));
+    uint32_t a = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t x = r[0], y = r[1];
+    a = __builtin_bit_cast(uint32_t, larger(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
+    const auto q = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    const uint32_t z = q[0], w = q[1];
+    return larger(__builtin_bit_cast(u16x2, z), __builtin_bit_cast(u16x2, w));
+}
+// (the list is asked for where other loads are waited for too)
+template <class T> struct GatedMaxes {
+    u32x4 raw[2];
+    __device__ __forceinline__ void load(const GatedMax* __restrict__ maxes) {
+        if constexpr (gated_scaled<T>()) {
+            const u32x4* p = reinterpret_cast<const u32x4*>(maxes) + 2 * (threadIdx.x & 63);
+            static_assert(GATED_MAX_WGS == 4 * 64, "two loads a lane");
+            raw[0] = p[0];
+            raw[1] = p[1];
+        }
+    }
+    __device__ __forceinline__ GatedScale scale(int in) const {
+        if constexpr (!gated_scaled<T>()) return {1.f, 1.f};
+        auto two = [&](int i, int j) { return __builtin_bit_cast(u16x2, (uint32_t)raw[i][j]); };
+        const u16x2 xw = largest_of_wave(larger(larger(two(0, 0), two(0, 2)), larger(two(1, 0), two(1, 2))));
+        const u16x2 bd = largest_of_wave(larger(larger(two(0, 1), two(0, 3)), larger(two(1, 1), two(1, 3))));
+        auto value = [](unsigned short b) { return (float)__builtin_bit_cast(f16, b); };
+        // 2^-24 .. 2^70, or 0
+        const float bound = value(bd[1]) * 1.25f * ((float)in * value(xw[0]) * value(xw[1]) + value(bd[0]) + 1.f);
+        const int e = (int)(__builtin_bit_cast(uint32_t, bound) >> 23);  // 2^(e - 127) <= bound
+        const int to = bound > 0.f ? 127 + 14 + 127 - e : 127;
+        return {__builtin_bit_cast(float, (uint32_t)to << 23), __builtin_bit_cast(float, (uint32_t)(254 - to) << 23)};
+    }
 };
 
 // A tile of BM rows x BC columns in LDS on its way to (from) memory, so that neighbouring lanes touch neighbouring bytes
@@ -126,7 +184,7 @@ template <class T, int BM, int BN, bool FAST, bool BWD>
 __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 : 3) void gated_kernel(
     GatedDims d, int ftiles, int mtiles, const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
     const T* __restrict__ bg, const T* __restrict__ bu, const T* __restrict__ dh, T* __restrict__ h, T* __restrict__ D,
-    float* __restrict__ part) {
+    float* __restrict__ part, const GatedMax* __restrict__ maxes) {
     extern __shared__ __align__(16) char lds[];
     constexpr int WG = gemm_wg(BM, BN), WM = gemm_waves(BM), WN = gemm_waves(BN);
     constexpr int FT = BN / 2, TN = FT / WN / 16, TM = BM / WM / 16;  // columns a tile; gate (and up) subtiles, row subtiles of a wave
@@ -143,6 +201,8 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
     Raw<T> dhr[BWD ? Out::U : 1];
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.inw, mrow,
                                [&](int j) { return j < TN ? nbase + j * 16 : FT + nbase + (j - TN) * 16; }, acc);
+    GatedMaxes<T> most;
+    if constexpr (BWD) most.load(maxes);
     f32x4 vbg[TN], vbu[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -159,6 +219,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
         Out::keep(dhr, lds);
         __syncthreads();
     }
+    const GatedScale scale = BWD ? most.scale(d.in) : GatedScale{1.f, 1.f};
     const bool whole = m0 + BM <= d.rows && f0 + FT <= d.out;
     // (a tile without edges needs no looks at them; swish has code of its own: with all kinds' in every place of the unrolled
     // loops the code outgrows its cache)
@@ -194,6 +255,12 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
                             og[e] = real && e < nf ? og[e] : 0.f;
                         }
                     }
+                    sg += og;
+                    su += ou;
+                    if constexpr (gated_scaled<T>()) {
+                        og *= scale.by;
+                        ou *= scale.by;
+                    }
                     store4(o, og, 4, true);
                     store4(Out::at(second, ml, fl), ou, 4, true);
                     if constexpr (REST) {
@@ -206,8 +273,6 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
                         store4(Out::at(second + Out::BYTES, ml, fl), rg, 4, true);
                         store4(Out::at(second + 2 * Out::BYTES, ml, fl), ru, 4, true);
                     }
-                    sg += og;
-                    su += ou;
                 }
             }
             if constexpr (BWD) {
@@ -249,11 +314,25 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
     }
 }
 
+template <class T, int NJ, int MI>
+__device__ __forceinline__ void gated_undo(f32x4 (&acc)[NJ][MI], const GatedMax* __restrict__ maxes, int in) {
+    if constexpr (gated_scaled<T>()) {
+        GatedMaxes<T> most;
+        most.load(maxes);
+        const GatedScale scale = most.scale(in);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[j][i] *= scale.undo;
+    }
+}
+
 // dx[m][k] = sum over f < 2 outp of D[m][f] [Wg; Wu][f][k]; several shares of f (blockIdx.y): their sums in fp32 to part
 template <class T, int BM, int BN, bool FAST>
 __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dx_kernel(GatedDims d, int ktiles, int mtiles, const T* __restrict__ D,
                                                            const T* __restrict__ wg, const T* __restrict__ wu,
-                                                           T* __restrict__ dx, int share, float* __restrict__ part) {
+                                                           T* __restrict__ dx, int share, float* __restrict__ part,
+                                                           const GatedMax* __restrict__ maxes) {
     extern __shared__ __align__(16) char lds[];
     using Out = OutTile<T, BM, BN, gemm_wg(BM, BN)>;
     const TileAt at = tile_at(blockIdx.x, ktiles);
@@ -268,6 +347,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dx_kernel(GatedDims d, 
     f32x4 acc[NJ][MI];
     const int fb = blockIdx.y * share, fe = fb + share < width ? fb + share : width;
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
+    gated_undo<T, NJ, MI>(acc, maxes, d.in);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     if (gridDim.y > 1) {
         float* o = part + (int64_t)blockIdx.y * d.rows * d.in;
@@ -295,7 +375,8 @@ __host__ __device__ constexpr int64_t gated_part(int outp, int in) { return (int
 // part[s][f][k] = sum over the rows of split s of D[m][f] x[m][k]
 template <class T, int BM, int BN, bool FAST>
 __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dw_kernel(GatedDims d, int ktiles, int rows_a_split, const T* __restrict__ D,
-                                                           const T* __restrict__ x, float* __restrict__ part) {
+                                                           const T* __restrict__ x, float* __restrict__ part,
+                                                           const GatedMax* __restrict__ maxes) {
     extern __shared__ __align__(16) char lds[];
     const int k0 = (blockIdx.x % ktiles) * BN, f0 = (blockIdx.x / ktiles) * BM;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -311,6 +392,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dw_kernel(GatedDims d, 
     f32x4 acc[NJ][MI];
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.planes == 2 ? half + n : n, mrow, [&](int j) { return nbase + j * 16; },
                                 acc);
+    gated_undo<T, NJ, MI>(acc, maxes, d.in);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + blockIdx.y * gated_part(d.outp, d.in);
 #pragma unroll
@@ -336,6 +418,75 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(GatedDims d, const T* _
     else load_raw(raw, wu + (row - d.rows - d.out) * d.in + c, n > 8 ? 8 : n, d.wvw);
     T* to = row < d.rows ? xp + row * d.inw + c : wp + (row - d.rows) * d.inw + c;
     __builtin_memcpy(__builtin_assume_aligned(to, 16), &raw, sizeof(raw));
+}
+
+// What GatedMaxes reads: the largest finite |value| of each workgroup's share of x, the weights, the biases and dh.  A pass over
+// them, by memory (65536 x 256 -> 2 x 1024, 169 MB: 41 us; 5003 x 204 -> 2 x 530, with the copies: 9 us): 1024 threads, four loads each under way.
+struct GatedScan {  // an array of one kind
+    const f16* p;
+    int64_t rows, ld, cols;  // (rows that follow each other are one row)
+    f16* copy;               // what gated_pack_kernel writes, on the way (or null)
+    int64_t share;           // chunks of 8 values a workgroup
+    int vw, last;            // the last of its workgroups + 1
+};
+enum { SCAN_X, SCAN_WG, SCAN_WU, SCAN_BG, SCAN_BU, SCAN_DH, SCANS };
+struct GatedScans {
+    GatedScan s[SCANS];
+};
+__global__ __launch_bounds__(GATED_MAX_WG) void gated_max_kernel(GatedScans all, GatedMax* __restrict__ maxes) {
+    int k = 0, first = 0;
+    for (; k < SCANS - 1 && (int)blockIdx.x >= all.s[k].last; ++k) first = all.s[k].last;
+    const GatedScan s = all.s[k];
+    const int64_t chunks = (s.cols + 7) / 8, at = ((int)blockIdx.x - first) * s.share, total = s.rows * chunks;
+    const int64_t end = at + s.share < total ? at + s.share : total, dr = GATED_MAX_WG / chunks, dc = GATED_MAX_WG % chunks;
+    int64_t i = at + threadIdx.x, row = i / chunks, c = i % chunks;
+    u16x2 m = {0, 0};
+    while (i < end) {
+        Raw<f16> raw[4];
+        f16* to[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t n = i < end ? s.cols - c * 8 : 0;
+            load_raw(raw[u], s.p + (n > 0 ? row * s.ld + c * 8 : 0), n > 8 ? 8 : (int)n, n < 8 ? 1 : s.vw);
+            to[u] = n > 0 && s.copy != nullptr ? s.copy + (row * chunks + c) * 8 : nullptr;
+            i += GATED_MAX_WG;
+            row += dr;
+            c += dc;
+            if (c >= chunks) {
+                c -= chunks;
+                ++row;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (to[u] != nullptr) *reinterpret_cast<u32x4*>(to[u]) = raw[u].a;
+            u16x2 w[4], t = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = __builtin_bit_cast(u16x2, (uint32_t)raw[u].a[j] & 0x7fff7fffu);
+                t = larger(t, w[j]);
+            }
+            if (t[0] >= 0x7c00 || t[1] >= 0x7c00) {  // infinities and NaN are left out
+                t = u16x2{0, 0};
+                for (int j = 0; j < 4; ++j)
+                    for (int h = 0; h < 2; ++h)
+                        if (w[j][h] < 0x7c00 && w[j][h] > t[0]) t[0] = w[j][h];
+            }
+            m = larger(m, t);
+        }
+    }
+    __shared__ unsigned short red[GATED_MAX_WG / 64];
+    m = largest_of_wave(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m[0] > m[1] ? m[0] : m[1];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned short v = 0;
+        for (int w = 0; w < GATED_MAX_WG / 64; ++w) v = red[w] > v ? red[w] : v;
+        const unsigned short none = 0;
+        maxes[blockIdx.x] = {u16x2{k == SCAN_X ? v : none, k == SCAN_WG || k == SCAN_WU ? v : none},
+                             u16x2{k == SCAN_BG || k == SCAN_BU ? v : none, k == SCAN_DH ? v : none}};
+    }
+    if (blockIdx.x == 0 && gridDim.x + threadIdx.x < GATED_MAX_WGS) maxes[gridDim.x + threadIdx.x] = {};
 }
 
 // the parts of dx (workgroups below xblocks), of dW (wblocks more) and of the column sums, added in order
@@ -423,7 +574,7 @@ static bool gated_fills(int64_t m, int64_t n, int t, int64_t times) {
     }
 
 struct GatedScratch {  // bytes from the start
-    size_t pack, D, bpart, wpart, xpart, total;
+    size_t pack, D, bpart, wpart, xpart, maxes, total;
     int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
     int wtile, splits, rows_a_split;   // of dW
     int xtile, xsplits, share;         // of dx
@@ -481,7 +632,8 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
     s.bpart = s.D + up((size_t)rows * width * es);
     s.wpart = s.bpart + up((size_t)s.mtiles * 2 * outp * 4);
     s.xpart = s.wpart + up((size_t)s.splits * (size_t)gated_part((int)outp, in) * 4);
-    s.total = s.xpart + (s.xsplits > 1 ? up((size_t)s.xsplits * rows * in * 4) : 0);
+    s.maxes = s.xpart + (s.xsplits > 1 ? up((size_t)s.xsplits * rows * in * 4) : 0);
+    s.total = s.maxes + (dtype == TSD_F16 ? up(GATED_MAX_WGS * sizeof(GatedMax)) : 0);
     return s;
 }
 
@@ -521,27 +673,36 @@ static GatedDims gated_dims(int rows, int in, int out, int act, const void* x, i
 // 16-byte loads everywhere, and a tile's rows within the 2 GiB that a buffer's offsets reach
 static bool gated_fast(const GatedDims& d) { return d.xvw == 8 && d.wvw == 8 && d.ldx <= (1 << 21); }
 
-// packed: x, wg and wu become the copies in scratch
-template <class T>
-static int gated_pack(GatedDims& d, const void*& x, const void*& wg, const void*& wu, char* scratch, hipStream_t st) {
-    if (gated_fast(d) || !gated_packed(d.rows, d.in, d.out)) return TSD_OK;
+// Where the copies in scratch lie; null: there are none
+template <class T> static T* gated_copies(const GatedDims& d, char* scratch) {
+    return gated_fast(d) || !gated_packed(d.rows, d.in, d.out) ? nullptr : reinterpret_cast<T*>(scratch);
+}
+// x, wg and wu become the copies
+template <class T> static void gated_use_copies(GatedDims& d, const void*& x, const void*& wg, const void*& wu, T* xp) {
     d.inw = (d.in + 7) / 8 * 8;
-    T *xp = reinterpret_cast<T*>(scratch), *wp = xp + (int64_t)d.rows * d.inw;
-    const int64_t chunks = ((int64_t)d.rows + 2 * (int64_t)d.out) * (d.inw / 8);
-    hipLaunchKernelGGL(gated_pack_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, d, (const T*)x,
-                       (const T*)wg, (const T*)wu, xp, wp);
-    TSD_LAUNCH_CHECK("gated_pack");
+    T* wp = xp + (int64_t)d.rows * d.inw;
     x = xp;
     wg = wp;
     wu = wp + (int64_t)d.out * d.inw;
     d.ldx = d.ldw = d.inw;
     d.xvw = d.wvw = 8;
+}
+template <class T>
+static int gated_pack(GatedDims& d, const void*& x, const void*& wg, const void*& wu, char* scratch, hipStream_t st) {
+    T* xp = gated_copies<T>(d, scratch);
+    if (xp == nullptr) return TSD_OK;
+    d.inw = (d.in + 7) / 8 * 8;
+    const int64_t chunks = ((int64_t)d.rows + 2 * (int64_t)d.out) * (d.inw / 8);
+    hipLaunchKernelGGL(gated_pack_kernel<T>, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, d, (const T*)x,
+                       (const T*)wg, (const T*)wu, xp, xp + (int64_t)d.rows * d.inw);
+    TSD_LAUNCH_CHECK("gated_pack");
+    gated_use_copies(d, x, wg, wu, xp);
     return TSD_OK;
 }
 
 template <class T, int BM, int BN, bool FAST, bool BWD>
 static int gated_first(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
-                       void* h, void* D, float* part, hipStream_t st) {
+                       void* h, void* D, float* part, const GatedMax* maxes, hipStream_t st) {
     static DeviceOnce once;
     constexpr int lds = gated_lds<T, BM, BN, FAST>(gated_behind<T, BM, BN>(BWD));
     auto k = gated_kernel<T, BM, BN, FAST, BWD>;
@@ -549,13 +710,13 @@ static int gated_first(GatedDims d, const void* x, const void* wg, const void* w
     if (rc != TSD_OK) return rc;
     const int ft = div_up(BWD ? d.outp : d.out, BN / 2), mt = div_up(d.rows, BM);
     hipLaunchKernelGGL(k, dim3(tile_grid(mt, ft)), dim3(gemm_wg(BM, BN)), lds, st, d, ft, mt, (const T*)x, (const T*)wg, (const T*)wu,
-                       (const T*)bg, (const T*)bu, (const T*)dh, (T*)h, (T*)D, part);
+                       (const T*)bg, (const T*)bu, (const T*)dh, (T*)h, (T*)D, part, maxes);
     TSD_LAUNCH_CHECK("gated_linear");
     return TSD_OK;
 }
 template <class T, int BM, int BN, bool FAST>
 static int gated_dx(GatedDims d, const GatedScratch& s, const T* D, const void* wg, const void* wu, void* dx, float* part,
-                    hipStream_t st) {
+                    const GatedMax* maxes, hipStream_t st) {
     static DeviceOnce once;
     constexpr int lds = gated_lds<T, BM, BN, FAST>(OutTile<T, BM, BN, 64>::BYTES);
     auto k = gated_dx_kernel<T, BM, BN, FAST>;
@@ -563,20 +724,53 @@ static int gated_dx(GatedDims d, const GatedScratch& s, const T* D, const void* 
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), mt = div_up(d.rows, BM);
     hipLaunchKernelGGL(k, dim3(tile_grid(mt, kt), s.xsplits), dim3(gemm_wg(BM, BN)), lds, st, d, kt, mt, D, (const T*)wg,
-                       (const T*)wu, (T*)dx, s.share, part);
+                       (const T*)wu, (T*)dx, s.share, part, maxes);
     TSD_LAUNCH_CHECK("gated_dx");
     return TSD_OK;
 }
 template <class T, int BM, int BN, bool FAST>
-static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* x, float* wpart, hipStream_t st) {
+static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* x, float* wpart, const GatedMax* maxes,
+                    hipStream_t st) {
     static DeviceOnce once;
     constexpr int lds = gated_lds<T, BM, BN, FAST>(0);
     auto k = gated_dw_kernel<T, BM, BN, FAST>;
     const int rc = allow_lds(k, lds, once);
     if (rc != TSD_OK) return rc;
     const int kt = div_up(d.in, BN), ft = div_up(2 * d.outp, BM);
-    hipLaunchKernelGGL(k, dim3(kt * ft, s.splits), dim3(gemm_wg(BM, BN)), lds, st, d, kt, s.rows_a_split, D, (const T*)x, wpart);
+    hipLaunchKernelGGL(k, dim3(kt * ft, s.splits), dim3(gemm_wg(BM, BN)), lds, st, d, kt, s.rows_a_split, D, (const T*)x, wpart,
+                       maxes);
     TSD_LAUNCH_CHECK("gated_dw");
+    return TSD_OK;
+}
+// The list of the largest values, one launch, with the copies of gated_pack where xp is not null: at most 250 shares of all chunks, and one more for each array's last piece
+static int gated_maxes(const GatedDims& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
+                       f16* xp, f16* wp, GatedMax* maxes, hipStream_t st) {
+    const int64_t rows = d.rows, in = d.in, out = d.out, inw = (in + 7) / 8 * 8;
+    f16* wp2 = wp != nullptr ? wp + out * inw : nullptr;
+    GatedScans all = {{{(const f16*)x, rows, d.ldx, in, xp, 0, d.xvw, 0},
+                       {(const f16*)wg, out, in, in, wp, 0, d.wvw, 0},
+                       {(const f16*)wu, out, in, in, wp2, 0, d.wvw, 0},
+                       {(const f16*)bg, bg != nullptr ? 1 : 0, out, out, nullptr, 0, 1, 0},
+                       {(const f16*)bu, bu != nullptr ? 1 : 0, out, out, nullptr, 0, 1, 0},
+                       {(const f16*)dh, rows, d.lddh, out, nullptr, 0, d.dhvw, 0}}};
+    int64_t chunks = 0;
+    for (GatedScan& s : all.s) {
+        if (s.ld == s.cols && s.copy == nullptr) {
+            s.cols *= s.rows;
+            s.rows = 1;
+            s.vw = load_width(sizeof(f16), 8, 8, s.p);
+        }
+        if (s.cols == 0) s.rows = 0;
+        chunks += s.rows * ((s.cols + 7) / 8);
+    }
+    int wgs = 0;
+    for (GatedScan& s : all.s) {
+        s.share = chunks / 250 + 1 < 4096 ? 4096 : chunks / 250 + 1;
+        wgs += div_up(s.rows * ((s.cols + 7) / 8), s.share);
+        s.last = wgs;
+    }
+    hipLaunchKernelGGL(gated_max_kernel, dim3(wgs), dim3(GATED_MAX_WG), 0, st, all, maxes);
+    TSD_LAUNCH_CHECK("gated_max");
     return TSD_OK;
 }
 template <class T, bool BWD, class... A> static int gated_first_by(int tile, const GatedDims& d, A... a) {
@@ -590,12 +784,11 @@ template <class T>
 static int gated_bwd(GatedDims d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
                      const void* dh, int64_t lddh, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
                      const GatedScratch& s, char* scratch, hipStream_t st) {
-    const int prc = d.rows > 0 ? gated_pack<T>(d, x, wg, wu, scratch + s.pack, st) : TSD_OK;
-    if (prc != TSD_OK) return prc;
     T* D = reinterpret_cast<T*>(scratch + s.D);
     float* bpart = reinterpret_cast<float*>(scratch + s.bpart);
     float* wpart = reinterpret_cast<float*>(scratch + s.wpart);
     float* xpart = reinterpret_cast<float*>(scratch + s.xpart);
+    GatedMax* maxes = reinterpret_cast<GatedMax*>(scratch + s.maxes);
     const bool sums = dbg != nullptr || dbu != nullptr, weights = dwg != nullptr || dwu != nullptr;
     int rc = TSD_OK;
     d.planes = s.planes;
@@ -603,14 +796,23 @@ static int gated_bwd(GatedDims d, const void* x, const void* wg, const void* wu,
         d.lddh = lddh;
         d.dhvw = load_width(sizeof(T), d.out, lddh, dh);
         d.dxvw = load_width(sizeof(T), d.in, d.in, dx);
-        rc = gated_first_by<T, true>(s.tile, d, x, wg, wu, bg, bu, dh, (void*)nullptr, (void*)D, sums ? bpart : (float*)nullptr, st);
+        if constexpr (gated_scaled<T>()) {
+            T* xp = gated_copies<T>(d, scratch + s.pack);
+            rc = gated_maxes(d, x, wg, wu, bg, bu, dh, xp, xp != nullptr ? xp + d.rows * (((int64_t)d.in + 7) / 8 * 8) : nullptr, maxes, st);
+            if (xp != nullptr) gated_use_copies(d, x, wg, wu, xp);
+        } else {
+            rc = gated_pack<T>(d, x, wg, wu, scratch + s.pack, st);
+        }
+        if (rc != TSD_OK) return rc;
+        rc = gated_first_by<T, true>(s.tile, d, x, wg, wu, bg, bu, dh, (void*)nullptr, (void*)D, sums ? bpart : (float*)nullptr,
+                                     (const GatedMax*)maxes, st);
         if (rc == TSD_OK && dx != nullptr) {
-            GATED_BY_TILE(s.xtile, BM, BN, { rc = gated_dx<T, BM, BN, true>(d, s, D, wg, wu, dx, xpart, st); });
-            if (s.xtile == TILE_GUARDED) rc = gated_dx<T, 32, 64, false>(d, s, D, wg, wu, dx, xpart, st);
+            GATED_BY_TILE(s.xtile, BM, BN, { rc = gated_dx<T, BM, BN, true>(d, s, D, wg, wu, dx, xpart, maxes, st); });
+            if (s.xtile == TILE_GUARDED) rc = gated_dx<T, 32, 64, false>(d, s, D, wg, wu, dx, xpart, maxes, st);
         }
         if (rc == TSD_OK && weights) {
-            GATED_BY_TILE(s.wtile, BM, BN, { rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, st); });
-            if (s.wtile == TILE_GUARDED) rc = gated_dw<T, 32, 64, false>(d, s, D, x, wpart, st);
+            GATED_BY_TILE(s.wtile, BM, BN, { rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, maxes, st); });
+            if (s.wtile == TILE_GUARDED) rc = gated_dw<T, 32, 64, false>(d, s, D, x, wpart, maxes, st);
         }
     }
     const bool parts = d.rows > 0 && dx != nullptr && s.xsplits > 1;
@@ -657,7 +859,7 @@ int tsd_gated_linear_fwd(int32_t dtype, int32_t act, int32_t rows, int32_t in, i
         d.hvw = load_width(sizeof(T), out, out, h);
         if ((rc = gated_pack<T>(d, x, w_gate, w_up, (char*)scratch, (hipStream_t)stream)) != TSD_OK) return rc;
         return gated_first_by<T, false>(s.tile, d, x, w_gate, w_up, b_gate, b_up, (const void*)nullptr, h, (void*)nullptr,
-                                        (float*)nullptr, (hipStream_t)stream);
+                                        (float*)nullptr, (const GatedMax*)nullptr, (hipStream_t)stream);
     });
     return TSD_OK;
 }
