@@ -1,16 +1,17 @@
 """MI355X: the operators of an attention block at the ends of their types' ranges: gradients far from 1 in float16, whose
-intermediates lie among its subnormal numbers or beyond its largest one.
+intermediates lie among its subnormal numbers or beyond its largest one, and weights of many far keys.
 
 Tolerances are those of tests/block_oracle.py with one change: an intermediate that is rounded to feed a matrix product
-(D = [dg | du]) may be off by half a step of its own size and by what its place in the type's range costs AFTER a
+(D = [dg | du], P, dS) may be off by half a step of its own size and by what its place in the type's range costs AFTER a
 power of two has moved it there -- no longer by half a step of the type's subnormal numbers."""
+import math
 from unittest import mock
 
 import pytest
 import torch
 
 from tests import block_oracle as O
-from tests.test_gpu_block_ops import DEV, dev, normal
+from tests.test_gpu_block_ops import DEV, attention_case, dev, normal
 
 pytestmark = pytest.mark.gpu
 HALF = torch.float16
@@ -49,13 +50,11 @@ def gated_run(x, wg, wu, bg, bu, dh, act="swish"):
     return dict(zip(("h", "dx", "dwg", "dwu", "dbg", "dbu"), (h,) + torch.autograd.grad(h, t, dh.to(DEV))))
 
 
-@pytest.mark.parametrize("act", ["swish", "ssp", "ReLU", "Softplus"])
-@pytest.mark.parametrize("rows,fin,out", [(40, 64, 48), (300, 72, 104), (2100, 121, 77), (4096, 256, 512)])
+@pytest.mark.parametrize("rows,fin,out,act", [(40, 64, 48, a) for a in ("swish", "ssp", "ReLU", "Softplus")] +
+                         [(300, 72, 104, "ssp"), (2100, 121, 77, "swish"), (4096, 256, 512, "swish")])
 @pytest.mark.parametrize("size", [1e-3, 1e-5])
 def test_gated_linear_of_small_half_precision_gradients(size, rows, fin, out, act):
     """tiles whose D keeps what its rounding left, others, copied rows, large tiles"""
-    if act != "swish" and rows > 300:
-        pytest.skip("one activation is enough for the sizes")
     x, wg, wu = (normal(1, rows, fin, dtype=HALF), normal(2, out, fin, dtype=HALF, scale=fin ** -0.5),
                  normal(3, out, fin, dtype=HALF, scale=fin ** -0.5))
     bg, bu, dh = normal(4, out, dtype=HALF), normal(5, out, dtype=HALF), normal(6, rows, out, dtype=HALF, scale=size)
@@ -96,3 +95,64 @@ def test_gated_linear_scale_ignores_what_is_not_finite():
     assert not got["dx"][7].isfinite().all() and plain["dx"].isfinite().all()
     for n, t in gated_run(x, wg, wu, bg, bu, torch.zeros_like(dh)).items():
         assert n == "h" or not t.any(), n
+
+
+# ---- attention ------------------------------------------------------------------------------------------------
+def attention_want(q, k, v, do, qp, kp, mask, scale):
+    # weights of the forward are off by 2^-34 of the largest, those of dV by 2^-40; dS by 2^-39 of the largest of its row or key
+    return oracle(O.attention, lambda x: 2.0 ** -40 + 2.0 ** -34 * x.abs().amax(), q, k, v, qp, kp, mask, scale, do, HALF)
+
+
+def attention_run(q, k, v, do, qp, kp, mask, scale):
+    from tsdiff_amd.block_ops import graph_attention
+    t = dev(q, k, v)
+    out = graph_attention(*t, torch.tensor(qp, dtype=torch.int32, device=DEV), torch.tensor(kp, dtype=torch.int32, device=DEV),
+                          None if mask is None else mask.to(DEV), scale)
+    return dict(zip(("out", "dq", "dk", "dv"), (out,) + torch.autograd.grad(out, t, do.to(DEV))))
+
+
+SHAPES = [([20, 31, 9], None, 4, 2, 32), ([20, 31, 9], None, 2, 2, 33), ([300, 129], None, 4, 2, 64), ([2000], None, 2, 1, 64),
+          ([1, 1], [3000, 700], 2, 2, 32), ([1500], [3], 2, 2, 40), ([90, 70], None, 2, 2, 100)]
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("qs,ks,heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("size", [1e-3, 1e-5])
+def test_attention_of_small_half_precision_gradients(size, qs, ks, heads, kv_heads, dim, masked):
+    q, k, v, do, qp, kp, mask, _ = attention_case(qs, ks, heads, kv_heads, dim, HALF, masked and len(qs) > 1, seed=3)
+    do = (do.float() * size).half()
+    want = attention_want(q, k, v, do, qp, kp, mask, dim ** -0.5)
+    got = attention_run(q, k, v, do, qp, kp, mask, dim ** -0.5)
+    for n in want:
+        check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("qs,ks,heads,kv_heads,dim", SHAPES)
+def test_attention_of_large_half_precision_gradients(qs, ks, heads, kv_heads, dim):
+    """dS beyond 65504 whose products are not; rows whose gradients differ by a factor of 2^20"""
+    q, k, v, do, qp, kp, mask, _ = attention_case(qs, ks, heads, kv_heads, dim, HALF, False, seed=3)
+    q, k, v = q * 2.0 ** -4, k * 2.0 ** -4, v * 8
+    rows = torch.arange(do.shape[0])
+    do = (do.float() * torch.where(rows % 3 == 0, 2.0 ** 13, torch.where(rows % 3 == 1, 1.0, 2.0 ** -7))[:, None, None]).clamp(-60000, 60000).half()
+    want = attention_want(q, k, v, do, qp, kp, mask, dim ** -0.5)
+    got = attention_run(q, k, v, do, qp, kp, mask, dim ** -0.5)
+    for n in want:
+        assert not got[n].isnan().any(), n
+        check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dim", [32, 33, 128])
+def test_attention_keeps_the_weights_of_many_far_keys(dim):
+    """one key's weight is 1 and its value 0, each of 60000 others' is 2^-25.2: alone the others answer"""
+    n = 60001
+    q, k, v = torch.zeros(1, 1, dim), torch.zeros(n, 1, dim), torch.ones(n, 1, dim)
+    q[..., 0] = 1
+    k[1:, 0, 0] = -25.2 * math.log(2)
+    v[0] = 0
+    q, k, v = q.half(), k.half(), v.half()
+    do = normal(1, 1, 1, dim, dtype=HALF)
+    want = attention_want(q, k, v, do, [0, 1], [0, n], None, 1.0)
+    got = attention_run(q, k, v, do, [0, 1], [0, n], None, 1.0)
+    assert 1.4e-3 < float(want["out"][0].min()) < 1.7e-3
+    for name in ("out", "dq", "dv"):
+        check(got[name], want[name], name)

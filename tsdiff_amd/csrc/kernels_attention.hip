@@ -33,6 +33,14 @@ namespace blk {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LAG = 6.f;  // (in powers of two: weights up to 64 times 1, far from the end of every type)
+// f16: the weights and dS become matrix operands as powers of two of themselves.  As they are, small ones fall among the
+// subnormal numbers (steps of 2^-24), where a long list of them is lost as a whole, and a dS beyond 65504 becomes infinite
+// (2000 nodes, 2 heads of 64, dO of 1e-3: dQ and dK off by 2.6e-3 so, by 5.1e-4 with these, the rounding of dQ itself 4.7e-4;
+// for 4 to 6 % of the time of a training step of long graphs).
+// Forward: 2^(S - m + 9), up to 2^15 with LAG; dK / dV: 2^(S - L + 15); dS: DsScale.
+template <class T> constexpr bool att_scaled() { return __is_same(T, f16); }
+template <class T> constexpr float att_fwd_shift() { return att_scaled<T>() ? 9.f : 0.f; }
+template <class T> constexpr float att_dkv_shift() { return att_scaled<T>() ? 15.f : 0.f; }
 
 struct AttDims {
     int graphs, rows_q, rows_k, heads, kv_heads, group, dim;
@@ -330,6 +338,30 @@ __device__ __forceinline__ float over_groups_max(float v) {
 __device__ __forceinline__ float over_groups_sum(float v) {
     return over_groups(v, [](float a, float b) { return a + b; });
 }
+// The power of two that a lane's dS (of one row or one key: the four lanes of it go together) are multiplied by: the largest so
+// far lies in 2^14 .. 2^15, or below where it is less than 2^-86.  A larger one lowers it, and what is summed up so far with it.
+struct DsScale {
+    float by = 0x1p100f;
+    __device__ __forceinline__ static float inverse(float power) {
+        return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, power));
+    }
+    template <int D> __device__ __forceinline__ void take(f32x4& a, f32x4& b, f32x4 (&acc)[D]) {
+        float hi = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, fmaxf(fabsf(a[e]), fabsf(b[e])));
+        if (__any(hi * by > 0x1p15f)) {
+            const float top = over_groups_max(hi);
+            const int e = 127 + 14 + 127 - (int)(__builtin_bit_cast(uint32_t, top) >> 23);  // 2^14 <= top 2^(e - 127) < 2^15
+            const float to = __builtin_bit_cast(float, (uint32_t)(e < 27 ? 27 : e > 227 ? 227 : e) << 23);
+            const float next = top * by > 0x1p15f ? to : by, ratio = next * inverse(by);
+            by = next;
+#pragma unroll
+            for (int t = 0; t < D; ++t) acc[t] *= ratio;
+        }
+        a *= by;
+        b *= by;
+    }
+};
 template <class T>
 __device__ __forceinline__ Rows<T> rows_of(const T* p, int64_t row, int64_t head, int start, int n, int first_head, int group,
                                            int dim, const uint8_t* mask, int vw) {
@@ -488,7 +520,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
 #pragma unroll
                         for (int t = 0; t < DP / 16; ++t) o[t] *= a;
                     }
-                    const float safe = m == -INFINITY ? 0.f : m;
+                    const float safe = (m == -INFINITY ? 0.f : m) - att_fwd_shift<T>();
 #pragma unroll
                     for (int t = 0; t < KT / 16; ++t)
 #pragma unroll
@@ -508,6 +540,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
                 });
         }
         const float ls = over_groups_sum(l);
+        m -= att_fwd_shift<T>();  // (what the weights were taken from)
         if (row >= nrows) continue;
         const int qi = query_of(row, d.group);
         const int64_t at = (int64_t)(sp.qs + qi) * d.heads + hk * d.group + row - qi * d.group;
@@ -634,6 +667,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
         if (mine && g == 0 && blockIdx.z == 0) delta[at] = del;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) acc[t] = f32x4{0, 0, 0, 0};
+        DsScale scale;
         Stage ks, vs;
         ks.init(kr);
         vs.init(vr);
@@ -687,6 +721,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                                 s[u][e] = __builtin_bit_cast(
                                     float, __builtin_bit_cast(uint32_t, w) & (uint32_t)__builtin_amdgcn_sbfe(bits, 4 * u + e, 1));
                             }
+                        if constexpr (att_scaled<T>()) scale.take(s[0], s[1], acc);
                         const Weights<T, att_rest<T, WAVES>()> f = {s[0], s[1]};
 #pragma unroll
                         for (int t = 0; t < DP / 16; ++t) {
@@ -700,6 +735,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
         // a row without an open key has dQ = 0 whatever dO and O hold
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
+            if constexpr (att_scaled<T>()) acc[t] *= DsScale::inverse(scale.by);
             const f32x4 r = L == INFINITY ? f32x4{0, 0, 0, 0} : acc[t] * d.scale;
             const int n = d.dim - t * 16 - g * 4;
             if (d.splits > 1)
@@ -751,6 +787,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
         const bool open_key = kr.has(key);
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) ak[t] = av[t] = f32x4{0, 0, 0, 0};
+        DsScale scale;
         Stage qs, gs;
         qs.init(qr);
         gs.init(gr);
@@ -818,7 +855,8 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                         const f32x4 del = *reinterpret_cast<const f32x4*>(stat + 64 + 32 * p + 8 * g + 4 * u);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float w = exp2_fast(__builtin_fmaf(s[u][e], d.scale2, -L[e]));
+                            const float from = att_scaled<T>() ? att_dkv_shift<T>() - L[e] : -L[e];
+                            const float w = exp2_fast(__builtin_fmaf(s[u][e], d.scale2, from));
                             s[u][e] = w;
                             dp[u][e] = w * (dp[u][e] - del[e]);
                         }
@@ -835,6 +873,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                                 dp[u][e] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, ds) & m);
                             }
                     }
+                    if constexpr (att_scaled<T>()) scale.take(dp[0], dp[1], ak);
                     const Weights<T, att_rest<T, WAVES>()> pf = {s[0], s[1]}, df = {dp[0], dp[1]};
 #pragma unroll
                     for (int t = 0; t < DP / 16; ++t) {
@@ -851,6 +890,10 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             const int y = t * 16 + g * 4, n = d.dim - y;
+            if constexpr (att_scaled<T>()) {
+                av[t] *= 0x1p-15f;  // 2^-att_dkv_shift, which dS has too
+                ak[t] *= DsScale::inverse(scale.by) * 0x1p-15f;
+            }
             // a masked key's gradients are 0 whatever the rows that do not read it hold (a lane's sums are one key's)
             const f32x4 zero = {0, 0, 0, 0}, rk = open_key ? ak[t] * d.scale : zero, rv = open_key ? av[t] : zero;
             if (d.splits > 1) {
