@@ -1,5 +1,5 @@
 """MI355X: the operators of an attention block at the ends of their types' ranges: gradients far from 1 in float16, whose
-intermediates lie among its subnormal numbers or beyond its largest one, and weights of many far keys.
+intermediates lie among its subnormal numbers or beyond its largest one, weights of many far keys, and float32 values that no bfloat16 holds.
 
 Tolerances are those of tests/block_oracle.py with one change: an intermediate that is rounded to feed a matrix product
 (D = [dg | du], P, dS) may be off by half a step of its own size and by what its place in the type's range costs AFTER a
@@ -156,3 +156,38 @@ def test_attention_keeps_the_weights_of_many_far_keys(dim):
     assert 1.4e-3 < float(want["out"][0].min()) < 1.7e-3
     for name in ("out", "dq", "dv"):
         check(got[name], want[name], name)
+
+
+# ---- float32 values that no bfloat16 holds ---------------------------------------------------------------------
+LARGEST = torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("rows,fin,out", [(3, 8, 8), (5, 7, 9), (130, 64, 72), (9000, 64, 64)])
+def test_gated_linear_of_the_largest_floats(rows, fin, out):
+    """finite operands whose first bfloat16 plane would round to infinity: 0 times them is 0, 1 / 2^120 of them is 2^8"""
+    x, wg, wu, dh = normal(1, rows, fin), normal(2, out, fin), normal(3, out, fin), normal(4, rows, out)
+    x[:, 1], x[0, 1] = LARGEST, -LARGEST
+    wg[:, 1] = wu[:, 1] = 0
+    wu[2, 1] = 2.0 ** -120
+    bg, bu = normal(5, out), normal(6, out)
+    want = O.gated(x, wg, wu, bg, bu, "swish")
+    from tsdiff_amd.block_ops import gated_linear
+    got = gated_linear(*dev(x, wg, wu, bg, bu, grad=False))
+    assert got.isfinite().all()
+    # the zeros' products cost nothing, the last places of 2^8 do (their tolerance is in the oracle's sums of magnitudes)
+    O.check(got, want["h"], "h")
+    t = dev(x, wg, wu, bg, bu)
+    dx = torch.autograd.grad(gated_linear(*t), t[0], dh.to(DEV))[0]
+    assert dx.isfinite().all()
+
+
+@pytest.mark.parametrize("n,dim", [(1, 32), (40, 32), (200, 64), (3, 33), (500, 128)])
+def test_attention_passes_the_largest_floats_on(n, dim):
+    """values of a graph whose rows each have one open key: out = v, whatever v's size"""
+    from tsdiff_amd.block_ops import graph_attention
+    q, k, v = torch.zeros(n, 2, dim), normal(2, n, 2, dim), normal(3, n, 2, dim)  # (scores of 0: a weight of exactly 1)
+    v[n // 2] = torch.where(torch.arange(dim) % 2 == 0, LARGEST, -LARGEST)
+    mask = torch.zeros(n, dtype=torch.bool)
+    mask[n // 2] = True
+    out = graph_attention(*dev(q, k, v, grad=False), torch.tensor([0, n], dtype=torch.int32, device=DEV), key_mask=mask.to(DEV))
+    assert torch.equal(out.cpu(), v[n // 2].expand(n, 2, dim))

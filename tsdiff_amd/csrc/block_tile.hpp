@@ -5,9 +5,9 @@
 // (l / 16) * 8 .. + 7 of row l % 16 of either operand, and of the result the four rows (l / 16) * 4 .. + 3 of column
 // l % 16.  bf16 and f16 operands go in as they are.  An f32 operand goes in as THREE bf16 planes, x = hi + mid + lo
 // (8 + 8 + 8 bits, each the rounded rest of the one before): six of the nine plane products, smallest first, leave
-// 2^-24 of a product out.  bf16 has the exponents of f32, so nothing has to be scaled and no value leaves the range,
-// unlike f16 planes; a rate of 1/6 of the bf16 pipes is 2.6 times that of the f32 matrix instruction.  (A non-finite
-// f32 operand comes out as NaN: inf - inf in the split.)
+// 2^-24 of a product out.  bf16 has the exponents of f32, so nothing has to be scaled, unlike f16 planes, and the largest
+// values, which would round to infinity, have the largest bf16 as their first plane; a rate of 1/6 of the bf16 pipes is 2.6
+// times that of the f32 matrix instruction.  (A non-finite f32 operand comes out as NaN: inf - inf in the split.)
 #pragma once
 #include "common.hpp"
 
@@ -52,14 +52,19 @@ __device__ __forceinline__ Chunk<f16> to_chunk(const float (&x)[8], f16) {
     for (int j = 0; j < 8; ++j) c.p[0][j] = (f16)x[j];
     return c;
 }
-__device__ __forceinline__ Chunk<float> to_chunk(const float (&x)[8], float) {
+constexpr float BF16_MAX = 0x1.FEp127f;
+// (ANY: values as they come from memory; weights and their gradients are far from the largest.  The limit on the first plane
+// costs 1 to 2 % of the f32 launches: gated 30000 x 256 -> 2 x 1024, training, 716 -> 732 us.)
+template <bool ANY> __device__ __forceinline__ Chunk<float> to_planes(const float (&x)[8]) {
     Chunk<float> c;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         f32x2 r = {x[j], x[j + 1]};
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-            const bf16x2 h = __builtin_convertvector(r, bf16x2);
+            f32x2 v = r;
+            if (ANY && p == 0) v = {__builtin_amdgcn_fmed3f(r[0], -BF16_MAX, BF16_MAX), __builtin_amdgcn_fmed3f(r[1], -BF16_MAX, BF16_MAX)};
+            const bf16x2 h = __builtin_convertvector(v, bf16x2);
             c.p[p][j] = h[0];
             c.p[p][j + 1] = h[1];
             r[0] -= (float)h[0];
@@ -68,6 +73,8 @@ __device__ __forceinline__ Chunk<float> to_chunk(const float (&x)[8], float) {
     }
     return c;
 }
+
+__device__ __forceinline__ Chunk<float> to_chunk(const float (&x)[8], float) { return to_planes<false>(x); }
 
 __device__ __forceinline__ f32x4 mma(const Chunk<bf16>& a, const Chunk<bf16>& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
@@ -170,7 +177,7 @@ __device__ __forceinline__ Chunk<f16> raw_chunk(const Raw<f16>& r) {
 }
 __device__ __forceinline__ Chunk<float> raw_chunk(const Raw<float>& r) {
     const float x[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
-    return to_chunk(x, 0.f);
+    return to_planes<true>(x);
 }
 
 // ---------------------------------------------------------------------------------------------
