@@ -1060,7 +1060,10 @@ int linear_bwd_impl(int rows, int in, int out, const float* X, const float* W, c
     if (dW) {  // dW = dY^T X
         const int S = rows >= 4096 ? 64 : (rows >= 1024 ? 32 : (rows >= 256 ? 16 : 4));  // row splits of the MFMA wgrad
         if (rows == 0) {
-            if (!accW) TSD_HIP(hipMemsetAsync(dW, 0, (size_t)out * in * sizeof(float), st));
+            if (!accW) {  // sums over no rows (a kernel: the call may be captured into a graph)
+                hipLaunchKernelGGL(wgrad_naive_kernel, dim3(out * in), dim3(256), 0, st, 0, in, out, dY, X, dW, 0);
+                TSD_LAUNCH_CHECK("wgrad_none");
+            }
         } else if (scratch && scratch_floats >= off_part + (size_t)S * out * in && out % 128 == 0 && in % 128 == 0) {
             const int per = ((rows + S - 1) / S + WG_T - 1) / WG_T * WG_T;
             float* part = scratch + off_part;

@@ -25,7 +25,8 @@ class GraphTransformerBlock(nn.Module):
 
     def forward(self, h, graph_ptr, key_mask=None):
         x = layer_norm(h, self.norm1.weight, self.norm1.bias, self.norm1.eps)
-        qkv = linear(x, self.qkv.weight, self.qkv.bias).view(h.shape[0], -1, self.head_dim)
+        qkv = linear(x, self.qkv.weight, self.qkv.bias)
+        qkv = qkv.view(h.shape[0], self.num_heads + 2 * self.num_kv_heads, self.head_dim)
         q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), dim=1)
         x = graph_attention(q, k, v, graph_ptr, key_mask=key_mask)
         h = h + linear(x.reshape(h.shape), self.proj.weight, self.proj.bias)
