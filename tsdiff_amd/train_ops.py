@@ -14,6 +14,7 @@ nodes serve the differentiable `forward()`, the legacy dual-encoder network and 
 step (`TSDIFF_TRAIN=ops`).
 """
 import ctypes as C
+import threading
 
 import torch
 
@@ -26,16 +27,19 @@ def _c(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
-_SCRATCH = {}
+_SCRATCH = threading.local()  # .kept: {(device, stream): tensor}
 
 
 def _scratch(device, n):
-    """per-device scratch for the two-stage bias-gradient reduction (64 * out floats)"""
-    key = str(device)
-    t = _SCRATCH.get(key)
+    """Scratch of the dense layers (packed weights, parts of gradients).  A thread and stream of its own each: what is queued on
+    one stream by one thread runs in order, and nothing else orders two calls.  A captured call's belongs to the graph's pool."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, dtype=torch.float32, device=device)
+    kept = _SCRATCH.__dict__.setdefault("kept", {})
+    key = (device, torch.cuda.current_stream().cuda_stream)
+    t = kept.get(key)
     if t is None or t.numel() < n:
-        t = torch.empty(max(n, 64 * 1024), dtype=torch.float32, device=device)
-        _SCRATCH[key] = t
+        t = kept[key] = torch.empty(max(n, 64 * 1024), dtype=torch.float32, device=device)
     return t
 
 
