@@ -111,3 +111,18 @@ def test_encoders_of_several_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_the_encoder_works_on_its_tensors_device(monkeypatch):
+    """whichever device is current (the dense layers ask for the current one)"""
+    enc, = encoders(1)
+    entered, device = [], torch.cuda.device
+
+    class Recorded(device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    enc(torch.zeros(3, 128, device=DEV), torch.tensor([0, 3], dtype=torch.int32, device=DEV))
+    assert entered == [0]

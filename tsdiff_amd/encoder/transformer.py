@@ -50,6 +50,7 @@ class GraphTransformerEncoder(nn.Module):
             raise _lib.TsdError("tsdiff_amd runs on the GPU only (no CPU fallback)")
         if h.dim() != 2 or h.shape[1] != self.hidden_dim or h.dtype != torch.float32:
             raise ValueError(f"h is {h.dtype} {tuple(h.shape)}, float32 [nodes, {self.hidden_dim}] expected")
-        for block in self.blocks:
-            h = block(h, graph_ptr, key_mask)
+        with torch.cuda.device(h.device):  # the dense layers go to the current device
+            for block in self.blocks:
+                h = block(h, graph_ptr, key_mask)
         return h
