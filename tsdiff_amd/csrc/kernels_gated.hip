@@ -594,8 +594,12 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
     s.mtiles = div_up(rows, TILE_M[s.tile]);
     s.planes = es == 2 && s.tile >= TILE_32 && (int64_t)rows * 2 * outp <= (1 << 18) ? 2 : 1;
     const size_t width = s.planes * 2 * outp;
-    // dW: the rows in shares: one workgroup a CU of the largest tiles, 2048 rows each at least (below, the parts cost what the
-    // tile saves: 16300 x 250 -> 2 x 600, 320 rows each: 48 + 27 us against 45 + 16); else about two, of at least 256 rows
+    // dW: the rows in shares: one workgroup a CU of the largest tiles, 1024 rows each at least; else about two, of at least 256
+    // rows.  The large tiles save time a row and cost more parts to add, 4 us.  bf16, launch and sum of the parts in us, at
+    // 512 / 768 / 1024 / 1536 / 2048 rows a share:
+    //   256 -> 2 x 1024: 256 x 256 44 / 54 / 62 / 83 / 106, 128 x 128 39 / 52 / 64 / 88 / 115
+    //   512 -> 2 x 512:  43 / 52 / 62 / 82 / 101, 39 / 51 / 64 / 90 / 121
+    //   1024 -> 2 x 2048: 47 / 53 / 62 / 74 / 90, 42 / 52 / 61 / 81 / 101
     const int most = div_up(rows, 256), large = guarded ? TILE_GUARDED : es == 4 ? TILE_128 : TILE_256;
     int n = 0;
     for (s.wtile = large;; s.wtile += s.wtile == TILE_256 ? 2 : 1) {
@@ -604,7 +608,7 @@ static GatedScratch gated_scratch(int dtype, int rows, int in, int out, bool fas
         n = n < most ? n : most;
         n = n < 1 ? 1 : n;
         if (s.wtile == TILE_GUARDED || s.wtile == TILE_64) break;
-        if (s.wtile == TILE_256 ? gated_fills(2 * outp, in, s.wtile, n) && rows / n >= 2048
+        if (s.wtile == TILE_256 ? gated_fills(2 * outp, in, s.wtile, n) && rows / n >= 1024
                                 : gated_fills(2 * outp, in, s.wtile, most))
             break;
     }
