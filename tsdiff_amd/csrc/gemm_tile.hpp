@@ -9,7 +9,7 @@
 namespace tsd {
 namespace blk {
 
-// Waves over one side of the output tile: two, of 64 rows or columns at most
+// Waves over one side of the output tile: two, or four of 64 rows or columns each over a side of 256
 constexpr int gemm_waves(int n) { return n > 128 ? n / 64 : 2; }
 constexpr int gemm_wg(int bm, int bn) { return 64 * gemm_waves(bm) * gemm_waves(bn); }
 constexpr int GEMM_K = 32;    // steps of the contraction a tile

@@ -10,7 +10,8 @@
 // of a tile are taken in the order (sub_row) in which a lane's eight scores are eight consecutive keys.  Every tile lies in
 // LDS as it lies in memory, for both products: S reads it along its rows, P V and dS K by the LDS's transposing read.
 // The backward computes the scores again from L: one launch over row tiles for dQ (and delta), one over key tiles for dK and
-// dV; every gradient is summed by one workgroup in a fixed order, without atomics.
+// dV.  Without atomics: a gradient is summed by one workgroup in a fixed order or, where few workgroups have long sums, in parts
+// that a further launch adds in order.
 //
 // Rows are (query, query head of the key head's group), so heads that share keys share their tiles.  Tiles never cross a
 // graph: workgroup s looks its graph up, slot(v) = floor((start_v + v (T - 1)) / T) being where graph v's tiles begin -- a
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_fwd_kernel(AttDims d, const T*
     }
 }
 
-// The parts of a row: out = sum_z 2^(m_z - m) O_z / sum_z 2^(m_z - m) l_z, 64 rows' values a workgroup
+// The parts of a row: out = sum_z 2^(m_z - m) O_z / sum_z 2^(m_z - m) l_z, a thread a value, 256 a workgroup
 template <class T>
 __global__ __launch_bounds__(256) void att_join_kernel(int64_t all, int dim, int splits, const float* __restrict__ part,
                                                         T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse) {

@@ -576,7 +576,7 @@ static bool gated_fills(int64_t m, int64_t n, int t, int64_t times) {
 struct GatedScratch {  // bytes from the start
     size_t pack, D, bpart, wpart, xpart, maxes, total;
     int tile, mtiles;                  // of the first launch, whose row tiles have a row of column sums each
-    int wtile, splits, rows_a_split;   // of dW
+    int wtile, splits, rows_a_split;   // of dW (TILE_256 of 16 bits, TILE_128, TILE_64, TILE_GUARDED)
     int xtile, xsplits, share;         // of dx
     int planes;                        // of D
 };
@@ -815,8 +815,10 @@ static int gated_bwd(GatedDims d, const void* x, const void* wg, const void* wu,
             if (s.xtile == TILE_GUARDED) rc = gated_dx<T, 32, 64, false>(d, s, D, wg, wu, dx, xpart, maxes, st);
         }
         if (rc == TSD_OK && weights) {
-            GATED_BY_TILE(s.wtile, BM, BN, { rc = gated_dw<T, BM, BN, true>(d, s, D, x, wpart, maxes, st); });
             if (s.wtile == TILE_GUARDED) rc = gated_dw<T, 32, 64, false>(d, s, D, x, wpart, maxes, st);
+            else if (s.wtile == TILE_64) rc = gated_dw<T, 64, 64, true>(d, s, D, x, wpart, maxes, st);
+            else if (s.wtile == TILE_128) rc = gated_dw<T, 128, 128, true>(d, s, D, x, wpart, maxes, st);
+            else if constexpr (sizeof(T) == 2) rc = gated_dw<T, 256, 256, true>(d, s, D, x, wpart, maxes, st);
         }
     }
     const bool parts = d.rows > 0 && dx != nullptr && s.xsplits > 1;

@@ -168,7 +168,7 @@ template <class T, int VE, bool SHIFT> __device__ __forceinline__ int norm_shift
 // A group's rows first, first + step, ..: each is fetched while the one before it is worked on.  With SHIFT the first and the
 // last row of all go by themselves: what lies beside them need not be theirs to read.  work(r, next): next >= rows: none.
 template <bool SHIFT, class Fetch, class Edge, class Work>
-__device__ __forceinline__ void norm_rows(int64_t first, int64_t step, int64_t rows, int s, Fetch fetch, Edge edge, Work work) {
+__device__ __forceinline__ void norm_rows(int64_t first, int64_t step, int64_t rows, Fetch fetch, Edge edge, Work work) {
     const int64_t none = (int64_t)1 << 62;
     if constexpr (SHIFT) {
         const int64_t last = rows - 1;
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_fwd_kernel(int rows, int dim, co
             rstd[r] = rs;
         }
     };
-    norm_rows<SHIFT>(first, step, rows, s, [&](int64_t r) { R::template fetch<false>(raw, x + r * ldx, dim, lane, s); },
+    norm_rows<SHIFT>(first, step, rows, [&](int64_t r) { R::template fetch<false>(raw, x + r * ldx, dim, lane, s); },
                      [&](int64_t r) { R::template fetch<true>(raw, x + r * ldx, dim, lane, s); }, work);
 }
 
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_bwd_kernel(int rows, int dim, co
             R::store(dx + r * dim, g, dim, lane, s);
         }
     };
-    norm_rows<SHIFT>(first, step, rows, s, fetch, edge, work);
+    norm_rows<SHIFT>(first, step, rows, fetch, edge, work);
     if (part == nullptr) return;
     constexpr int W = LANES * E;  // columns that a group has room for
     if constexpr (GROUPS > 1) {
@@ -384,7 +384,7 @@ template <class T, int VE, bool SHIFT, int LANES, int E> static int norm_launch(
     return TSD_OK;
 }
 
-// The smallest group that holds a row: a wave (or part of one) up to 32 values a lane, four waves beyond.
+// The smallest group that holds a row: a wave (or part of one) up to 32 values a lane (2048 columns), four waves beyond.
 template <class T, int VE, bool SHIFT> static int norm_by_dim(const NormCall& c) {
     const int n = (c.dim + (SHIFT ? VE - 1 : 0) + VE - 1) / VE;  // loads a row
     if constexpr (VE > 1) {
@@ -402,7 +402,6 @@ template <class T, int VE, bool SHIFT> static int norm_by_dim(const NormCall& c)
         if (n <= 1024) return norm_launch<T, VE, SHIFT, 64, 16>(c);
         if (n <= 2048) return norm_launch<T, VE, SHIFT, 64, 32>(c);
     }
-    if (n * VE <= 256 * 8) return norm_launch<T, VE, SHIFT, 256, 8>(c);
     if (n * VE <= 256 * 16) return norm_launch<T, VE, SHIFT, 256, 16>(c);
     if (n * VE <= 256 * 32) return norm_launch<T, VE, SHIFT, 256, 32>(c);
     return norm_launch<T, 1, false, 256, 32>(c);  // (8192 columns and a shift)
