@@ -38,8 +38,8 @@ def check(got, want, what):
 def gated_want(x, wg, wu, bg, bu, dh, act="swish"):
     # D is scaled by a power of two that takes the bound B of its values into 2^14 .. 2^15; half a step of the subnormal
     # numbers there is B 2^-39 at most in D's own units
-    n, most = x.shape[1], [float(t.abs().max()) for t in (x, torch.cat((wg, wu)), torch.cat((bg, bu)), dh)]
-    bound = most[3] * 1.25 * (n * most[0] * most[1] + most[2] + 1)
+    most = [float(t.double().norm(dim=1).max()) for t in (x, torch.cat((wg, wu)))] + [float(t.abs().max()) for t in (torch.cat((bg, bu)), dh)]
+    bound = most[3] * 1.25 * (most[0] * most[1] * 1.02 + most[2] + 1)  # (norms are bf16 rounded up)
     return oracle(O.gated, lambda v: bound * 2.0 ** -39, x, wg, wu, bg, bu, act, dh, HALF)
 
 
@@ -77,6 +77,35 @@ def test_gated_linear_of_large_half_precision_gradients(rows, fin, out):
     for n in ("h", "dx", "dwg", "dwu"):
         assert got[n].isfinite().all(), n
         check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("rows,fin,out", [(40, 64, 48), (300, 1000, 104), (2100, 121, 77)])
+def test_gated_linear_with_single_large_values(rows, fin, out):
+    """one large value in x and in the weights: the other rows' gradients stay what they are"""
+    x, wg, wu = (normal(1, rows, fin, dtype=HALF), normal(2, out, fin, dtype=HALF, scale=fin ** -0.5),
+                 normal(3, out, fin, dtype=HALF, scale=fin ** -0.5))
+    bg, bu, dh = normal(4, out, dtype=HALF), normal(5, out, dtype=HALF), normal(6, rows, out, dtype=HALF)
+    x[3, 5] = 30000.0
+    wu[2, 7] = 50.0
+    dh[3] = 0
+    want, got = gated_want(x, wg, wu, bg, bu, dh), gated_run(x, wg, wu, bg, bu, dh)
+    for n in ("dx", "dwg", "dwu", "dbg", "dbu"):
+        check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("rows", [1040])
+def test_gated_linear_of_half_precision_rows_far_apart(rows):
+    """rows of x and of dh 2^21 values apart: the last ones lie past 2^31 values"""
+    from tsdiff_amd.block_ops import gated_linear
+    gap = 1 << 21
+    far = torch.empty(rows * gap, dtype=HALF, device=DEV).view(rows, gap)
+    x, wg, wu, dh = (normal(s, *shape, dtype=HALF).to(DEV) for s, shape in ((1, (rows, 64)), (2, (24, 64)), (3, (24, 64)), (4, (rows, 24))))
+    far[:, :64], far[:, 64:88] = x, dh * 1e-5
+    got = []
+    for a, d in ((x, far[:, 64:88].contiguous()), (far[:, :64], far[:, 64:88])):
+        a = a.detach().requires_grad_()
+        got.append(torch.autograd.grad(gated_linear(a, wg, wu), a, d)[0])
+    assert torch.equal(*got)
 
 
 def test_gated_linear_scale_ignores_what_is_not_finite():

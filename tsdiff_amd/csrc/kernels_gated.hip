@@ -67,16 +67,18 @@ struct GatedDims {
 // f16: D = [dg | du] times a power of two s, by which neither small gradients fall among the subnormal numbers (steps of 2^-24)
 // nor large products beyond 65504 (4096 x 256 -> 2 x 512, dh of 1e-5: dW off by 1.8e-3 without s, by 2.9e-4 with it, as for dh
 // of 1; rounding dW alone: 2.1e-4).  One s for all of D, since its rows and its columns are both summed over; it takes the bound
-//   |D| <= max |dh| (in max |x| max |W| + max |b| + 1) 1.25   (|a'| < 1.1, |a(g)| < |g| + 0.7, the rest is room for roundings)
-// into 2^14 .. 2^15.  The bound lies above D's ordinary values by about 16 sqrt(in), which leaves them 14 to 26 powers of two
-// above the subnormal numbers.  Values that are not finite are left out: their rows are lost either way.
+//   |D| <= max |dh| (X W + max |b| + 1) 1.25   (|a'| < 1.1, |a(g)| < |g| + 0.7, the rest is room for roundings)
+// into 2^14 .. 2^15, X and W being the largest norms of a row of x and of a row of the weights.  The bound lies above D's ordinary
+// values by about 5 sqrt(in), which leaves them 16 to 26 powers of two above the subnormal numbers; with norms a single large
+// value in x or the weights costs what it may make of u, not in times that.  What is not finite is left out: its rows are lost
+// either way.
 template <class T> constexpr bool gated_scaled() { return std::is_same<T, f16>::value; }
 struct GatedScale {
     float by, undo;
 };
 using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
 constexpr int GATED_MAX_WG = 1024, GATED_MAX_WGS = 256;
-struct GatedMax {  // bits of f16 values, which compare like the values: of x and the weights, of the biases and dh
+struct GatedMax {  // bits that compare like the values: norms of x and the weights (bf16, rounded up), biases and dh (f16)
     u16x2 xw, bd;
 };
 __device__ __forceinline__ u16x2 larger(u16x2 a, u16x2 b) { return __builtin_elementwise_max(a, b); }
@@ -107,14 +109,15 @@ template <class T> struct GatedMaxes {
             raw[1] = p[1];
         }
     }
-    __device__ __forceinline__ GatedScale scale(int in) const {
+    __device__ __forceinline__ GatedScale scale() const {
         if constexpr (!gated_scaled<T>()) return {1.f, 1.f};
         auto two = [&](int i, int j) { return __builtin_bit_cast(u16x2, (uint32_t)raw[i][j]); };
         const u16x2 xw = largest_of_wave(larger(larger(two(0, 0), two(0, 2)), larger(two(1, 0), two(1, 2))));
         const u16x2 bd = largest_of_wave(larger(larger(two(0, 1), two(0, 3)), larger(two(1, 1), two(1, 3))));
         auto value = [](unsigned short b) { return (float)__builtin_bit_cast(f16, b); };
+        auto norm = [](unsigned short b) { return __builtin_bit_cast(float, (uint32_t)b << 16); };
         // 2^-24 .. 2^70, or 0
-        const float bound = value(bd[1]) * 1.25f * ((float)in * value(xw[0]) * value(xw[1]) + value(bd[0]) + 1.f);
+        const float bound = value(bd[1]) * 1.25f * (norm(xw[0]) * norm(xw[1]) + value(bd[0]) + 1.f);
         const int e = (int)(__builtin_bit_cast(uint32_t, bound) >> 23);  // 2^(e - 127) <= bound
         const int to = bound > 0.f ? 127 + 14 + 127 - e : 127;
         return {__builtin_bit_cast(float, (uint32_t)to << 23), __builtin_bit_cast(float, (uint32_t)(254 - to) << 23)};
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
         Out::keep(dhr, lds);
         __syncthreads();
     }
-    const GatedScale scale = BWD ? most.scale(d.in) : GatedScale{1.f, 1.f};
+    const GatedScale scale = BWD ? most.scale() : GatedScale{1.f, 1.f};
     const bool whole = m0 + BM <= d.rows && f0 + FT <= d.out;
     // (a tile without edges needs no looks at them; swish has code of its own: with all kinds' in every place of the unrolled
     // loops the code outgrows its cache)
@@ -315,11 +318,11 @@ __global__ __launch_bounds__(gemm_wg(BM, BN), sizeof(T) == 4 ? 2 : BM > 128 ? 4 
 }
 
 template <class T, int NJ, int MI>
-__device__ __forceinline__ void gated_undo(f32x4 (&acc)[NJ][MI], const GatedMax* __restrict__ maxes, int in) {
+__device__ __forceinline__ void gated_undo(f32x4 (&acc)[NJ][MI], const GatedMax* __restrict__ maxes) {
     if constexpr (gated_scaled<T>()) {
         GatedMaxes<T> most;
         most.load(maxes);
-        const GatedScale scale = most.scale(in);
+        const GatedScale scale = most.scale();
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -347,7 +350,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dx_kernel(GatedDims d, 
     f32x4 acc[NJ][MI];
     const int fb = blockIdx.y * share, fe = fb + share < width ? fb + share : width;
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, fb, fe, mrow, [&](int j) { return nbase + j * 16; }, acc);
-    gated_undo<T, NJ, MI>(acc, maxes, d.in);
+    gated_undo<T, NJ, MI>(acc, maxes);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     if (gridDim.y > 1) {
         float* o = part + (int64_t)blockIdx.y * d.rows * d.in;
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(gemm_wg(BM, BN)) void gated_dw_kernel(GatedDims d, 
     f32x4 acc[NJ][MI];
     gated_gemm<T, BM, BN, FAST>(lds, ns, ms, 0, d.planes == 2 ? half + n : n, mrow, [&](int j) { return nbase + j * 16; },
                                 acc);
-    gated_undo<T, NJ, MI>(acc, maxes, d.in);
+    gated_undo<T, NJ, MI>(acc, maxes);
     const int r = lane & 15, c4 = (lane >> 4) * 4;
     float* o = part + blockIdx.y * gated_part(d.outp, d.in);
 #pragma unroll
@@ -420,35 +423,67 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(GatedDims d, const T* _
     __builtin_memcpy(__builtin_assume_aligned(to, 16), &raw, sizeof(raw));
 }
 
-// What GatedMaxes reads: the largest finite |value| of each workgroup's share of x, the weights, the biases and dh.  A pass over
-// them, by memory (65536 x 256 -> 2 x 1024, 169 MB: 41 us; 5003 x 204 -> 2 x 530, with the copies: 9 us): 1024 threads, four loads each under way.
+// What GatedMaxes reads: of each workgroup's share the largest norm of a row of x or the weights, the largest |bias| or |dh|.  A
+// pass over them, by memory (65536 x 256 -> 2 x 1024, 169 MB: 42 us; 5003 x 204 -> 2 x 530, with the copies: 10 us): 16 waves, four
+// loads a lane under way.
 struct GatedScan {  // an array of one kind
     const f16* p;
-    int64_t rows, ld, cols;  // (rows that follow each other are one row)
+    int64_t rows, ld, cols;  // (biases and dh: where rows follow each other they are one)
     f16* copy;               // what gated_pack_kernel writes, on the way (or null)
-    int64_t share;           // chunks of 8 values a workgroup
+    int64_t share;           // rows (biases and dh: chunks of 8 values) a workgroup
     int vw, last;            // the last of its workgroups + 1
 };
 enum { SCAN_X, SCAN_WG, SCAN_WU, SCAN_BG, SCAN_BU, SCAN_DH, SCANS };
 struct GatedScans {
     GatedScan s[SCANS];
 };
-__global__ __launch_bounds__(GATED_MAX_WG) void gated_max_kernel(GatedScans all, GatedMax* __restrict__ maxes) {
-    int k = 0, first = 0;
-    for (; k < SCANS - 1 && (int)blockIdx.x >= all.s[k].last; ++k) first = all.s[k].last;
-    const GatedScan s = all.s[k];
-    const int64_t chunks = (s.cols + 7) / 8, at = ((int)blockIdx.x - first) * s.share, total = s.rows * chunks;
-    const int64_t end = at + s.share < total ? at + s.share : total, dr = GATED_MAX_WG / chunks, dc = GATED_MAX_WG % chunks;
+__device__ __forceinline__ bool gated_has_norms(int k) { return k <= SCAN_WU; }
+// rows at .. end - 1: G lanes a row, four rows of a group at once
+__device__ __forceinline__ unsigned short gated_norms(const GatedScan& s, int64_t at, int64_t end) {
+    const int chunks = (int)((s.cols + 7) / 8);
+    int G = 1;
+    while (G < chunks && G < 64) G *= 2;
+    const int64_t groups = GATED_MAX_WG / G;
+    float top = 0.f;
+    for (int64_t row = at + threadIdx.x / G; row < end; row += 4 * groups) {  // (the same in all lanes of a group)
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = threadIdx.x % G; c < chunks; c += G) {
+            const int n = (int)s.cols - c * 8;
+            Raw<f16> raw[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t r = row + u * groups;
+                load_raw(raw[u], s.p + (r < end ? r * s.ld + c * 8 : 0), r >= end ? 0 : n > 8 ? 8 : n, s.vw);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t r = row + u * groups;
+                if (s.copy != nullptr && r < end) *reinterpret_cast<u32x4*>(s.copy + (r * chunks + c) * 8) = raw[u].a;
+                const f16x8 v = __builtin_bit_cast(f16x8, raw[u].a);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[u] += (float)v[j] * (float)v[j];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            for (int k = 1; k < G; k *= 2) sum[u] += __shfl_xor(sum[u], k, 64);
+            top = sum[u] < INFINITY && sum[u] > top ? sum[u] : top;
+        }
+    }
+    // (past the bf16 below it, by one or two of its steps)
+    return top > 0.f ? (unsigned short)((__builtin_bit_cast(uint32_t, sqrtf(top)) >> 16) + 1) : 0;
+}
+// chunks at .. end - 1
+__device__ __forceinline__ unsigned short gated_largest(const GatedScan& s, int64_t at, int64_t end) {
+    const int64_t chunks = (s.cols + 7) / 8, dr = GATED_MAX_WG / chunks, dc = GATED_MAX_WG % chunks;
     int64_t i = at + threadIdx.x, row = i / chunks, c = i % chunks;
     u16x2 m = {0, 0};
     while (i < end) {
         Raw<f16> raw[4];
-        f16* to[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int64_t n = i < end ? s.cols - c * 8 : 0;
-            load_raw(raw[u], s.p + (n > 0 ? row * s.ld + c * 8 : 0), n > 8 ? 8 : (int)n, n < 8 ? 1 : s.vw);
-            to[u] = n > 0 && s.copy != nullptr ? s.copy + (row * chunks + c) * 8 : nullptr;
+            load_raw(raw[u], s.p + (n > 0 ? row * s.ld + c * 8 : 0), n > 8 ? 8 : (int)n, n < 8 ? 1 : s.vw);  // (a whole array's end)
             i += GATED_MAX_WG;
             row += dr;
             c += dc;
@@ -459,7 +494,6 @@ __global__ __launch_bounds__(GATED_MAX_WG) void gated_max_kernel(GatedScans all,
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (to[u] != nullptr) *reinterpret_cast<u32x4*>(to[u]) = raw[u].a;
             u16x2 w[4], t = {0, 0};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -475,9 +509,18 @@ __global__ __launch_bounds__(GATED_MAX_WG) void gated_max_kernel(GatedScans all,
             m = larger(m, t);
         }
     }
+    return m[0] > m[1] ? m[0] : m[1];
+}
+__global__ __launch_bounds__(GATED_MAX_WG) void gated_max_kernel(GatedScans all, GatedMax* __restrict__ maxes) {
+    int k = 0, first = 0;
+    for (; k < SCANS - 1 && (int)blockIdx.x >= all.s[k].last; ++k) first = all.s[k].last;
+    const GatedScan s = all.s[k];
+    const int64_t total = gated_has_norms(k) ? s.rows : s.rows * ((s.cols + 7) / 8);
+    const int64_t at = ((int)blockIdx.x - first) * s.share, end = at + s.share < total ? at + s.share : total;
+    const unsigned short mine = gated_has_norms(k) ? gated_norms(s, at, end) : gated_largest(s, at, end);
     __shared__ unsigned short red[GATED_MAX_WG / 64];
-    m = largest_of_wave(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m[0] > m[1] ? m[0] : m[1];
+    const u16x2 m = largest_of_wave(u16x2{mine, 0});
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m[0];
     __syncthreads();
     if (threadIdx.x == 0) {
         unsigned short v = 0;
@@ -746,7 +789,8 @@ static int gated_dw(GatedDims d, const GatedScratch& s, const T* D, const void* 
     TSD_LAUNCH_CHECK("gated_dw");
     return TSD_OK;
 }
-// The list of the largest values, one launch, with the copies of gated_pack where xp is not null: at most 250 shares of all chunks, and one more for each array's last piece
+// The list of the largest values, one launch, with the copies of gated_pack where xp is not null: at most 250 shares of all
+// chunks, and one more for each array
 static int gated_maxes(const GatedDims& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh,
                        f16* xp, f16* wp, GatedMax* maxes, hipStream_t st) {
     const int64_t rows = d.rows, in = d.in, out = d.out, inw = (in + 7) / 8 * 8;
@@ -758,19 +802,22 @@ static int gated_maxes(const GatedDims& d, const void* x, const void* wg, const 
                        {(const f16*)bu, bu != nullptr ? 1 : 0, out, out, nullptr, 0, 1, 0},
                        {(const f16*)dh, rows, d.lddh, out, nullptr, 0, d.dhvw, 0}}};
     int64_t chunks = 0;
-    for (GatedScan& s : all.s) {
-        if (s.ld == s.cols && s.copy == nullptr) {
+    for (int k = 0; k < SCANS; ++k) {
+        GatedScan& s = all.s[k];
+        if (k > SCAN_WU && s.ld == s.cols) {
             s.cols *= s.rows;
-            s.rows = 1;
+            s.rows = s.cols > 0 ? 1 : 0;
             s.vw = load_width(sizeof(f16), 8, 8, s.p);
         }
-        if (s.cols == 0) s.rows = 0;
         chunks += s.rows * ((s.cols + 7) / 8);
     }
+    const int64_t share = chunks / 250 + 1 < 4096 ? 4096 : chunks / 250 + 1;
     int wgs = 0;
-    for (GatedScan& s : all.s) {
-        s.share = chunks / 250 + 1 < 4096 ? 4096 : chunks / 250 + 1;
-        wgs += div_up(s.rows * ((s.cols + 7) / 8), s.share);
+    for (int k = 0; k < SCANS; ++k) {
+        GatedScan& s = all.s[k];
+        const int64_t c = (s.cols + 7) / 8, parts = s.rows > 0 ? div_up(s.rows * c, share) : 0;
+        s.share = k > SCAN_WU ? share : parts > 0 ? div_up(s.rows, parts) : 0;
+        wgs += (int)parts;
         s.last = wgs;
     }
     hipLaunchKernelGGL(gated_max_kernel, dim3(wgs), dim3(GATED_MAX_WG), 0, st, all, maxes);
