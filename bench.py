@@ -51,10 +51,13 @@ PEAK_HBM_GBS = 8000.0          # /opt/skills/guides/MI355X_MICROARCH.md:35 (spec
 # HBM-side bytes per launch come from the committed rocprofv3 PMC passes of this round (tools/profile_round.sh), read
 # here because counters cannot be collected inside a bench run; a missing file gives `traffic: null`
 PMC_C2, PMC_C5, MFMA_BUSY = "r06_pmc_traffic.json", "r06_pmc_traffic_c5.json", "r06_mfma_busy.json"
+# the attention block's sources (layer norm, gated layer, attention): no workload here launches them
+BLOCK_SOURCES = ("block_tile.hpp", "gemm_tile.hpp", "kernels_norm.hip", "kernels_gated.hip", "kernels_attention.hip")
 
 
 def kernel_source_sha():
-    """sha256 (16 hex digits) over the kernel sources the counters describe (csrc/*.hip, *.hpp, the C header): the
+    """sha256 (16 hex digits) over the kernel sources the counters describe (csrc/*.hip, *.hpp, the C header; not the attention
+    block's, which no profiled run launches): the
     profile tools (tools/pmc_summary.py, tools/mfma_busy.py) stamp it into the files they write, and the line below prints
     `traffic` / `mfma_busy` only from files whose stamp equals the tree's -- counters of older kernels are refused
     (`traffic: null`, `traffic_note`) instead of being quoted beside a live timing"""
@@ -64,6 +67,8 @@ def kernel_source_sha():
     d = os.path.join(ROOT, "tsdiff_amd", "csrc")
     for f in sorted(glob.glob(os.path.join(d, "*.hip")) + glob.glob(os.path.join(d, "*.hpp")) +
                     [os.path.join(ROOT, "include", "tsdiff_hip.h")]):
+        if os.path.basename(f) in BLOCK_SOURCES:
+            continue
         h.update(os.path.basename(f).encode())
         h.update(open(f, "rb").read())
     return h.hexdigest()[:16]
