@@ -50,7 +50,7 @@ PEAK_SPLIT_F16_TFLOPS = PEAK_F16_MFMA_TFLOPS / 3.0
 PEAK_HBM_GBS = 8000.0          # /opt/skills/guides/MI355X_MICROARCH.md:35 (spec)
 # HBM-side bytes per launch come from the committed rocprofv3 PMC passes of this round (tools/profile_round.sh), read
 # here because counters cannot be collected inside a bench run; a missing file gives `traffic: null`
-PMC_C2, PMC_C5, MFMA_BUSY = "r06_pmc_traffic.json", "r06_pmc_traffic_c5.json", "r06_mfma_busy.json"
+PMC_C2, PMC_C5, MFMA_BUSY = "pmc_traffic.json", "pmc_traffic_c5.json", "mfma_busy.json"
 # the attention block's sources (layer norm, gated layer, attention): no workload here launches them
 BLOCK_SOURCES = ("block_tile.hpp", "gemm_tile.hpp", "kernels_norm.hip", "kernels_gated.hip", "kernels_attention.hip")
 

@@ -14,6 +14,9 @@ for f in mfma_busy pmc_traffic pmc_traffic_c5 pmc_traffic_train bench_c2_1000 be
          bench_train_torchrun_3range; do
   [ -s $O/${R}_$f.json ] && cp $O/${R}_$f.json $P/
 done
+for f in mfma_busy pmc_traffic pmc_traffic_c5; do  # what bench.py reads
+  [ -s $O/${R}_$f.json ] && cp $O/${R}_$f.json $P/$f.json
+done
 wrap() {  # log -> fenced markdown with a title
   [ -s $O/$1 ] || return
   { echo "# $2"; echo; echo '```'; cat $O/$1; echo '```'; } > $P/$3

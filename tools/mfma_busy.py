@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """MFMA-busy fraction per kernel from rocprofv3 SQ-counter passes (rocpd .db files of tools/profile_round.sh):
     frac = SQ_VALU_MFMA_BUSY_CYCLES / (1024 SIMDs x average launch duration x 2.4 GHz)
-python tools/mfma_busy.py label=x_results.db ... > profiles/rNN_mfma_busy.json   (bench.py reads it)"""
+python tools/mfma_busy.py label=x_results.db ... > profiles/mfma_busy.json   (bench.py reads it)"""
 import json
 import os
 import sqlite3

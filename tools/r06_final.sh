@@ -8,7 +8,7 @@ O=gpurun_out; R=r06
 python3 -c 'import __graft_entry__ as g; g.smoke(); print("smoke ok")' 2>&1 | tail -2
 ( time timeout 1500 python3 -m pytest tests -q -m gpu ) > $O/${R}_gpu_tests.log 2>&1; tail -3 $O/${R}_gpu_tests.log
 bash tools/profile_round.sh $R > $O/${R}_profile_round.log 2>&1
-cp $O/${R}_pmc_traffic*.json $O/${R}_mfma_busy.json profiles/ 2>/dev/null  # (bench.py reads the counter files of THIS campaign)
+for f in mfma_busy pmc_traffic pmc_traffic_c5; do cp $O/${R}_$f.json profiles/$f.json; done  # (bench.py reads the counter files of THIS campaign)
 bash tools/bench_round.sh $R > $O/${R}_bench_round.log 2>&1; tail -14 $O/${R}_bench_round.log
 python3 tools/power_trace.py --hz 20 --seconds 6 --out $O/${R}_c5_power_clock.md c5 ens8 c2 > $O/${R}_power.log 2>&1; cat $O/${R}_c5_power_clock.md
 # the windowed aggregation against the one-wave-per-row form (variant build -DTSD_AGW_MIN_ROWS=0), interleaved processes
