@@ -54,19 +54,16 @@ __device__ __forceinline__ Chunk<f16> to_chunk(const float (&x)[8], f16) {
 }
 constexpr float BF16_MAX = 0x1.FEp127f;
 // (ANY: values as they come from memory; weights and their gradients are far from the largest.  The limit on the first plane
-// costs 1 to 2 % of the f32 launches and more of the long gated ones: training, 3600 x 256 -> 2 x 1024 125.6 -> 127.5 us, 30000 rows
-// 738 -> 774.  A look at the largest of eight values with a branch around the limits: 1 % slower than the limits.)
+// costs 1 to 2 % of the f32 launches: gated 30000 x 256 -> 2 x 1024, training, 716 -> 732 us.)
 template <bool ANY> __device__ __forceinline__ Chunk<float> to_planes(const float (&x)[8]) {
     Chunk<float> c;
-    float most = BF16_MAX;
-    if (ANY) asm("" : "+s"(most));  // (a scalar register: the compiler spends two of the lanes' on it and its negative)
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         f32x2 r = {x[j], x[j + 1]};
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
             f32x2 v = r;
-            if (ANY && p == 0) v = {__builtin_amdgcn_fmed3f(r[0], -most, most), __builtin_amdgcn_fmed3f(r[1], -most, most)};
+            if (ANY && p == 0) v = {__builtin_amdgcn_fmed3f(r[0], -BF16_MAX, BF16_MAX), __builtin_amdgcn_fmed3f(r[1], -BF16_MAX, BF16_MAX)};
             const bf16x2 h = __builtin_convertvector(v, bf16x2);
             c.p[p][j] = h[0];
             c.p[p][j + 1] = h[1];
