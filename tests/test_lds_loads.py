@@ -12,7 +12,7 @@ spec.loader.exec_module(chk)
 GOOD = """
 \t;;#ASMSTART
 \ts_mov_b32 m0, s7
-\ts_nop 0
+\ts_nop 3
 \tbuffer_load_dwordx4 v3, s[8:11], 0 offen lds
 \t;;#ASMEND
 \tv_add_f32_e32 v2, v3, v4   ; m0 in a comment
@@ -34,6 +34,11 @@ def test_a_move_and_its_load_pass(tmp_path):
                                   "\t;;#ASMSTART\n\ts_nop 0\n\tbuffer_load_dword v3, s[8:11], 0 offen lds\n\t;;#ASMEND\n"])
 def test_other_uses_of_m0_and_loads_without_a_move_fail(line, tmp_path):
     assert run(GOOD + line, tmp_path) == 1
+
+
+def test_a_load_too_close_behind_a_scalar_register_fails(tmp_path):
+    for nop in range(3):
+        assert run(GOOD.replace("s_nop 3", f"s_nop {nop}"), tmp_path) == 1
 
 
 def test_a_listing_without_such_loads_fails(tmp_path):

@@ -233,6 +233,8 @@ template <class T, int ROWS_, int C_> struct Tile {
 // ---------------------------------------------------------------------------------------------
 // Loads from memory to LDS that pass no register (16-bit types): lane l of a wave writes 16 bytes at the wave's base +
 // 16 l (m0 holds the base: nothing else in these kernels uses it); an offset past the buffer's end (NOWHERE) writes zeros.
+// The buffer's address may come from a vector instruction (v_readfirstlane) right in front, and the compiler's hazard recognizer
+// does not look into the statement: it lets the five wait states pass itself that the load needs then (s_mov 1, s_nop 3 4).
 // The compiler does not see them: dma_wait<N> waits until at most the N youngest loads of the wave are under way, behind it
 // stands a barrier.
 // ---------------------------------------------------------------------------------------------
@@ -256,14 +258,14 @@ __device__ __forceinline__ f32x4 buffer_load(i32x4 buf, uint32_t off) {
         (int)off, 0, 0));
 }
 __device__ __forceinline__ void dma_load(i32x4 buf, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(buf)
                  : "memory");
 }
 // 4 bytes a lane: lane l writes the wave's base + 4 l
 __device__ __forceinline__ void dma_load4(i32x4 buf, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(buf)
                  : "memory");
