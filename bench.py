@@ -31,6 +31,7 @@ import argparse
 import ctypes as C
 import json
 import os
+import re
 import sys
 import time
 
@@ -56,9 +57,8 @@ BLOCK_SOURCES = ("block_tile.hpp", "gemm_tile.hpp", "kernels_norm.hip", "kernels
 
 
 def kernel_source_sha():
-    """sha256 (16 hex digits) over the kernel sources the counters describe (csrc/*.hip, *.hpp, the C header; not the attention
-    block's, which no profiled run launches): the
-    profile tools (tools/pmc_summary.py, tools/mfma_busy.py) stamp it into the files they write, and the line below prints
+    """sha256 (16 hex digits) over the kernel sources the counters describe (csrc/*.hip, *.hpp, the C header without its comments;
+    not the attention block's, which no profiled run launches): the profile tools (tools/pmc_summary.py, tools/mfma_busy.py) stamp it into the files they write, and the line below prints
     `traffic` / `mfma_busy` only from files whose stamp equals the tree's -- counters of older kernels are refused
     (`traffic: null`, `traffic_note`) instead of being quoted beside a live timing"""
     import glob
@@ -70,7 +70,8 @@ def kernel_source_sha():
         if os.path.basename(f) in BLOCK_SOURCES:
             continue
         h.update(os.path.basename(f).encode())
-        h.update(open(f, "rb").read())
+        text = open(f, "rb").read()
+        h.update(re.sub(rb"/\*.*?\*/|[ \t]+$", b"", text, flags=re.S | re.M) if f.endswith(".h") else text)
     return h.hexdigest()[:16]
 
 

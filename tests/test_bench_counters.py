@@ -17,6 +17,9 @@ def test_the_stamp_follows_the_profiled_kernels_alone(tmp_path, monkeypatch):
         assert (csrc / name).exists()
         (csrc / name).write_text("// another kernel")
         assert bench.kernel_source_sha() == want, name
+    header = tmp_path / "include" / "tsdiff_hip.h"
+    header.write_text(header.read_text().replace("/* element types", "/* the element types"))
+    assert bench.kernel_source_sha() == want
     (csrc / "kernels_combo.hip").write_text("// another kernel")
     assert bench.kernel_source_sha() != want
 

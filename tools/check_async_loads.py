@@ -11,6 +11,9 @@ in order among loads; stores only add to the outstanding count), carries the set
 branches to their labels, and reports any instruction that names a destination register of an asm-issued load that a
 preceding wait has not covered on some path.
 
+And since the compiler's hazard recognizer does not look into inline asm either: a load there has to stand five wait states behind
+a vector instruction (v_readfirstlane, v_readlane of a spilled register, v_cmp) that writes a scalar register it reads.
+
     python tools/check_async_loads.py file.s [...]        exit code 1 on a violation
 """
 import re
@@ -47,6 +50,46 @@ def merge(a, b):
     for r, (line, y) in b.items():
         out[r] = (line, min(y, out[r][1])) if r in out else (line, y)
     return out
+
+
+SREG = re.compile(r"\bs(\d+)\b|\bs\[(\d+):(\d+)\]")
+VALU_TO_SGPR = re.compile(r"^v_(readlane|readfirstlane|cmp)\w*\s+(s\d+|s\[\d+:\d+\])")
+SGPR_WAITS = 5
+
+
+def sregs_of(text):
+    out = set()
+    for m in SREG.finditer(text):
+        out.update([int(m.group(1))] if m.group(1) is not None else range(int(m.group(2)), int(m.group(3)) + 1))
+    return out
+
+
+def check_scalars(lines):
+    """`young`: scalar register -> wait states since a vector instruction wrote it (up to SGPR_WAITS; a scalar instruction that
+    writes it ends that).  In text order: a branch takes longer than these states."""
+    young, in_asm, bad = {}, False, []
+    for no, raw in lines:
+        st = raw.strip()
+        if st.startswith((";;#ASMSTART", ";;#ASMEND")):
+            in_asm = st.startswith(";;#ASMSTART")
+            continue
+        line = raw.split(";", 1)[0].strip()
+        if not line or line.startswith(".") or line.endswith(":"):
+            continue
+        if in_asm and VMEM.match(line):
+            clash = sregs_of(line) & young.keys()
+            if clash:
+                bad.append((no, line, sorted(clash), sorted(young[r] for r in clash)))
+        nop = re.match(r"s_nop (\d+)", line)
+        passed = int(nop.group(1)) + 1 if nop else 1
+        young = {r: a + passed for r, a in young.items() if a + passed < SGPR_WAITS}
+        m = VALU_TO_SGPR.match(line)
+        if m:
+            young.update((r, 0) for r in sregs_of(m.group(2)))
+        elif line.startswith("s_") and " " in line:
+            for r in sregs_of(line.split(None, 1)[1].split(",")[0]):
+                young.pop(r, None)
+    return bad
 
 
 def check_kernel(name, lines):
@@ -108,7 +151,7 @@ def check_kernel(name, lines):
             bad.append((no, raw.strip(), sorted(clash), sorted({hot[r][0] for r in clash})))
         if VMEM.match(line) is not None and "_load" in line.split()[0]:
             hot = {r: (l, y + 1) for r, (l, y) in hot.items()}
-            if in_asm:
+            if in_asm and not line.endswith(" lds"):  # (a load to LDS has no destination register)
                 first = line.split(None, 1)[1].split(",")[0]
                 for r in regs_of(first):
                     hot[r] = (no, 0)
@@ -146,6 +189,9 @@ def main(paths):
             if len(bad) > 8:
                 print(f"{path}: {name[:70]}: ... {len(bad) - 8} more")
             total += len(bad)
+            for no, text, regs, ages in check_scalars(body):
+                print(f"{path}:{no}: {name[:70]}: `{text}` reads s{regs} {ages} wait states behind the vector instruction that wrote it")
+                total += 1
     print(f"check_async_loads: {kernels} kernels with inline asm, {total} violation(s)")
     return 1 if total else 0
 

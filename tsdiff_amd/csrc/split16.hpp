@@ -236,6 +236,9 @@ __device__ __forceinline__ void hgemm_ring_start(HRing<CB, R>& r, const float* _
 #endif
     r.plane_bytes = 32 * nout;
     r.cb_bytes = 32 * 16;
+    // (the base may have come out of a vector register just now -- a scalar register's spill -- and a load needs five wait states
+    // behind that, which the compiler does not count for inline asm; tools/check_async_loads.py looks at every load's)
+    asm volatile("s_nop 4" : : "s"(r.base));
     constexpr int KS = K / 16;
     static_for<0, (R < KS ? R : KS)>([&](auto i) {
         constexpr int I = decltype(i)::value;
