@@ -613,8 +613,9 @@ int tsd_gaussian_edge_encode(int64_t num_edges, int32_t K, float coeff, const fl
  * Three operators by which the nodes of a graph see each other beside message passing, forward and backward
  * (tsdiff_amd/block_ops.py: the same as autograd functions; tsdiff_amd/encoder/transformer.py: an encoder of them).
  * `dtype` (TSD_F32 / TSD_BF16 / TSD_F16) is the type of every tensor that is not declared float or int; sums,
- * statistics and softmax state are fp32, outputs are rounded once.  f32 products run on the bf16 matrix pipes with
- * three-plane operands at fp32 accuracy (non-finite f32 operands of the products come out as NaN).  No atomics: the same
+ * statistics and softmax state are fp32, outputs are rounded once; in bf16 and f16 the operands of a matrix product that a call
+ * computes itself (softmax weights, their gradients, the gated layer's [dg | du]) are rounded to that type too.  f32 products
+ * run on the bf16 matrix pipes with three-plane operands at fp32 accuracy (non-finite f32 operands of the products come out as NaN).  No atomics: the same
  * bits on every run; no host synchronisation, capturable.
  *
  * Layer norm over the last dimension (1 .. 8192):  y = (x - mean) rstd weight + bias, rstd = (var + eps)^-1/2.
@@ -657,8 +658,8 @@ typedef struct tsd_attention {
 size_t tsd_graph_attention_scratch_floats(const tsd_attention* a, int32_t backward);
 /* out [num_queries, heads, dim] dense.  For the backward: lse [num_queries, heads], log2 of the sum of 2^(score log2 e) (+inf
  * where there is no open key), and for bf16 / f16 out_rest, what the rounding of `out` left (same type and shape: sum dO O,
- * which the gradients of the scores are taken from, needs more digits than `out` has).  Either NULL: not kept.  scratch (16-byte aligned) may be NULL where the query
- * function says 0 floats. */
+ * which the gradients of the scores are taken from, needs more digits than `out` has).  Either NULL: not kept.  scratch (16-byte
+ * aligned) may be NULL where the query function says 0 floats. */
 int tsd_graph_attention_fwd(const tsd_attention* a, void* out, void* out_rest, float* lse, float* scratch, size_t scratch_floats,
                             void* stream);
 /* dq, dk, dv dense in the layouts of q, k, v; do_row / do_head: strides of dout; out_rest may be NULL */

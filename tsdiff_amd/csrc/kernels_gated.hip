@@ -4,20 +4,23 @@
 //   dg = dh u a'(g), du = dh a(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x;  dbg, dbu = column sums
 //
 // Forward: one launch; a workgroup multiplies a tile of rows with the same columns of both weights, so a lane holds g and u
-// of one place and the product leaves the kernel as h.  Backward: launch 1 computes g and u again (they are not kept: at 256
-// inputs reading them back in f32 costs more than the products) and writes D = [dg | du] in the tensors' type -- the one
-// rounding of an intermediate, since D is the next two products' matrix operand; a small D (at most 2^18 values of 16 bits) is
+// of one place and the product leaves the kernel as h.  Backward: launch 1 computes g and u again (they are not kept, which saves
+// 2 rows out values between the passes; in time that is the cheaper choice in 16 bits up to about 460 inputs, where writing and
+// reading them costs as much as the products, in f32 only up to about 120) and writes D = [dg | du] in the tensors' type -- the
+// one rounding of an intermediate, since D is the next two products' matrix operand; a small D (at most 2^18 values of 16 bits) is
 // written with what the rounding left as a second half of twice the width, which the products go over too, since sums of few
 // terms show one rounding more than large ones, and time is no matter there -- with each row tile's column sums in fp32;
 // f16 gradients put a launch in front, by which D lies in the middle of f16's range whatever the size of dh (GatedMaxes);
 // launch 2 is dx = D [Wg; Wu]; launch 3 dW = D^T x, the rows split over workgroups; launch 4 adds the parts in a fixed order.
 //
 // Measured (GPU time a launch; each product is 4 rows in out operations):
-//   bf16, 65536 x 256 -> 2 x 1024: forward 119 us (580 TFLOP/s, h and x are 170 MB of it), first of the backward 180 us (it
-//   writes D, 268 MB, and reads dh, 134 MB), dx 82 us (840 TFLOP/s), dW 92 us (747 TFLOP/s), sums 13 us.  Bound by what a CU
-//   draws from L2 (about 10 TB/s over the chip), the two first ones by that and by memory.
-//   f32, 3600 x 256 -> 2 x 1024: 30, 34, 31, 30 and 11 us; six plane products each: 126 TFLOP/s of f32 are 755 of bf16.
-//   f32, 17 x 256 -> 2 x 512, forward: 7 us, of which launching and one pass through memory are nearly all.
+//   bf16, 65536 x 256 -> 2 x 1024: forward 121 us (568 TFLOP/s, h and x are 170 MB of it), first of the backward 178 us (it
+//   writes D, 268 MB, and reads dh, 134 MB), dx 85 us (809 TFLOP/s), dW 90 us (764 TFLOP/s), sums 13 us.  Bound by what a CU
+//   draws from L2 (about 10 TB/s over the chip: each row of x goes to 16 column tiles), the two first ones by that and by memory.
+//   f32, 3600 x 256 -> 2 x 1024: 30, 36, 32, 32 and 11 us; six plane products each: 118 to 124 TFLOP/s of f32 are 710 to 743 of
+//   bf16.
+//   f16, 5003 x 204 -> 2 x 530: 14 us and 3 for the copies of odd rows, then 10 (gated_max_kernel), 18, 13, 14 and 8 us.
+//   f32, 17 x 256 -> 2 x 512, forward: 8 us: a chain of eight steps in 16 workgroups.
 #include <type_traits>
 
 #include "gemm_tile.hpp"
