@@ -257,6 +257,11 @@ __device__ __forceinline__ f32x4 buffer_load(i32x4 buf, uint32_t off) {
         __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)(uint32_t)buf[0] | (uint64_t)(uint32_t)buf[1] << 32), 0, buf[2], buf[3]),
         (int)off, 0, 0));
 }
+__device__ __forceinline__ float buffer_load1(i32x4 buf, uint32_t off) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+        __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)(uint32_t)buf[0] | (uint64_t)(uint32_t)buf[1] << 32), 0, buf[2], buf[3]),
+        (int)off, 0, 0));
+}
 __device__ __forceinline__ void dma_load(i32x4 buf, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :

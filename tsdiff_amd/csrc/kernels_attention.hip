@@ -819,10 +819,17 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                         const int which = STATS == 2 ? w : wave & 1;
                         dma_load4(dma_buffer((which ? delta : lse) + stat0 + first), off, at_lds + buf * BUF + STAT + which * 256);
                     }
-                } else if (threadIdx.x < 2 * RT) {
+                } else {
+                    // Without a branch: at the join behind one the compiler has put a register away while the lanes that stay
+                    // out of it were still switched off (tools/check_spills.py).
                     static_assert(NT >= 2 * RT, "a thread a value");
                     const int r = threadIdx.x % RT;
-                    stat_reg = open >> r & 1 ? (threadIdx.x / RT ? delta : lse)[stat0 + stat_at(i * RT + r)] : 0.f;
+                    const int64_t first = stat_at(i * RT);
+                    const uint32_t gone = (uint32_t)(~open >> r) << 31;  // DMA_NOWHERE and beyond
+                    const uint32_t off = (uint32_t)((stat_at(i * RT + r) - first) * 4) | gone;
+                    const float l = buffer_load1(dma_buffer(lse + stat0 + first), off);
+                    const float del = buffer_load1(dma_buffer(delta + stat0 + first), off);
+                    stat_reg = threadIdx.x / RT & 1 ? del : l;
                 }
             },
             [&](int buf) {
