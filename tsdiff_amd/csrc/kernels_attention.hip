@@ -143,6 +143,14 @@ template <class T> struct Rows {
         return __ballot(lane < ROWS && has(r0 + lane));
     }
 };
+// Is exactly one key open (the same in every lane)?  Its weight is then 1 whatever its score, dS = 0, and what is left of
+// dP - delta in 24 bits is no gradient: dQ and dK are their sums times 0 (a NaN stays one).
+template <class T> __device__ __forceinline__ bool one_open(const Rows<T>& s) {
+    if (s.mask == nullptr) return s.n == 1;
+    int count = 0;
+    for (int r0 = 0; r0 < s.n && count < 2; r0 += 64) count += __popcll(s.template open<64>(r0));
+    return count == 1;
+}
 // Which keys are open, a word a tile, MASK_TILES tiles at a time in LDS: looked up tile by tile, the mask's bytes would be
 // waited for in front of every tile's loads.
 constexpr int MASK_TILES = 128, MASK_BYTES = MASK_TILES * 8;
@@ -679,6 +687,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
         int first, last;
         split_range(kr.n, KT, d.splits, blockIdx.z, &first, &last);
         uint64_t* words = reinterpret_cast<uint64_t*>(lds + att_buffers<T, FAST>() * BUF);
+        int opened = 0;  // open keys of this share
         for (int tb = first; tb < last; tb += MASK_TILES) {
             const int te = tb + MASK_TILES < last ? tb + MASK_TILES : last;
             if (tb > first) lds_barrier();  // the last tiles have been read
@@ -700,6 +709,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                 },
                 [&](int, uint64_t open, int buf) {
                     if (open == 0) return;  // nothing to attend to
+                    opened += __popcll(open);
                     const char* kl = lds + buf * BUF;
                     const char* vl = kl + KTile::BYTES;
 #pragma unroll
@@ -735,12 +745,13 @@ __global__ __launch_bounds__(WAVES * 64) void att_dq_kernel(AttDims d, const T* 
                     }
                 });
         }
+        const float times = opened == 1 && (d.splits == 1 || one_open(kr)) ? 0.f : d.scale;
         if (!mine) continue;
         // a row without an open key has dQ = 0 whatever dO and O hold
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) {
             if constexpr (att_scaled<T>()) acc[t] *= DsScale::inverse(scale.by);
-            const f32x4 r = L == INFINITY ? f32x4{0, 0, 0, 0} : acc[t] * d.scale;
+            const f32x4 r = L == INFINITY ? f32x4{0, 0, 0, 0} : acc[t] * times;
             const int n = d.dim - t * 16 - g * 4;
             if (d.splits > 1)
                 store4(part + (blockIdx.z * (int64_t)d.rows_q * d.heads + at) * d.dim + t * 16 + g * 4, r, n, d.dim % 4 == 0);
@@ -800,9 +811,8 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
         const uint32_t at_lds = lds_offset(lds);
         int tb, te;
         split_range(nrows, RT, d.splits, blockIdx.z, &tb, &te);
-        uint64_t any = 0;
-#pragma unroll
-        for (int i = 0; i < TK; i += 64) any |= kr.template open<(TK < 64 ? TK : 64)>(k0 + i);
+        static_assert(TK <= 64, "a word");
+        const uint64_t any = kr.template open<TK>(k0);
         if (any == 0) te = tb;  // nobody attends to these keys
         over_tiles<2 * Stage::U + STATS, Stage::DMA>(
             tb, te, [&](int i) { return qr.there(i * RT); },
@@ -896,6 +906,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                 }
             });
         const int64_t all = (int64_t)d.rows_k * d.kv_heads;
+        const float times = any != 0 && (any & (any - 1)) == 0 && one_open(kr) ? 0.f : d.scale;
         if (key >= nkeys) continue;
         const int64_t at = (int64_t)(sp.ks + key) * d.kv_heads + hk;
 #pragma unroll
@@ -906,7 +917,7 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                 ak[t] *= DsScale::inverse(scale.by) * 0x1p-15f;
             }
             // a masked key's gradients are 0 whatever the rows that do not read it hold (a lane's sums are one key's)
-            const f32x4 zero = {0, 0, 0, 0}, rk = open_key ? ak[t] * d.scale : zero, rv = open_key ? av[t] : zero;
+            const f32x4 zero = {0, 0, 0, 0}, rk = open_key ? ak[t] * times : zero, rv = open_key ? av[t] : zero;
             if (d.splits > 1) {
                 store4(part + (blockIdx.z * all + at) * d.dim + y, rk, n, d.dim % 4 == 0);
                 store4(part + ((d.splits + blockIdx.z) * all + at) * d.dim + y, rv, n, d.dim % 4 == 0);
