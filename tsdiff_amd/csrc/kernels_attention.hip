@@ -21,8 +21,8 @@
 // as zeros.  Masked and missing keys are zeros in LDS whatever memory holds there, so that no NaN meets a zero weight.
 //
 // Measured (GPU time a launch):
-//   f32, 1024 graphs of 64, 8 heads of 32: forward 78 us (3.5 TB/s of 268 MB), dQ 104 us (3.9 TB/s), dK and dV 117 us
-//   (3.4 TB/s): by memory, and by the six plane products of each f32 one, which take as long.
+//   f32, 1024 graphs of 64, 8 heads of 32: forward 77 us (3.5 TB/s of 268 MB), dQ 105 us (3.8 TB/s), dK and dV 121 us
+//   (3.3 TB/s): by memory, and by the six plane products of each f32 one, which take as long.
 //   bf16, 3 graphs of 1888, 1493 and 2405, 8 heads on 2 key heads of 64, the first closed and a fifth of the others' keys:
 //   forward 56 us, dQ 65 us, dK and dV 80 us: 294, 378 and 412 TFLOP/s of the pairs in open graphs, a quarter to a third of the
 //   pipes' rate: the two open graphs are 490 workgroups of the forward, under two waves a SIMD, and a wave's chain S, maximum,
@@ -832,21 +832,27 @@ __global__ __launch_bounds__(WAVES * 64) void att_dkv_kernel(AttDims d, const T*
                 } else {
                     // Without a branch: at the join behind one the compiler has put a register away while the lanes that stay
                     // out of it were still switched off (tools/check_spills.py).
-                    static_assert(NT >= 2 * RT, "a thread a value");
-                    const int r = threadIdx.x % RT;
+                    // Two waves load one of the two each; one wave loads both (both in each of four waves: dK and dV of 1024 graphs
+                    // of 64, 8 heads of 32, 131 -> 121 us).
+                    static_assert(RT == 32, "half a wave");
+                    const int r = lane % RT;
                     const int64_t first = stat_at(i * RT);
                     const uint32_t gone = (uint32_t)(~open >> r) << 31;  // DMA_NOWHERE and beyond
                     const uint32_t off = (uint32_t)((stat_at(i * RT + r) - first) * 4) | gone;
-                    const float l = buffer_load1(dma_buffer(lse + stat0 + first), off);
-                    const float del = buffer_load1(dma_buffer(delta + stat0 + first), off);
-                    stat_reg = threadIdx.x / RT & 1 ? del : l;
+                    if constexpr (STATS == 1) {
+                        stat_reg = buffer_load1(dma_buffer((wave & 1 ? delta : lse) + stat0 + first), off);
+                    } else {
+                        const float l = buffer_load1(dma_buffer(lse + stat0 + first), off);
+                        const float del = buffer_load1(dma_buffer(delta + stat0 + first), off);
+                        stat_reg = lane / RT ? del : l;
+                    }
                 }
             },
             [&](int buf) {
                 qs.store(lds + buf * BUF);
                 gs.store(lds + buf * BUF + RTile::BYTES);
-                if (!Stage::DMA && threadIdx.x < 2 * RT)
-                    reinterpret_cast<float*>(lds + buf * BUF + STAT)[threadIdx.x / RT * 64 + threadIdx.x % RT] = stat_reg;
+                if (!Stage::DMA && wave < 2)
+                    reinterpret_cast<float*>(lds + buf * BUF + STAT)[STATS == 1 ? threadIdx.x : lane / RT * 64 + lane % RT] = stat_reg;
             },
             [&]() {
                 in_registers<T>(kf);
