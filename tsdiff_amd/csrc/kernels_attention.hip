@@ -21,10 +21,10 @@
 // as zeros.  Masked and missing keys are zeros in LDS whatever memory holds there, so that no NaN meets a zero weight.
 //
 // Measured (GPU time a launch):
-//   f32, 1024 graphs of 64, 8 heads of 32: forward 77 us (3.5 TB/s of 268 MB), dQ 105 us (3.8 TB/s), dK and dV 121 us
-//   (3.3 TB/s): by memory, and by the six plane products of each f32 one, which take as long.
+//   f32, 1024 graphs of 64, 8 heads of 32: forward 77 us (3.5 TB/s of 268 MB), dQ 104 us (3.9 TB/s), dK and dV 120 us
+//   (3.4 TB/s): by memory, and by the six plane products of each f32 one, which take as long.
 //   bf16, 3 graphs of 1888, 1493 and 2405, 8 heads on 2 key heads of 64, the first closed and a fifth of the others' keys:
-//   forward 56 us, dQ 65 us, dK and dV 80 us: 294, 378 and 412 TFLOP/s of the pairs in open graphs, a quarter to a third of the
+//   forward 57 us, dQ 67 us, dK and dV 81 us: 286, 367 and 407 TFLOP/s of the pairs in open graphs, a quarter to a third of the
 //   pipes' rate: the two open graphs are 490 workgroups of the forward, under two waves a SIMD, and a wave's chain S, maximum,
 //   exp2, P V has nothing of the next tile to work on while it waits.
 //   f16, 8 graphs of 2000 .. 8192, one query, 8 heads of 64: 20 us (3.5 TB/s of the keys and values that are read) and 4 us to
